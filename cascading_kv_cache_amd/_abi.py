@@ -104,6 +104,21 @@ class DenseBwdArgs(C.Structure):
     ]
 
 
+class NormRotateArgs(C.Structure):
+    _fields_ = [
+        ("q", VP), ("q_stride", I64 * 4), ("k", VP), ("k_stride", I64 * 4),
+        ("q_weight", VP), ("k_weight", VP),
+        ("positions", VP), ("pos_stride", I64), ("inv_freq", VP),
+        ("q_out", VP), ("q_out_stride", I64 * 4), ("k_out", VP), ("k_out_stride", I64 * 4),
+        ("q_grad", VP), ("q_grad_stride", I64 * 4), ("k_grad", VP), ("k_grad_stride", I64 * 4),
+        ("dq", VP), ("dq_stride", I64 * 4), ("dk", VP), ("dk_stride", I64 * 4),
+        ("dq_weight", VP), ("dk_weight", VP),
+        ("B", I64), ("H", I64), ("KVH", I64), ("n", I64), ("D", I64), ("rot", I64),
+        ("eps", C.c_float), ("dtype", C.c_int32),
+        ("workspace", VP), ("workspace_bytes", I64),
+    ]
+
+
 def set_strides(field, tensor_or_strides):
     strides = tensor_or_strides.stride() if hasattr(tensor_or_strides, "stride") else tensor_or_strides
     assert len(strides) == len(field), (len(strides), len(field))
@@ -252,6 +267,20 @@ def lib():
         L.ckv_dense_bwd_key_order_bytes.restype = I64
         L.ckv_dense_bwd_split_bytes.argtypes = [I64, I64, I64, I64, I64, C.c_int32]
         L.ckv_dense_bwd_split_bytes.restype = I64
+        L.ckv_norm_rotate.argtypes = [C.POINTER(NormRotateArgs), VP]
+        L.ckv_norm_rotate.restype = C.c_int
+        L.ckv_norm_rotate_bwd.argtypes = [C.POINTER(NormRotateArgs), VP]
+        L.ckv_norm_rotate_bwd.restype = C.c_int
+        L.ckv_norm_rotate_workspace_bytes.argtypes = [I64]
+        L.ckv_norm_rotate_workspace_bytes.restype = I64
+        L.ckv_gated_linear_workspace_bytes.argtypes = [I64, I64, I64, C.c_int32]
+        L.ckv_gated_linear_workspace_bytes.restype = I64
+        L.ckv_gated_linear.argtypes = [VP, VP, VP, VP, I64, I64, I64, I64, C.c_int32, VP, I64, VP]
+        L.ckv_gated_linear.restype = C.c_int
+        L.ckv_gated_linear_bwd_workspace_bytes.argtypes = [I64, I64, I64, C.c_int32]
+        L.ckv_gated_linear_bwd_workspace_bytes.restype = I64
+        L.ckv_gated_linear_bwd.argtypes = [VP, VP, VP, VP, VP, VP, I64, I64, I64, I64, C.c_int32, VP, I64, VP]
+        L.ckv_gated_linear_bwd.restype = C.c_int
         L.ckv_chunk_positions.argtypes = [C.c_void_p, I64, I64, C.c_void_p, I64, I64, C.c_void_p, C.c_void_p]
         L.ckv_chunk_positions.restype = C.c_int
         L.ckv_profile_enable.argtypes = [C.c_int]

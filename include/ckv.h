@@ -333,6 +333,71 @@ int ckv_linear_rows(const void* x, const void* w, const void* bias, const void* 
                     void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * RMSNorm of every head's query and key rows over the head dims and the half rotation of the rows at their tokens'
+ * positions, in one pass (the reference rotates in its mixin, cascade_attention.py:343-353, and has no norm there):
+ *   y = x / sqrt(mean(x^2) + eps) * weight;  with weights NULL (both) y = x
+ *   out[j] = y[j] cos - y[j + rot/2] sin,  out[j + rot/2] = y[j + rot/2] cos + y[j] sin  for j < rot/2, the rest as it is;
+ *   angle = position * inv_freq[j], of the exact product; rot 0: norm alone.
+ * float32 throughout, rounded once.  Any strides but along the head dims (1); outputs may not overlap inputs.
+ * head_dim up to 256.  ckv_norm_rotate_bwd takes the same arguments and the gradients of the outputs instead of the
+ * outputs, and writes those of q, k and the weights (summed in a fixed order).
+ * ---------------------------------------------------------------------------------------- */
+typedef struct ckv_norm_rotate_args {
+    const void* q;                 /* (B, H, n, D)                                        */
+    int64_t q_stride[4];
+    const void* k;                 /* (B, KVH, n, D)                                      */
+    int64_t k_stride[4];
+    const void* q_weight;          /* (D,) or NULL, contiguous, dtype of q                */
+    const void* k_weight;          /* (D,) or NULL                                        */
+    const int64_t* positions;      /* (n,), or (B, n) with pos_stride between the rows    */
+    int64_t pos_stride;            /* 0: one row for all                                  */
+    const float* inv_freq;         /* (rot / 2,)                                          */
+
+    void* q_out;                   /* forward: (B, H, n, D)                               */
+    int64_t q_out_stride[4];
+    void* k_out;                   /* forward: (B, KVH, n, D)                             */
+    int64_t k_out_stride[4];
+
+    const void* q_grad;            /* backward: gradient of q_out                         */
+    int64_t q_grad_stride[4];
+    const void* k_grad;
+    int64_t k_grad_stride[4];
+    void* dq;                      /* backward: gradient of q                             */
+    int64_t dq_stride[4];
+    void* dk;
+    int64_t dk_stride[4];
+    void* dq_weight;               /* backward: (D,), with weights                        */
+    void* dk_weight;
+
+    int64_t B, H, KVH, n, D, rot;
+    float eps;
+    int32_t dtype;
+    void* workspace;               /* backward with weights                               */
+    int64_t workspace_bytes;
+} ckv_norm_rotate_args;
+
+int64_t ckv_norm_rotate_workspace_bytes(int64_t D);
+int ckv_norm_rotate(const ckv_norm_rotate_args* args, void* stream);
+int ckv_norm_rotate_bwd(const ckv_norm_rotate_args* args, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * out (rows, inter) = silu(x Wg^T) * (x Wu^T), the two projections of a gated MLP, the activation and the product in one
+ * call: x (rows, k), rows x_stride >= k elements apart, w (2 inter, k) contiguous: gate rows, then up rows.  float32
+ * throughout, rounded once (ckv_linear_rows with `gated` and ckv_gated_silu round the projections and the activation too).
+ * `gate_up` (rows, 2 inter), optional: the projections, rounded, as the backward pass takes them.  Everything but x
+ * contiguous.  The backward pass writes dx (rows, k) and dw (2 inter, k), either of which may be NULL; it rounds the
+ * gradients of the projections to the tensor dtype for its two products, whose sums are float32.  Sums are added up in a
+ * fixed order.  The workspace sizes are those of a call on the current device.
+ * ---------------------------------------------------------------------------------------- */
+int64_t ckv_gated_linear_workspace_bytes(int64_t rows, int64_t inter, int64_t k, int32_t dtype);
+int ckv_gated_linear(const void* x, const void* w, void* out, void* gate_up, int64_t rows, int64_t inter, int64_t k, int64_t x_stride,
+                     int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t ckv_gated_linear_bwd_workspace_bytes(int64_t rows, int64_t inter, int64_t k, int32_t dtype);
+int ckv_gated_linear_bwd(const void* x, const void* w, const void* gate_up, const void* dout, void* dx, void* dw, int64_t rows,
+                         int64_t inter, int64_t k, int64_t x_stride, int32_t dtype, void* workspace, int64_t workspace_bytes,
+                         void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Stage timing (the reference's BENCHMARK=True switch, cascading_cache.py:986-1026, extended to
  * every kernel stage).  While enabled, each stage of ckv_attn / ckv_update is bracketed by HIP
  * events on the caller's stream; ckv_profile_read waits for them, ADDS the elapsed milliseconds
