@@ -1,0 +1,411 @@
+// The first half of a gated MLP, h = silu(x Wg^T) * (x Wu^T), and its gradients.
+//
+//   g = x Wg^T, u = x Wu^T, h = g s(g) u             s the logistic function
+//   dg = dh u s (1 + g (1 - s)),  du = dh g s,        dx = [dg du] [Wg; Wu],  dW = [dg du]^T x
+//
+// Three matrix products, of one kind: C (M, N) = sum over k of A (m, k) B (n, k), where an operand's elements are adjacent along k (x and W of
+// the forward pass, [dg du] of dx) or along its rows (W of dx, both operands of dW).  With the gate, a tile of C has as many gate columns as
+// up columns, the same ones, and a wavefront holds both: g and u meet in registers, and C itself is written only for the backward pass.
+#include "ckv_common.h"
+
+#include <algorithm>
+
+namespace ckv {
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+struct Operand {
+    const void* p;
+    int64_t rows;      // M or N
+    int64_t stride;    // between rows (along_k) or between the elements of a row, which are k steps apart
+};
+
+struct ProductParams {
+    Operand a, b;
+    void* out;          // (M, N) contiguous, or the gated (M, N / 2)
+    void* both;         // gated, optional: (M, N), gate and up columns
+    float* partial;     // (splits, M, N) where the sums are shared out, else null
+    int64_t M, N, K;
+    int64_t k_share;    // k steps a share
+    int tiles_m, tiles_n;
+    bool a_vectors, b_vectors;   // rows of whole, aligned pieces of 16 bytes
+};
+
+enum Epilogue { kStore, kGate };
+
+__device__ inline float gate_product(float g, float u) { return g / (1.f + expf(-g)) * u; }
+
+// Tiles go round the eight XCDs: each gets a stretch of them, eight tiles of M high, so that the tiles of a stretch that run at a time share
+// operands in its L2.
+__device__ inline void tile_of(const ProductParams& p, int& tm, int& tn) {
+    const int all = p.tiles_m * p.tiles_n, xcd = blockIdx.x % 8, many = all / 8, over = all % 8;
+    const int tile = xcd * many + min(xcd, over) + blockIdx.x / 8;
+    constexpr int kHigh = 8;
+    const int band = tile / (kHigh * p.tiles_n), in = tile - band * kHigh * p.tiles_n;
+    const int high = min(kHigh, p.tiles_m - band * kHigh);
+    tm = band * kHigh + in % high;
+    tn = in / high;
+}
+
+// ---- any type, stride and size: float32 products on v_mfma_f32_32x32x2 -----------------------------------------------------------------
+
+constexpr int kTile = 128, kStep = 16, kPitch = kTile + 4;
+
+// A thread's eight elements of a tile of 128 rows and 16 steps: along k of one row, or along the rows of one step.
+template <typename T, bool kAlongK>
+struct Piece {
+    int row, step;   // of the first
+    float v[8];
+    __device__ Piece() {
+        row = kAlongK ? threadIdx.x >> 1 : (threadIdx.x & 15) * 8;
+        step = kAlongK ? (threadIdx.x & 1) * 8 : threadIdx.x >> 4;
+    }
+    // base: the operand's row 0; `first` the tile's first row, counted from base; rows behind `rows` and steps behind `end` are zeros
+    __device__ void load(const T* base, int64_t stride, int64_t first, int64_t rows, int64_t k, int64_t end, bool vectors) {
+        const int64_t r = first + row, s = k + step;
+        const T* at = base + (kAlongK ? r * stride + s : s * stride + r);
+        const bool whole = kAlongK ? r < rows && s + 8 <= end : s < end && r + 8 <= rows;
+        if (vectors && whole) {
+            struct alignas(16) Sixteen {
+                T v[16 / sizeof(T)];
+            };
+            constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+            for (int i = 0; i < 8 / kPer; i++) {
+                const Sixteen x = reinterpret_cast<const Sixteen*>(at)[i];
+#pragma unroll
+                for (int e = 0; e < kPer; e++) v[i * kPer + e] = Elem<T>::to_float(x.v[e]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const bool there = kAlongK ? r < rows && s + i < end : s < end && r + i < rows;
+                v[i] = there ? Elem<T>::to_float(at[i]) : 0.f;
+            }
+        }
+    }
+    __device__ void store(float (*tile)[kPitch], int row_in_tile) const {
+        if constexpr (kAlongK) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) tile[step + i][row_in_tile] = v[i];
+        } else {
+            float4* to = reinterpret_cast<float4*>(&tile[step][row_in_tile]);
+            to[0] = make_float4(v[0], v[1], v[2], v[3]);
+            to[1] = make_float4(v[4], v[5], v[6], v[7]);
+        }
+    }
+};
+
+template <typename T, bool kAlongKA, bool kAlongKB, Epilogue kEpilogue>
+__global__ void __launch_bounds__(256) product_kernel(ProductParams p) {
+    __shared__ __align__(16) float as[2][kStep][kPitch], bs[2][kStep][kPitch];
+    int tm, tn;
+    tile_of(p, tm, tn);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1, half = lane >> 5, l = lane & 31;
+    constexpr bool kGated = kEpilogue == kGate;
+    const int64_t inter = p.N / 2;
+    const int64_t m0 = (int64_t)tm * kTile, n0 = (int64_t)tn * (kGated ? kTile / 2 : kTile);
+    const int64_t k0 = blockIdx.y * p.k_share, k1 = min(p.K, k0 + p.k_share);
+    Piece<T, kAlongKA> pa;
+    Piece<T, kAlongKB> pb;
+    const T* a = (const T*)p.a.p;
+    const T* b = (const T*)p.b.p;
+    // gated: rows 0..63 of B's tile are gate rows, 64..127 up rows
+    const bool up = kGated && pb.row >= kTile / 2;
+    auto load = [&](int64_t k) {
+        pa.load(a, p.a.stride, m0, p.M, k, k1, p.a_vectors);
+        if constexpr (kGated) pb.load(b + (up ? inter * p.b.stride : 0), p.b.stride, n0 - (up ? kTile / 2 : 0), inter, k, k1, p.b_vectors);
+        else pb.load(b, p.b.stride, n0, p.N, k, k1, p.b_vectors);
+    };
+    auto store = [&](int at) {
+        pa.store(as[at], pa.row);
+        pb.store(bs[at], pb.row);
+    };
+    f32x16 acc[2][2] = {};
+    load(k0);
+    store(0);
+    __syncthreads();
+    int at = 0;
+    for (int64_t k = k0; k < k1; k += kStep) {
+        const bool more = k + kStep < k1;
+        if (more) load(k + kStep);
+#pragma unroll
+        for (int s = 0; s < kStep; s += 2) {
+            float av[2], bv[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                av[i] = as[at][s + half][wm * 64 + i * 32 + l];
+                bv[i] = bs[at][s + half][kGated ? i * 64 + wn * 32 + l : wn * 64 + i * 32 + l];
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(av[i], bv[j], acc[i][j], 0, 0, 0);
+        }
+        if (more) store(at ^ 1);
+        __syncthreads();
+        at ^= 1;
+    }
+    // element r of an accumulator: row 8 (r / 4) + 4 half + r % 4, column l
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            const int64_t m = m0 + wm * 64 + i * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
+            if (m >= p.M) continue;
+            if constexpr (kGated) {
+                const int64_t n = n0 + wn * 32 + l;
+                if (n >= inter) continue;
+                const float g = acc[i][0][r], u = acc[i][1][r];
+                if (p.partial) {
+                    float* to = p.partial + (blockIdx.y * p.M + m) * p.N + n;
+                    to[0] = g;
+                    to[inter] = u;
+                    continue;
+                }
+                ((T*)p.out)[m * inter + n] = Elem<T>::from_float(gate_product(g, u));
+                if (p.both) {
+                    T* to = (T*)p.both + m * p.N + n;
+                    to[0] = Elem<T>::from_float(g);
+                    to[inter] = Elem<T>::from_float(u);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const int64_t n = n0 + wn * 64 + j * 32 + l;
+                    if (n >= p.N) continue;
+                    if (p.partial) p.partial[(blockIdx.y * p.M + m) * p.N + n] = acc[i][j][r];
+                    else ((T*)p.out)[m * p.N + n] = Elem<T>::from_float(acc[i][j][r]);
+                }
+            }
+        }
+}
+
+// Sums of the shares, in their order, and what the product's own epilogue does.
+template <typename T, Epilogue kEpilogue>
+__global__ void __launch_bounds__(256) merge_kernel(ProductParams p, int shares) {
+    constexpr bool kGated = kEpilogue == kGate;
+    const int64_t cols = kGated ? p.N / 2 : p.N, all = p.M * cols, share = p.M * p.N;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+        int64_t n;
+        const int64_t m = div_index(i, cols, n);
+        const float* from = p.partial + m * p.N + n;
+        float g = 0.f, u = 0.f;
+        for (int s = 0; s < shares; s++) {
+            g += from[s * share];
+            if constexpr (kGated) u += from[s * share + cols];
+        }
+        if constexpr (kGated) {
+            ((T*)p.out)[i] = Elem<T>::from_float(gate_product(g, u));
+            if (p.both) {
+                T* to = (T*)p.both + m * p.N + n;
+                to[0] = Elem<T>::from_float(g);
+                to[cols] = Elem<T>::from_float(u);
+            }
+        } else {
+            ((T*)p.out)[i] = Elem<T>::from_float(g);
+        }
+    }
+}
+
+// ---- gradients of the projections ------------------------------------------------------------------------------------------------------
+
+template <typename T, int kPer>
+__global__ void __launch_bounds__(256) gate_gradient_kernel(const T* gate_up, const T* dout, T* grad, int64_t rows, int64_t inter) {
+    struct alignas(sizeof(T) * kPer) Piece {
+        T v[kPer];
+    };
+    const int64_t pieces = inter / kPer, all = rows * pieces;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+        int64_t c;
+        const int64_t row = div_index(i, pieces, c);
+        const T* from = gate_up + row * 2 * inter + c * kPer;
+        const Piece gate = *reinterpret_cast<const Piece*>(from), up = *reinterpret_cast<const Piece*>(from + inter);
+        const Piece dh = *reinterpret_cast<const Piece*>(dout + row * inter + c * kPer);
+        Piece dg, du;
+#pragma unroll
+        for (int e = 0; e < kPer; e++) {
+            const float g = Elem<T>::to_float(gate.v[e]), u = Elem<T>::to_float(up.v[e]), d = Elem<T>::to_float(dh.v[e]);
+            const float s = 1.f / (1.f + expf(-g));
+            dg.v[e] = Elem<T>::from_float(d * u * s * (1.f + g * (1.f - s)));
+            du.v[e] = Elem<T>::from_float(d * g * s);
+        }
+        T* to = grad + row * 2 * inter + c * kPer;
+        *reinterpret_cast<Piece*>(to) = dg;
+        *reinterpret_cast<Piece*>(to + inter) = du;
+    }
+}
+
+template <typename T>
+int gate_gradient(const void* gate_up, const void* dout, void* grad, int64_t rows, int64_t inter, hipStream_t stream) {
+    constexpr int kPer = 16 / (int)sizeof(T);
+    const bool pieces = inter % kPer == 0 &&
+                        ((reinterpret_cast<uintptr_t>(gate_up) | reinterpret_cast<uintptr_t>(dout) | reinterpret_cast<uintptr_t>(grad)) & 15) == 0;
+    const int64_t all = rows * inter / (pieces ? kPer : 1);
+    const unsigned blocks = (unsigned)std::min<int64_t>((all + 255) / 256, 256 * 16);
+    if (pieces) hipLaunchKernelGGL((gate_gradient_kernel<T, kPer>), dim3(blocks), dim3(256), 0, stream, (const T*)gate_up, (const T*)dout, (T*)grad, rows, inter);
+    else hipLaunchKernelGGL((gate_gradient_kernel<T, 1>), dim3(blocks), dim3(256), 0, stream, (const T*)gate_up, (const T*)dout, (T*)grad, rows, inter);
+    CKV_HIP_TRY(hipGetLastError());
+    return CKV_OK;
+}
+
+// ---- which kernel, how many shares -----------------------------------------------------------------------------------------------------
+
+struct Plan {
+    int64_t k_share;
+    int shares, tiles_m, tiles_n;
+    int64_t bytes;   // of the shares' sums
+};
+
+// Where the tiles leave compute units idle, the steps are shared out over as many workgroups as come to one each, none with fewer than 256.
+Plan plan_product(int64_t M, int64_t N, int64_t K, bool gated, int cus) {
+    Plan r;
+    r.tiles_m = (int)((M + kTile - 1) / kTile);
+    r.tiles_n = (int)((N + kTile - 1) / kTile);
+    if (gated) r.tiles_n = (int)((N / 2 + kTile / 2 - 1) / (kTile / 2));
+    const int64_t tiles = (int64_t)r.tiles_m * r.tiles_n;
+    const int64_t shares = std::max<int64_t>(1, std::min<int64_t>(cus / tiles, K / 256));
+    r.k_share = ((K + shares - 1) / shares + kStep - 1) / kStep * kStep;
+    r.shares = (int)((K + r.k_share - 1) / r.k_share);
+    r.bytes = r.shares > 1 ? r.shares * M * N * 4 : 0;
+    return r;
+}
+
+template <typename T, bool kAlongKA, bool kAlongKB, Epilogue kEpilogue>
+int run_product(ProductParams& p, const DeviceInfo& di, void* workspace, int64_t bytes, hipStream_t stream) {
+    const Plan plan = plan_product(p.M, p.N, p.K, kEpilogue == kGate, di.cus);
+    if (plan.bytes > bytes || (plan.bytes && !workspace)) return CKV_ERR_WORKSPACE;
+    if ((int64_t)plan.tiles_m * plan.tiles_n > 0x7fffffff) return CKV_ERR_UNSUPPORTED;
+    auto vectors = [](const Operand& o) { return reinterpret_cast<uintptr_t>(o.p) % 16 == 0 && o.stride % (16 / (int64_t)sizeof(T)) == 0; };
+    p.a_vectors = vectors(p.a);
+    p.b_vectors = vectors(p.b) && (kEpilogue != kGate || kAlongKB);
+    p.tiles_m = plan.tiles_m;
+    p.tiles_n = plan.tiles_n;
+    p.k_share = plan.k_share;
+    p.partial = plan.shares > 1 ? (float*)workspace : nullptr;
+    hipLaunchKernelGGL((product_kernel<T, kAlongKA, kAlongKB, kEpilogue>), dim3(plan.tiles_m * plan.tiles_n, plan.shares), dim3(256), 0, stream, p);
+    CKV_HIP_TRY(hipGetLastError());
+    if (p.partial) {
+        const int64_t all = p.M * (kEpilogue == kGate ? p.N / 2 : p.N);
+        hipLaunchKernelGGL((merge_kernel<T, kEpilogue>), dim3((unsigned)std::min<int64_t>((all + 255) / 256, 256 * 16)), dim3(256), 0, stream, p, plan.shares);
+        CKV_HIP_TRY(hipGetLastError());
+    }
+    return CKV_OK;
+}
+
+int check_sizes(int64_t rows, int64_t inter, int64_t k, int64_t x_stride, int32_t dtype) {
+    if (dtype != CKV_F32 && dtype != CKV_F16 && dtype != CKV_BF16) return CKV_ERR_DTYPE;
+    if (rows < 0 || inter <= 0 || k <= 0 || x_stride < k) return CKV_ERR_SHAPE;
+    if (rows > 0x7fffffff || inter > 0x3fffffff || k > 0x7fffffff) return CKV_ERR_UNSUPPORTED;
+    return CKV_OK;
+}
+
+template <typename T>
+int run_forward(const void* x, const void* w, void* out, void* gate_up, int64_t rows, int64_t inter, int64_t k, int64_t x_stride, void* workspace,
+                int64_t bytes, const DeviceInfo& di, hipStream_t stream) {
+    ProductParams p = {};
+    p.a = Operand{x, rows, x_stride};
+    p.b = Operand{w, 2 * inter, k};
+    p.out = out;
+    p.both = gate_up;
+    p.M = rows;
+    p.N = 2 * inter;
+    p.K = k;
+    return run_product<T, true, true, kGate>(p, di, workspace, bytes, stream);
+}
+
+template <typename T>
+int run_backward(const void* x, const void* w, const void* gate_up, const void* dout, void* dx, void* dw, int64_t rows, int64_t inter, int64_t k,
+                 int64_t x_stride, char* workspace, int64_t bytes, const DeviceInfo& di, hipStream_t stream) {
+    const int64_t grad_bytes = align_up(rows * 2 * inter * (int64_t)sizeof(T), 256);
+    void* grad = workspace;
+    if (int rc = gate_gradient<T>(gate_up, dout, grad, rows, inter, stream)) return rc;
+    workspace += grad_bytes;
+    bytes -= grad_bytes;
+    if (dx) {
+        ProductParams p = {};
+        p.a = Operand{grad, rows, 2 * inter};
+        p.b = Operand{w, k, k};
+        p.out = dx;
+        p.M = rows;
+        p.N = k;
+        p.K = 2 * inter;
+        if (int rc = run_product<T, true, false, kStore>(p, di, workspace, bytes, stream)) return rc;
+    }
+    if (dw) {
+        ProductParams p = {};
+        p.a = Operand{grad, 2 * inter, 2 * inter};
+        p.b = Operand{x, k, x_stride};
+        p.out = dw;
+        p.M = 2 * inter;
+        p.N = k;
+        p.K = rows;
+        if (int rc = run_product<T, false, false, kStore>(p, di, workspace, bytes, stream)) return rc;
+    }
+    return CKV_OK;
+}
+
+// A weight without rows to learn from: zeros, by a kernel (a recorded memset is no good).
+__global__ void __launch_bounds__(256) zero_kernel(uint16_t* p, int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = 0;
+}
+
+}  // namespace
+}  // namespace ckv
+
+extern "C" int64_t ckv_gated_linear_workspace_bytes(int64_t rows, int64_t inter, int64_t k, int32_t dtype) {
+    using namespace ckv;
+    DeviceInfo di;
+    if (check_sizes(rows, inter, k, k, dtype) || rows == 0 || current_device_info(&di)) return 0;
+    return plan_product(rows, 2 * inter, k, true, di.cus).bytes;
+}
+
+extern "C" int ckv_gated_linear(const void* x, const void* w, void* out, void* gate_up, int64_t rows, int64_t inter, int64_t k, int64_t x_stride,
+                                int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream_) {
+    using namespace ckv;
+    if (int rc = check_sizes(rows, inter, k, x_stride, dtype)) return rc;
+    if (rows == 0) return CKV_OK;
+    if (!x || !w || !out) return CKV_ERR_NULL;
+    DeviceInfo di;
+    if (int rc = current_device_info(&di)) return rc;
+    hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+    switch (dtype) {
+        case CKV_F32: return run_forward<float>(x, w, out, gate_up, rows, inter, k, x_stride, workspace, workspace_bytes, di, stream);
+        case CKV_F16: return run_forward<__half>(x, w, out, gate_up, rows, inter, k, x_stride, workspace, workspace_bytes, di, stream);
+        default: return run_forward<__hip_bfloat16>(x, w, out, gate_up, rows, inter, k, x_stride, workspace, workspace_bytes, di, stream);
+    }
+}
+
+extern "C" int64_t ckv_gated_linear_bwd_workspace_bytes(int64_t rows, int64_t inter, int64_t k, int32_t dtype) {
+    using namespace ckv;
+    DeviceInfo di;
+    if (check_sizes(rows, inter, k, k, dtype) || rows == 0 || current_device_info(&di)) return 0;
+    const int64_t dx = plan_product(rows, k, 2 * inter, false, di.cus).bytes, dw = plan_product(2 * inter, k, rows, false, di.cus).bytes;
+    return align_up(rows * 2 * inter * elem_bytes(dtype), 256) + std::max(dx, dw);
+}
+
+extern "C" int ckv_gated_linear_bwd(const void* x, const void* w, const void* gate_up, const void* dout, void* dx, void* dw, int64_t rows,
+                                    int64_t inter, int64_t k, int64_t x_stride, int32_t dtype, void* workspace, int64_t workspace_bytes,
+                                    void* stream_) {
+    using namespace ckv;
+    if (int rc = check_sizes(rows, inter, k, x_stride, dtype)) return rc;
+    if (!dx && !dw) return CKV_OK;
+    hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+    if (rows == 0) {
+        if (!dw) return CKV_OK;
+        hipLaunchKernelGGL(zero_kernel, dim3(2048), dim3(256), 0, stream, (uint16_t*)dw, 2 * inter * k * elem_bytes(dtype) / 2);
+        CKV_HIP_TRY(hipGetLastError());
+        return CKV_OK;
+    }
+    if (!x || !w || !gate_up || !dout) return CKV_ERR_NULL;
+    DeviceInfo di;
+    if (int rc = current_device_info(&di)) return rc;
+    if (!workspace || workspace_bytes < align_up(rows * 2 * inter * elem_bytes(dtype), 256)) return CKV_ERR_WORKSPACE;
+    char* ws = (char*)workspace;
+    switch (dtype) {
+        case CKV_F32: return run_backward<float>(x, w, gate_up, dout, dx, dw, rows, inter, k, x_stride, ws, workspace_bytes, di, stream);
+        case CKV_F16: return run_backward<__half>(x, w, gate_up, dout, dx, dw, rows, inter, k, x_stride, ws, workspace_bytes, di, stream);
+        default: return run_backward<__hip_bfloat16>(x, w, gate_up, dout, dx, dw, rows, inter, k, x_stride, ws, workspace_bytes, di, stream);
+    }
+}
