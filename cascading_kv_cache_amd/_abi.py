@@ -119,6 +119,17 @@ class NormRotateArgs(C.Structure):
     ]
 
 
+class SampleArgs(C.Structure):
+    _fields_ = [
+        ("logits", VP), ("logit_stride", I64), ("uniforms", VP),
+        ("temperatures", VP), ("top_ks", VP), ("top_ps", VP), ("min_ps", VP),
+        ("temperature", C.c_double), ("top_p", C.c_double), ("min_p", C.c_double), ("top_k", I64),
+        ("tokens", VP), ("logprobs", VP),
+        ("rows", I64), ("vocab", I64), ("dtype", C.c_int32), ("reserved", C.c_int32),
+        ("workspace", VP), ("workspace_bytes", I64),
+    ]
+
+
 def set_strides(field, tensor_or_strides):
     strides = tensor_or_strides.stride() if hasattr(tensor_or_strides, "stride") else tensor_or_strides
     assert len(strides) == len(field), (len(strides), len(field))
@@ -281,6 +292,10 @@ def lib():
         L.ckv_gated_linear_bwd_workspace_bytes.restype = I64
         L.ckv_gated_linear_bwd.argtypes = [VP, VP, VP, VP, VP, VP, I64, I64, I64, I64, C.c_int32, VP, I64, VP]
         L.ckv_gated_linear_bwd.restype = C.c_int
+        L.ckv_sample.argtypes = [C.POINTER(SampleArgs), VP]
+        L.ckv_sample.restype = C.c_int
+        L.ckv_sample_workspace_bytes.argtypes = [I64, I64]
+        L.ckv_sample_workspace_bytes.restype = I64
         L.ckv_chunk_positions.argtypes = [C.c_void_p, I64, I64, C.c_void_p, I64, I64, C.c_void_p, C.c_void_p]
         L.ckv_chunk_positions.restype = C.c_int
         L.ckv_profile_enable.argtypes = [C.c_int]

@@ -243,3 +243,4 @@ extern "C" int64_t ckv_sizeof_attn_args(void) { return (int64_t)sizeof(ckv_attn_
 extern "C" int64_t ckv_sizeof_dense_args(void) { return (int64_t)sizeof(ckv_dense_args); }
 extern "C" int64_t ckv_sizeof_dense_bwd_args(void) { return (int64_t)sizeof(ckv_dense_bwd_args); }
 extern "C" int64_t ckv_sizeof_norm_rotate_args(void) { return (int64_t)sizeof(ckv_norm_rotate_args); }
+extern "C" int64_t ckv_sizeof_sample_args(void) { return (int64_t)sizeof(ckv_sample_args); }

@@ -398,6 +398,39 @@ int ckv_gated_linear_bwd(const void* x, const void* w, const void* gate_up, cons
                          void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * A token a row from logits, with given random numbers (the reference's generation loop takes the largest logit,
+ * cascade_attention.py:473-499).  Order: falling logits, equal ones by rising index; w = exp((logit - largest) / temperature).
+ * Kept are the first top_k; of those what has less than top_p of their mass in front of it; of those what has w >= min_p;
+ * and the first one in any case.  The token is the first whose running kept mass exceeds uniform * kept mass; logprob is the
+ * logarithm of its share of the kept mass.  Settings are numbers for all rows or arrays with one a row.  temperature that is
+ * not above 0: the first one.  top_k <= 0, top_p >= 1, min_p <= 0: no limit; top_p <= 0, min_p >= 1: the first one and (min_p)
+ * its equals.  A uniform at or above 1 takes the last kept token, one below 0 the first.  Logits of NaN and minus infinity
+ * are no tokens, one of plus infinity is the only one besides its equals; a row without tokens gives -1 and NaN.  Masses are
+ * whole numbers of 2^-44 of the first one's: the same call gives the same tokens.  vocab < 2^20.
+ * ---------------------------------------------------------------------------------------- */
+typedef struct ckv_sample_args {
+    const void* logits;            /* (rows, vocab), elements of a row adjacent           */
+    int64_t logit_stride;          /* between rows                                        */
+    const float* uniforms;         /* (rows,) in [0, 1)                                   */
+    const float* temperatures;     /* (rows,) or NULL: `temperature`                      */
+    const int64_t* top_ks;         /* (rows,) or NULL: `top_k`                            */
+    const float* top_ps;           /* (rows,) or NULL: `top_p`                            */
+    const float* min_ps;           /* (rows,) or NULL: `min_p`                            */
+    double temperature, top_p, min_p;
+    int64_t top_k;
+    int64_t* tokens;               /* (rows,)                                             */
+    float* logprobs;               /* (rows,)                                             */
+    int64_t rows, vocab;
+    int32_t dtype, reserved;
+    void* workspace;               /* 16-byte aligned                                     */
+    int64_t workspace_bytes;
+} ckv_sample_args;
+
+/* 0 where rows are many enough for a workgroup each; on the current device */
+int64_t ckv_sample_workspace_bytes(int64_t rows, int64_t vocab);
+int ckv_sample(const ckv_sample_args* args, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Stage timing (the reference's BENCHMARK=True switch, cascading_cache.py:986-1026, extended to
  * every kernel stage).  While enabled, each stage of ckv_attn / ckv_update is bracketed by HIP
  * events on the caller's stream; ckv_profile_read waits for them, ADDS the elapsed milliseconds

@@ -8,6 +8,7 @@ import torch
 from cascading_kv_cache_amd import _abi
 from cascading_kv_cache_amd.feed_forward import gated_feed_forward
 from cascading_kv_cache_amd.norm_rotate import norm_rotate
+from cascading_kv_cache_amd.sampling import sample_tokens
 
 
 @pytest.fixture(scope="module")
@@ -123,3 +124,46 @@ def test_gated_linear_in_c(lib):
     assert backward(x=None) == backward(both=None) == backward(dout=None) == -1
     assert backward(dx=None, dw=None) == 0
     assert lib.ckv_gated_linear_workspace_bytes(0, 4, 8, 0) == lib.ckv_gated_linear_bwd_workspace_bytes(4, 4, 8, 7) == 0
+
+
+@pytest.mark.parametrize("change,error,text", [
+    (dict(logits=torch.zeros(8)), ValueError, "rows, vocab"),
+    (dict(logits=torch.zeros(3, 8)), ValueError, "rows, vocab"),
+    (dict(uniforms=torch.zeros(2, 1)), ValueError, "rows, vocab"),
+    (dict(logits=torch.zeros(2, 0)), ValueError, "to draw from"),
+    (dict(logits=torch.empty(2, 1 << 20, device="meta")), ValueError, "to draw from"),
+    (dict(logits=torch.zeros(2, 8, dtype=torch.float64)), TypeError, "float64"),
+    (dict(uniforms=torch.zeros(2, dtype=torch.float64)), TypeError, "random numbers"),
+    (dict(temperature=float("nan")), ValueError, "temperature"),
+    (dict(top_p=float("nan")), ValueError, "top_p"),
+    (dict(top_k=torch.zeros(2)), TypeError, "top_k"),
+    (dict(min_p=torch.zeros(2, dtype=torch.float64)), TypeError, "min_p"),
+    (dict(temperature=torch.ones(3)), ValueError, "temperature"),
+    (dict(temperature=torch.ones(2, device="meta")), ValueError, "temperature"),
+    (dict(), _abi.CkvError, "no CPU fallback"),
+])
+def test_sample_tokens(change, error, text):
+    args = dict(logits=torch.zeros(2, 8), uniforms=torch.zeros(2))
+    args.update(change)
+    with pytest.raises(error, match=text):
+        sample_tokens(**args)
+
+
+def test_sample_in_c(lib):
+    assert lib.ckv_sample(None, None) == -1
+    a = _abi.SampleArgs()
+    a.dtype = 5
+    assert lib.ckv_sample(C.byref(a), None) == -4
+    a.dtype, a.rows, a.vocab, a.logit_stride = _abi.CKV_F32, 2, 8, 8
+    for name, value, status in (("rows", -1, -2), ("vocab", 0, -2), ("logit_stride", -8, -2), ("vocab", 1 << 20, -6)):
+        was = getattr(a, name)
+        setattr(a, name, value)
+        assert lib.ckv_sample(C.byref(a), None) == status, name
+        setattr(a, name, was)
+    assert lib.ckv_sample(C.byref(a), None) == -1
+    a.rows = 0
+    assert lib.ckv_sample(C.byref(a), None) == 0
+    assert lib.ckv_sample_workspace_bytes(0, 8) == lib.ckv_sample_workspace_bytes(2, 1 << 20) == 0
+    f = C.CDLL(_abi.LIB_PATH).ckv_sizeof_sample_args
+    f.restype = C.c_int64
+    assert f() == C.sizeof(_abi.SampleArgs)
