@@ -5,7 +5,7 @@ strides, then greedy decoding one token at a time (cascade/models/cascade_attent
 The reference patches Hugging Face Llama / Qwen2 models; this module carries just enough of such a
 decoder (embedding, RMSNorm, gated MLP, untied head; projections with optional bias) to run the
 benchmark shapes end to end with random weights.  Attention, scores and the cache are the library's
-(:class:`ProjectedCascadeAttention`), and so are, once the projections are fused, the gate and the products of a decoding step
+(:class:`ProjectedCascadeAttention`), so are the norms of heads, where a model has them, and the drawing of tokens, and so are, once the projections are fused, the gate and the products of a decoding step
 (``row_products.py``); everything else is plain PyTorch.
 
     python -m cascading_kv_cache_amd.decoder --preset llama3.1-8b --layers 4 --prompt 16384 --stride 4096 --new 32
@@ -19,8 +19,10 @@ import torch
 from torch import nn
 
 from .cascading_cache import CascadingKVCache
+from .feed_forward import gated_feed_forward
 from .latency import ProjectedCascadeAttention
 from .row_products import followed as _followed, gated_silu, library_orders, own_methods, plain, product_settings, row_linear
+from .sampling import sample_tokens
 
 
 @dataclass
@@ -36,6 +38,7 @@ class DecoderConfig:
     rms_eps: float = 1e-5
     qkv_bias: bool = False
     head_reduction: str = "max"
+    qk_norm: bool = False   # RMSNorm of every head's queries and keys
 
 
 PRESETS = {
@@ -72,6 +75,8 @@ class GatedMLP(nn.Module):
 
         self._w_gate_up = None
 
+    one_launch = False   # of both projections and the gate, see CascadeDecoder.fuse_projections
+
     def fuse_projections(self):
         """``gate_proj`` and ``up_proj`` as views of one buffer: one matrix product instead of two."""
         with torch.no_grad():
@@ -83,6 +88,8 @@ class GatedMLP(nn.Module):
     def forward(self, x):
         if self._w_gate_up is None:
             return self.down_proj(nn.functional.silu(self.gate_proj(x)) * self.up_proj(x))
+        if self.one_launch and not torch.is_autocast_enabled():
+            return self.down_proj(gated_feed_forward(x, self._w_gate_up))
         return self.down_proj(gated_silu(nn.functional.linear(x, self._w_gate_up)))
 
 
@@ -99,7 +106,7 @@ class DecoderLayer(nn.Module):
         self.self_attn = ProjectedCascadeAttention(cfg.hidden_size, cfg.num_heads, cfg.num_kv_heads, cfg.head_dim,
                                                    rope_theta=cfg.rope_theta, qkv_bias=cfg.qkv_bias,
                                                    head_reduction=cfg.head_reduction, layer_idx=layer_idx, dtype=dtype,
-                                                   device=device)
+                                                   device=device, qk_norm=cfg.qk_norm, norm_eps=cfg.rms_eps)
         self.mlp = GatedMLP(cfg, dtype, device)
         self.input_layernorm = RMSNorm(cfg.hidden_size, cfg.rms_eps, dtype, device)
         self.post_attention_layernorm = RMSNorm(cfg.hidden_size, cfg.rms_eps, dtype, device)
@@ -154,21 +161,24 @@ class CascadeDecoder(nn.Module):
         gen = torch.Generator(device=device if init_on_device else "cpu").manual_seed(seed)
         with torch.no_grad():
             for name, prm in self.named_parameters():
-                if name.endswith("layernorm.weight") or name == "norm.weight":
+                if name.endswith(("layernorm.weight", "_norm_weight")) or name == "norm.weight":
                     continue
                 if init_on_device:
                     prm.normal_(0.0, 0.02, generator=gen)
                 else:
                     prm.copy_((torch.randn(prm.shape, generator=gen) * 0.02).to(dtype))
 
-    def fuse_projections(self):
+    def fuse_projections(self, feed_forward=False):
         """Fewer, larger launches outside attention (same weights, kept in shared buffers): q/k/v and gate/up
         projections as one matrix product each, the norms as one kernel, the products of few rows by the library where they have
         the bits of torch's (which holds for torch's settings as they are now: under others its products are taken).  Off by
-        default: the parity tests compare the plain formulation with the CPU's."""
+        default: the parity tests compare the plain formulation with the CPU's.  ``feed_forward``: the first half of a chunk's MLP is
+        the library's too (:func:`gated_feed_forward`), in float32 up to one rounding: not the bits of torch's operations."""
         for layer in self.layers:
             layer.self_attn.fuse_projections()
             layer.mlp.fuse_projections()
+            if feed_forward:
+                layer.mlp.one_launch = True
             layer.input_layernorm.fused = layer.post_attention_layernorm.fused = True
         self.norm.fused = True
         for layer in self.layers:
@@ -207,15 +217,20 @@ class CascadeDecoder(nn.Module):
 
 
 @torch.no_grad()
-def generate(model, input_ids, cache, stride, max_new_tokens):
-    """Greedy generation as the reference runs it: the prompt goes through in strides of ``stride`` tokens,
-    every later step feeds the last token only (cascade_attention.py:473-499, 527-538)."""
+def generate(model, input_ids, cache, stride, max_new_tokens, sampling=None, generator=None):
+    """Generation as the reference runs it: the prompt goes through in strides of ``stride`` tokens, every later step feeds the last
+    token only (cascade_attention.py:473-499, 527-538).  Greedy, as there, or with ``sampling`` (``temperature``, ``top_k``, ``top_p``,
+    ``min_p`` of :func:`sample_tokens`, numbers or one a stream) drawn, the random numbers by ``generator``."""
     logits = None
     for i in range(0, input_ids.size(1), stride):
         logits = model(input_ids[:, i:i + stride], cache)
     out = input_ids
     for step in range(max_new_tokens):
-        nxt = torch.argmax(logits[:, -1, :], dim=-1)
+        if sampling is None:
+            nxt = torch.argmax(logits[:, -1, :], dim=-1)
+        else:
+            uniforms = torch.rand(logits.size(0), generator=generator, device=logits.device)
+            nxt = sample_tokens(logits[:, -1, :], uniforms, **sampling)[0].clamp_(min=0)   # a row of NaN gives -1, which is no embedding
         out = torch.cat([out, nxt[:, None]], dim=-1)
         if step + 1 < max_new_tokens:
             logits = model(out[:, -1:], cache)

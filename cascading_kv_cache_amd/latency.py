@@ -21,15 +21,18 @@ from torch import nn
 
 from .cascade_attention import CascadeAttention
 from .cascading_cache import CascadingKVCache
+from .norm_rotate import norm_rotate
 
 
 class ProjectedCascadeAttention(CascadeAttention):
     """A concrete layer for :class:`CascadeAttention`: the attributes the reference's mixin reads off
-    a Llama / Qwen2 attention module (cascade_attention.py:103-112, llama_eval.py:142-152)."""
+    a Llama / Qwen2 attention module (cascade_attention.py:103-112, llama_eval.py:142-152).  ``qk_norm``: every head's
+    queries and keys are normed behind the projections; the cache then holds normed keys, un-rotated as ever."""
+    qk_norm = False   # saved layers may have none
 
     def __init__(self, hidden_size=4096, num_heads=32, num_key_value_heads=8, head_dim=128, rope_theta=5e5,
                  qkv_bias=False, head_reduction="max", homogeneous_heads=False, do_og_pos=False, layer_idx=0,
-                 dtype=torch.float16, device="cuda"):
+                 dtype=torch.float16, device="cuda", qk_norm=False, norm_eps=1e-6):
         super().__init__()
         self.hidden_size, self.num_heads, self.num_key_value_heads = hidden_size, num_heads, num_key_value_heads
         self.head_dim, self.rope_theta, self.layer_idx = head_dim, rope_theta, layer_idx
@@ -41,6 +44,10 @@ class ProjectedCascadeAttention(CascadeAttention):
         self.v_proj = nn.Linear(hidden_size, num_key_value_heads * head_dim, bias=qkv_bias, **kw)
         self.o_proj = nn.Linear(num_heads * head_dim, hidden_size, bias=False, **kw)
         self._w_qkv = self._b_qkv = None
+        if qk_norm:
+            self.qk_norm, self.norm_eps = True, norm_eps
+            self.q_norm_weight = nn.Parameter(torch.ones(head_dim, **kw))
+            self.k_norm_weight = nn.Parameter(torch.ones(head_dim, **kw))
 
     def fuse_projections(self):
         """Keep the three projection matrices in one buffer (``q_proj`` / ``k_proj`` / ``v_proj`` become views of
@@ -63,6 +70,16 @@ class ProjectedCascadeAttention(CascadeAttention):
         if self._w_qkv is None:
             return super().qkv(x, size, kv_size)
         return self._split_qkv(nn.functional.linear(x, self._w_qkv, self._b_qkv), size, kv_size)
+
+    def _attend(self, query_states, key_states, value_states, past_key_value, homogeneous_heads, do_og_pos):
+        if self.qk_norm:
+            # the rows of a fused product are this call's alone: normed where they are, beside the values
+            alone = self._w_qkv is not None and type(self).qkv is ProjectedCascadeAttention.qkv and not torch.is_grad_enabled()
+            query_states, key_states = norm_rotate(query_states, key_states, self.q_norm_weight, self.k_norm_weight, eps=self.norm_eps,
+                                                   out=(query_states, key_states) if alone else None)
+            if not alone:
+                value_states = value_states.contiguous()   # as the keys lie
+        return super()._attend(query_states, key_states, value_states, past_key_value, homogeneous_heads, do_og_pos)
 
     def _split_qkv(self, rows, size=None, kv_size=None):
         """Rows of ``q | k | v`` as ``qkv`` returns them."""

@@ -38,9 +38,9 @@ def _describe(q, k, q_weight, k_weight, positions, inv_freq, eps):
     return a
 
 
-def _forward(q, k, q_weight, k_weight, positions, inv_freq, eps):
+def _forward(q, k, q_weight, k_weight, positions, inv_freq, eps, out=None):
     # not torch.empty_like: the inputs are usually parts of one wider buffer, and may be expanded
-    q_out, k_out = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
+    q_out, k_out = out or (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
     a = _describe(q, k, q_weight, k_weight, positions, inv_freq, eps)
     a.q_out, a.k_out = q_out.data_ptr(), k_out.data_ptr()
     _abi.set_strides(a.q_out_stride, q_out)
@@ -120,8 +120,19 @@ def _check(q, k, q_weight, k_weight, positions, inv_freq):
             raise ValueError("inv_freq has no gradient here")
 
 
-def norm_rotate(q, k, q_weight=None, k_weight=None, positions=None, inv_freq=None, eps=1e-6):
-    """``(q, k)`` with every head's row normed and rotated, contiguous.
+def _check_out(out, q, k):
+    for name, t, like in (("queries", out[0], q), ("keys", out[1], k)):
+        if t.dtype != like.dtype or t.device != like.device or t.shape != like.shape:
+            raise ValueError(f"out holds {name} {tuple(t.shape)} of {t.dtype} on {t.device}; expected {tuple(like.shape)} of {like.dtype} on {like.device}")
+        if t.size(-1) > 1 and t.stride(-1) != 1:
+            raise ValueError("the head dims of out are not adjacent")
+        if any(s == 0 for n, s in zip(t.shape, t.stride()) if n > 1):
+            raise ValueError("out is expanded: its rows are not its own")
+
+
+def norm_rotate(q, k, q_weight=None, k_weight=None, positions=None, inv_freq=None, eps=1e-6, out=None):
+    """``(q, k)`` with every head's row normed and rotated, contiguous, or written to ``out``: two tensors of their shapes, apart from the inputs
+    or the inputs themselves (a decoding step has no other use for them); such a call has no gradients.
 
     q ``(B, H, n, D)`` and k ``(B, KVH, n, D)``, float32, float16 or bfloat16, any strides.  ``q_weight``, ``k_weight`` ``(D,)``, dtype of q: the
     weights of the norm, or None for no norm.  ``positions`` int64 ``(n,)`` or ``(B, n)`` and ``inv_freq`` float32 ``(R / 2,)``: the first
@@ -132,6 +143,12 @@ def norm_rotate(q, k, q_weight=None, k_weight=None, positions=None, inv_freq=Non
     q_weight, k_weight, inv_freq = (None if t is None else t.contiguous() for t in (q_weight, k_weight, inv_freq))
     if positions is not None and positions.stride(-1) != 1:
         positions = positions.contiguous()
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+    followed = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight))
+    if out is not None:
+        if followed:
+            raise ValueError("no gradients go through out")
+        _check_out(out, q, k)
+        return _forward(q, k, q_weight, k_weight, positions, inv_freq, eps, tuple(out))
+    if followed:
         return _NormRotate.apply(q, k, q_weight, k_weight, positions, inv_freq, float(eps))
     return _forward(q, k, q_weight, k_weight, positions, inv_freq, eps)

@@ -338,8 +338,8 @@ int ckv_linear_rows(const void* x, const void* w, const void* bias, const void* 
  *   y = x / sqrt(mean(x^2) + eps) * weight;  with weights NULL (both) y = x
  *   out[j] = y[j] cos - y[j + rot/2] sin,  out[j + rot/2] = y[j + rot/2] cos + y[j] sin  for j < rot/2, the rest as it is;
  *   angle = position * inv_freq[j], of the exact product; rot 0: norm alone.
- * float32 throughout, rounded once.  Any strides but along the head dims (1); outputs may not overlap inputs.
- * head_dim up to 256.  ckv_norm_rotate_bwd takes the same arguments and the gradients of the outputs instead of the
+ * float32 throughout, rounded once.  Any strides but along the head dims (1); forward outputs may be the inputs themselves (same
+ * strides), else nothing written may overlap anything read.  head_dim up to 256.  ckv_norm_rotate_bwd takes the same arguments and the gradients of the outputs instead of the
  * outputs, and writes those of q, k and the weights (summed in a fixed order).
  * ---------------------------------------------------------------------------------------- */
 typedef struct ckv_norm_rotate_args {

@@ -244,3 +244,23 @@ def test_another_stream_and_replays_of_a_graph():
         fresh = step()          # the program's own work between two replays
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(recorded, fresh)), rep
+
+
+def test_written_over_the_inputs_and_elsewhere():
+    for layout, D in (("projected", 128), ("dense", 64), ("odd", 80)):
+        q, k, qw, kw, _ = inputs(2, 4, 2, 7, D, torch.bfloat16, layout)
+        pos, inv_freq = torch.arange(7, device="cuda"), freqs(D)
+        want = norm_rotate(q, k, qw, kw, pos, inv_freq)
+        there = torch.zeros(7, 2, 4, D, dtype=q.dtype, device="cuda").permute(1, 2, 0, 3), torch.zeros_like(k)
+        for out in (there, (q, k)):
+            got = norm_rotate(q, k, qw, kw, pos, inv_freq, out=out)
+            assert got[0] is out[0] and torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+def test_outputs_that_cannot_be_written_to():
+    q, k, qw, kw, _ = inputs(2, 4, 2, 7, 64, torch.float32, "dense")
+    for out in ((q[:, :3], k), (q, k.half()), (q.transpose(2, 3).contiguous().transpose(2, 3), k), (q[:1].expand(2, -1, -1, -1), k), (q.cpu(), k)):
+        with pytest.raises(ValueError):
+            norm_rotate(q, k, qw, kw, out=out)
+    with pytest.raises(ValueError, match="gradients"):
+        norm_rotate(q, k, qw.requires_grad_(), kw, out=(q, k))
