@@ -6,47 +6,12 @@
 // Three matrix products, of one kind: C (M, N) = sum over k of A (m, k) B (n, k), where an operand's elements are adjacent along k (x and W of
 // the forward pass, [dg du] of dx) or along its rows (W of dx, both operands of dW).  With the gate, a tile of C has as many gate columns as
 // up columns, the same ones, and a wavefront holds both: g and u meet in registers, and C itself is written only for the backward pass.
-#include "ckv_common.h"
+#include "ckv_product.h"
 
 #include <algorithm>
 
 namespace ckv {
 namespace {
-
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-
-struct Operand {
-    const void* p;
-    int64_t rows;      // M or N
-    int64_t stride;    // between rows (along_k) or between the elements of a row, which are k steps apart
-};
-
-struct ProductParams {
-    Operand a, b;
-    void* out;          // (M, N) contiguous, or the gated (M, N / 2)
-    void* both;         // gated, optional: (M, N), gate and up columns
-    float* partial;     // (splits, M, N) where the sums are shared out, else null
-    int64_t M, N, K;
-    int64_t k_share;    // k steps a share
-    int tiles_m, tiles_n;
-    bool a_vectors, b_vectors;   // rows of whole, aligned pieces of 16 bytes
-};
-
-enum Epilogue { kStore, kGate };
-
-__device__ inline float gate_product(float g, float u) { return g / (1.f + expf(-g)) * u; }
-
-// Tiles go round the eight XCDs: each gets a stretch of them, eight tiles of M high, so that the tiles of a stretch that run at a time share
-// operands in its L2.
-__device__ inline void tile_of(const ProductParams& p, int& tm, int& tn) {
-    const int all = p.tiles_m * p.tiles_n, xcd = blockIdx.x % 8, many = all / 8, over = all % 8;
-    const int tile = xcd * many + min(xcd, over) + blockIdx.x / 8;
-    constexpr int kHigh = 8;
-    const int band = tile / (kHigh * p.tiles_n), in = tile - band * kHigh * p.tiles_n;
-    const int high = min(kHigh, p.tiles_m - band * kHigh);
-    tm = band * kHigh + in % high;
-    tn = in / high;
-}
 
 // ---- any type, stride and size: float32 products on v_mfma_f32_32x32x2 -----------------------------------------------------------------
 
@@ -101,7 +66,7 @@ template <typename T, bool kAlongKA, bool kAlongKB, Epilogue kEpilogue>
 __global__ void __launch_bounds__(256) product_kernel(ProductParams p) {
     __shared__ __align__(16) float as[2][kStep][kPitch], bs[2][kStep][kPitch];
     int tm, tn;
-    tile_of(p, tm, tn);
+    tile_of<8>(p, tm, tn);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1, half = lane >> 5, l = lane & 31;
     constexpr bool kGated = kEpilogue == kGate;
     const int64_t inter = p.N / 2;
@@ -122,7 +87,7 @@ __global__ void __launch_bounds__(256) product_kernel(ProductParams p) {
         pa.store(as[at], pa.row);
         pb.store(bs[at], pb.row);
     };
-    f32x16 acc[2][2] = {};
+    f32x16_t acc[2][2] = {};
     load(k0);
     store(0);
     __syncthreads();
@@ -252,42 +217,61 @@ int gate_gradient(const void* gate_up, const void* dout, void* grad, int64_t row
 
 // ---- which kernel, how many shares -----------------------------------------------------------------------------------------------------
 
-struct Plan {
-    int64_t k_share;
-    int shares, tiles_m, tiles_n;
-    int64_t bytes;   // of the shares' sums
-};
+// The kernels of 16-bit tiles take operands of whole pieces of 16 bytes: all but odd sizes, strides and addresses.
+template <typename T>
+bool fits_tiles(const ProductParams& p, bool along_a, bool along_b, bool gated) {
+    if (sizeof(T) != 2) return false;
+    auto whole = [&](const Operand& o, bool along, int64_t rows) {
+        return reinterpret_cast<uintptr_t>(o.p) % 16 == 0 && o.stride % 8 == 0 && (along ? p.K : rows) % 8 == 0 && o.stride < (1 << 22);
+    };
+    return whole(p.a, along_a, p.M) && whole(p.b, along_b, p.N) && (gated ? p.N / 2 : p.N) % 8 == 0 &&
+           ((reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.both)) & 15) == 0;
+}
 
-// Where the tiles leave compute units idle, the steps are shared out over as many workgroups as come to one each, none with fewer than 256.
-Plan plan_product(int64_t M, int64_t N, int64_t K, bool gated, int cus) {
-    Plan r;
+// Where the tiles of float32 products leave compute units idle, the steps are shared out over as many workgroups as come to one each, none with
+// fewer than 256.
+TilePlan plan_float(int64_t M, int64_t N, int64_t K, bool gated, int cus) {
+    TilePlan r;
+    r.tile_m = r.tile_n = kTile;
     r.tiles_m = (int)((M + kTile - 1) / kTile);
-    r.tiles_n = (int)((N + kTile - 1) / kTile);
-    if (gated) r.tiles_n = (int)((N / 2 + kTile / 2 - 1) / (kTile / 2));
+    r.tiles_n = (int)(gated ? (N / 2 + kTile / 2 - 1) / (kTile / 2) : (N + kTile - 1) / kTile);
     const int64_t tiles = (int64_t)r.tiles_m * r.tiles_n;
     const int64_t shares = std::max<int64_t>(1, std::min<int64_t>(cus / tiles, K / 256));
     r.k_share = ((K + shares - 1) / shares + kStep - 1) / kStep * kStep;
     r.shares = (int)((K + r.k_share - 1) / r.k_share);
-    r.bytes = r.shares > 1 ? r.shares * M * N * 4 : 0;
     return r;
+}
+
+int64_t share_bytes(const TilePlan& plan, int64_t M, int64_t N) { return plan.shares > 1 ? align_up(plan.shares * M * N * 4, 256) : 0; }
+
+// Scratch of a product, whichever kernel takes it.
+int64_t product_bytes(int64_t M, int64_t N, int64_t K, bool a_along_k, bool gated, int cus) {
+    return std::max(share_bytes(plan_tiles(M, N, K, a_along_k, gated, cus), M, N), share_bytes(plan_float(M, N, K, gated, cus), M, N));
 }
 
 template <typename T, bool kAlongKA, bool kAlongKB, Epilogue kEpilogue>
 int run_product(ProductParams& p, const DeviceInfo& di, void* workspace, int64_t bytes, hipStream_t stream) {
-    const Plan plan = plan_product(p.M, p.N, p.K, kEpilogue == kGate, di.cus);
-    if (plan.bytes > bytes || (plan.bytes && !workspace)) return CKV_ERR_WORKSPACE;
+    constexpr bool kGated = kEpilogue == kGate;
+    const bool tiles = fits_tiles<T>(p, kAlongKA, kAlongKB, kGated);
+    const TilePlan plan = tiles ? plan_tiles(p.M, p.N, p.K, kAlongKA, kGated, di.cus) : plan_float(p.M, p.N, p.K, kGated, di.cus);
+    if (plan.shares > 1 && (!workspace || share_bytes(plan, p.M, p.N) > bytes)) return CKV_ERR_WORKSPACE;
     if ((int64_t)plan.tiles_m * plan.tiles_n > 0x7fffffff) return CKV_ERR_UNSUPPORTED;
-    auto vectors = [](const Operand& o) { return reinterpret_cast<uintptr_t>(o.p) % 16 == 0 && o.stride % (16 / (int64_t)sizeof(T)) == 0; };
-    p.a_vectors = vectors(p.a);
-    p.b_vectors = vectors(p.b) && (kEpilogue != kGate || kAlongKB);
-    p.tiles_m = plan.tiles_m;
-    p.tiles_n = plan.tiles_n;
-    p.k_share = plan.k_share;
     p.partial = plan.shares > 1 ? (float*)workspace : nullptr;
-    hipLaunchKernelGGL((product_kernel<T, kAlongKA, kAlongKB, kEpilogue>), dim3(plan.tiles_m * plan.tiles_n, plan.shares), dim3(256), 0, stream, p);
-    CKV_HIP_TRY(hipGetLastError());
+    if (tiles) {
+        if constexpr (sizeof(T) == 2)
+            if (int rc = run_tiles<T>(p, plan, kAlongKA, kAlongKB, kEpilogue, stream)) return rc;
+    } else {
+        auto vectors = [](const Operand& o) { return reinterpret_cast<uintptr_t>(o.p) % 16 == 0 && o.stride % (16 / (int64_t)sizeof(T)) == 0; };
+        p.a_vectors = vectors(p.a);
+        p.b_vectors = vectors(p.b);
+        p.tiles_m = plan.tiles_m;
+        p.tiles_n = plan.tiles_n;
+        p.k_share = plan.k_share;
+        hipLaunchKernelGGL((product_kernel<T, kAlongKA, kAlongKB, kEpilogue>), dim3(plan.tiles_m * plan.tiles_n, plan.shares), dim3(256), 0, stream, p);
+        CKV_HIP_TRY(hipGetLastError());
+    }
     if (p.partial) {
-        const int64_t all = p.M * (kEpilogue == kGate ? p.N / 2 : p.N);
+        const int64_t all = p.M * (kGated ? p.N / 2 : p.N);
         hipLaunchKernelGGL((merge_kernel<T, kEpilogue>), dim3((unsigned)std::min<int64_t>((all + 255) / 256, 256 * 16)), dim3(256), 0, stream, p, plan.shares);
         CKV_HIP_TRY(hipGetLastError());
     }
@@ -305,8 +289,8 @@ template <typename T>
 int run_forward(const void* x, const void* w, void* out, void* gate_up, int64_t rows, int64_t inter, int64_t k, int64_t x_stride, void* workspace,
                 int64_t bytes, const DeviceInfo& di, hipStream_t stream) {
     ProductParams p = {};
-    p.a = Operand{x, rows, x_stride};
-    p.b = Operand{w, 2 * inter, k};
+    p.a = Operand{x, x_stride};
+    p.b = Operand{w, k};
     p.out = out;
     p.both = gate_up;
     p.M = rows;
@@ -325,8 +309,8 @@ int run_backward(const void* x, const void* w, const void* gate_up, const void* 
     bytes -= grad_bytes;
     if (dx) {
         ProductParams p = {};
-        p.a = Operand{grad, rows, 2 * inter};
-        p.b = Operand{w, k, k};
+        p.a = Operand{grad, 2 * inter};
+        p.b = Operand{w, k};
         p.out = dx;
         p.M = rows;
         p.N = k;
@@ -335,8 +319,8 @@ int run_backward(const void* x, const void* w, const void* gate_up, const void* 
     }
     if (dw) {
         ProductParams p = {};
-        p.a = Operand{grad, 2 * inter, 2 * inter};
-        p.b = Operand{x, k, x_stride};
+        p.a = Operand{grad, 2 * inter};
+        p.b = Operand{x, x_stride};
         p.out = dw;
         p.M = 2 * inter;
         p.N = k;
@@ -358,7 +342,7 @@ extern "C" int64_t ckv_gated_linear_workspace_bytes(int64_t rows, int64_t inter,
     using namespace ckv;
     DeviceInfo di;
     if (check_sizes(rows, inter, k, k, dtype) || rows == 0 || current_device_info(&di)) return 0;
-    return plan_product(rows, 2 * inter, k, true, di.cus).bytes;
+    return product_bytes(rows, 2 * inter, k, true, true, di.cus);
 }
 
 extern "C" int ckv_gated_linear(const void* x, const void* w, void* out, void* gate_up, int64_t rows, int64_t inter, int64_t k, int64_t x_stride,
@@ -381,7 +365,7 @@ extern "C" int64_t ckv_gated_linear_bwd_workspace_bytes(int64_t rows, int64_t in
     using namespace ckv;
     DeviceInfo di;
     if (check_sizes(rows, inter, k, k, dtype) || rows == 0 || current_device_info(&di)) return 0;
-    const int64_t dx = plan_product(rows, k, 2 * inter, false, di.cus).bytes, dw = plan_product(2 * inter, k, rows, false, di.cus).bytes;
+    const int64_t dx = product_bytes(rows, k, 2 * inter, true, false, di.cus), dw = product_bytes(2 * inter, k, rows, false, false, di.cus);
     return align_up(rows * 2 * inter * elem_bytes(dtype), 256) + std::max(dx, dw);
 }
 
