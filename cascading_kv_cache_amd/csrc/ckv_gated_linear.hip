@@ -65,13 +65,13 @@ struct Piece {
 template <typename T, bool kAlongKA, bool kAlongKB, Epilogue kEpilogue>
 __global__ void __launch_bounds__(256) product_kernel(ProductParams p) {
     __shared__ __align__(16) float as[2][kStep][kPitch], bs[2][kStep][kPitch];
-    int tm, tn;
-    tile_of<8>(p, tm, tn);
+    int tm, tn, share;
+    float* sums = work_of<8>(p, kTile * kTile, tm, tn, share);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1, half = lane >> 5, l = lane & 31;
     constexpr bool kGated = kEpilogue == kGate;
     const int64_t inter = p.N / 2;
     const int64_t m0 = (int64_t)tm * kTile, n0 = (int64_t)tn * (kGated ? kTile / 2 : kTile);
-    const int64_t k0 = blockIdx.y * p.k_share, k1 = min(p.K, k0 + p.k_share);
+    const int64_t k0 = share * p.k_share, k1 = sums ? min(p.K, k0 + p.k_share) : p.K;
     Piece<T, kAlongKA> pa;
     Piece<T, kAlongKB> pb;
     const T* a = (const T*)p.a.p;
@@ -117,18 +117,18 @@ __global__ void __launch_bounds__(256) product_kernel(ProductParams p) {
     for (int i = 0; i < 2; i++)
 #pragma unroll
         for (int r = 0; r < 16; r++) {
-            const int64_t m = m0 + wm * 64 + i * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
+            const int row = wm * 64 + i * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
+            const int64_t m = m0 + row;
+            if (sums) {
+#pragma unroll
+                for (int j = 0; j < 2; j++) sums[row * kTile + (kGated ? j * 64 + wn * 32 : wn * 64 + j * 32) + l] = acc[i][j][r];
+                continue;
+            }
             if (m >= p.M) continue;
             if constexpr (kGated) {
                 const int64_t n = n0 + wn * 32 + l;
                 if (n >= inter) continue;
                 const float g = acc[i][0][r], u = acc[i][1][r];
-                if (p.partial) {
-                    float* to = p.partial + (blockIdx.y * p.M + m) * p.N + n;
-                    to[0] = g;
-                    to[inter] = u;
-                    continue;
-                }
                 ((T*)p.out)[m * inter + n] = Elem<T>::from_float(gate_product(g, u));
                 if (p.both) {
                     T* to = (T*)p.both + m * p.N + n;
@@ -139,37 +139,52 @@ __global__ void __launch_bounds__(256) product_kernel(ProductParams p) {
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
                     const int64_t n = n0 + wn * 64 + j * 32 + l;
-                    if (n >= p.N) continue;
-                    if (p.partial) p.partial[(blockIdx.y * p.M + m) * p.N + n] = acc[i][j][r];
-                    else ((T*)p.out)[m * p.N + n] = Elem<T>::from_float(acc[i][j][r]);
+                    if (n < p.N) ((T*)p.out)[m * p.N + n] = Elem<T>::from_float(acc[i][j][r]);
                 }
             }
         }
 }
 
-// Sums of the shares, in their order, and what the product's own epilogue does.
+// Sums of the shares of a tile, in their order, and what the product's own epilogue does.  A workgroup has some rows of a tile, a thread four
+// columns.
 template <typename T, Epilogue kEpilogue>
-__global__ void __launch_bounds__(256) merge_kernel(ProductParams p, int shares) {
+__global__ void __launch_bounds__(256) merge_kernel(ProductParams p, int tile_m, int tile_n, int high, int rows) {
     constexpr bool kGated = kEpilogue == kGate;
-    const int64_t cols = kGated ? p.N / 2 : p.N, all = p.M * cols, share = p.M * p.N;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
-        int64_t n;
-        const int64_t m = div_index(i, cols, n);
-        const float* from = p.partial + m * p.N + n;
-        float g = 0.f, u = 0.f;
-        for (int s = 0; s < shares; s++) {
-            g += from[s * share];
-            if constexpr (kGated) u += from[s * share + cols];
-        }
-        if constexpr (kGated) {
-            ((T*)p.out)[i] = Elem<T>::from_float(gate_product(g, u));
-            if (p.both) {
-                T* to = (T*)p.both + m * p.N + n;
-                to[0] = Elem<T>::from_float(g);
-                to[cols] = Elem<T>::from_float(u);
+    const int tile = p.whole_tiles + blockIdx.x;
+    int tm, tn;
+    if (high == 8) place_of<8>(p, tile, tm, tn);
+    else place_of<4>(p, tile, tm, tn);
+    const int width = kGated ? tile_n / 2 : tile_n;
+    const int64_t cols = kGated ? p.N / 2 : p.N, n0 = (int64_t)tn * width, m0 = (int64_t)tm * tile_m, share = (int64_t)tile_m * tile_n;
+    const float* from = p.partial + blockIdx.x * p.shares * share;
+    const int per_row = width / 4;
+    for (int i = threadIdx.x; i < rows * per_row; i += 256) {
+        const int row = blockIdx.y * rows + i / per_row, col = i % per_row * 4;
+        const int64_t m = m0 + row, n = n0 + col;
+        if (m >= p.M || n >= cols) continue;
+        const float* at = from + (int64_t)row * tile_n + col;
+        float g[4] = {}, u[4] = {};
+        for (int s = 0; s < p.shares; s++) {
+            const float4 a = *reinterpret_cast<const float4*>(at + s * share);
+            g[0] += a.x; g[1] += a.y; g[2] += a.z; g[3] += a.w;
+            if constexpr (kGated) {
+                const float4 b = *reinterpret_cast<const float4*>(at + s * share + width);
+                u[0] += b.x; u[1] += b.y; u[2] += b.z; u[3] += b.w;
             }
-        } else {
-            ((T*)p.out)[i] = Elem<T>::from_float(g);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if (n + e >= cols) break;
+            if constexpr (kGated) {
+                ((T*)p.out)[m * cols + n + e] = Elem<T>::from_float(gate_product(g[e], u[e]));
+                if (p.both) {
+                    T* to = (T*)p.both + m * p.N + n + e;
+                    to[0] = Elem<T>::from_float(g[e]);
+                    to[cols] = Elem<T>::from_float(u[e]);
+                }
+            } else {
+                ((T*)p.out)[m * cols + n + e] = Elem<T>::from_float(g[e]);
+            }
         }
     }
 }
@@ -230,49 +245,54 @@ bool fits_tiles(const ProductParams& p, bool along_a, bool along_b, bool gated) 
 
 // Where the tiles of float32 products leave compute units idle, the steps are shared out over as many workgroups as come to one each, none with
 // fewer than 256.
-TilePlan plan_float(int64_t M, int64_t N, int64_t K, bool gated, int cus) {
+TilePlan plan_float(int64_t M, int64_t N, int64_t K, int cus) {
     TilePlan r;
     r.tile_m = r.tile_n = kTile;
+    r.stages = 2;
     r.tiles_m = (int)((M + kTile - 1) / kTile);
-    r.tiles_n = (int)(gated ? (N / 2 + kTile / 2 - 1) / (kTile / 2) : (N + kTile - 1) / kTile);
+    r.tiles_n = (int)((N + kTile - 1) / kTile);
     const int64_t tiles = (int64_t)r.tiles_m * r.tiles_n;
     const int64_t shares = std::max<int64_t>(1, std::min<int64_t>(cus / tiles, K / 256));
     r.k_share = ((K + shares - 1) / shares + kStep - 1) / kStep * kStep;
     r.shares = (int)((K + r.k_share - 1) / r.k_share);
+    r.whole_tiles = r.shares > 1 ? 0 : (int)std::min<int64_t>(tiles, 0x7fffffff);
     return r;
 }
 
-int64_t share_bytes(const TilePlan& plan, int64_t M, int64_t N) { return plan.shares > 1 ? align_up(plan.shares * M * N * 4, 256) : 0; }
+// Columns of B's tiles are gate and up columns by halves, so there may be tiles with few of either.
+int64_t tiled_columns(int64_t N, bool gated, int tile_n) {
+    return gated ? (N / 2 + tile_n / 2 - 1) / (tile_n / 2) * tile_n : N;
+}
 
 // Scratch of a product, whichever kernel takes it.
 int64_t product_bytes(int64_t M, int64_t N, int64_t K, bool a_along_k, bool gated, int cus) {
-    return std::max(share_bytes(plan_tiles(M, N, K, a_along_k, gated, cus), M, N), share_bytes(plan_float(M, N, K, gated, cus), M, N));
+    return std::max(plan_tiles(M, tiled_columns(N, gated, 128), K, a_along_k, cus).bytes(), plan_float(M, tiled_columns(N, gated, kTile), K, cus).bytes());
 }
 
 template <typename T, bool kAlongKA, bool kAlongKB, Epilogue kEpilogue>
 int run_product(ProductParams& p, const DeviceInfo& di, void* workspace, int64_t bytes, hipStream_t stream) {
     constexpr bool kGated = kEpilogue == kGate;
     const bool tiles = fits_tiles<T>(p, kAlongKA, kAlongKB, kGated);
-    const TilePlan plan = tiles ? plan_tiles(p.M, p.N, p.K, kAlongKA, kGated, di.cus) : plan_float(p.M, p.N, p.K, kGated, di.cus);
-    if (plan.shares > 1 && (!workspace || share_bytes(plan, p.M, p.N) > bytes)) return CKV_ERR_WORKSPACE;
-    if ((int64_t)plan.tiles_m * plan.tiles_n > 0x7fffffff) return CKV_ERR_UNSUPPORTED;
-    p.partial = plan.shares > 1 ? (float*)workspace : nullptr;
+    const TilePlan plan = tiles ? plan_tiles(p.M, tiled_columns(p.N, kGated, 128), p.K, kAlongKA, di.cus)
+                                : plan_float(p.M, tiled_columns(p.N, kGated, kTile), p.K, di.cus);
+    if (plan.bytes() && (!workspace || plan.bytes() > bytes || reinterpret_cast<uintptr_t>(workspace) & 15)) return CKV_ERR_WORKSPACE;
+    if ((int64_t)plan.tiles_m * plan.tiles_n > 0x3fffffff || plan.blocks() > 0x7fffffff) return CKV_ERR_UNSUPPORTED;
+    plan.fill(p);
+    p.partial = (float*)workspace;
     if (tiles) {
         if constexpr (sizeof(T) == 2)
-            if (int rc = run_tiles<T>(p, plan, kAlongKA, kAlongKB, kEpilogue, stream)) return rc;
+            if (int rc = run_tiles<T>(p, plan, kAlongKA, kEpilogue, stream)) return rc;
     } else {
         auto vectors = [](const Operand& o) { return reinterpret_cast<uintptr_t>(o.p) % 16 == 0 && o.stride % (16 / (int64_t)sizeof(T)) == 0; };
         p.a_vectors = vectors(p.a);
         p.b_vectors = vectors(p.b);
-        p.tiles_m = plan.tiles_m;
-        p.tiles_n = plan.tiles_n;
-        p.k_share = plan.k_share;
-        hipLaunchKernelGGL((product_kernel<T, kAlongKA, kAlongKB, kEpilogue>), dim3(plan.tiles_m * plan.tiles_n, plan.shares), dim3(256), 0, stream, p);
+        hipLaunchKernelGGL((product_kernel<T, kAlongKA, kAlongKB, kEpilogue>), dim3((unsigned)plan.blocks()), dim3(256), 0, stream, p);
         CKV_HIP_TRY(hipGetLastError());
     }
-    if (p.partial) {
-        const int64_t all = p.M * (kGated ? p.N / 2 : p.N);
-        hipLaunchKernelGGL((merge_kernel<T, kEpilogue>), dim3((unsigned)std::min<int64_t>((all + 255) / 256, 256 * 16)), dim3(256), 0, stream, p, plan.shares);
+    if (plan.shares > 1) {
+        constexpr int kRows = 8;
+        hipLaunchKernelGGL((merge_kernel<T, kEpilogue>), dim3(plan.tiles_m * plan.tiles_n - plan.whole_tiles, plan.tile_m / kRows), dim3(256), 0, stream, p, plan.tile_m,
+                           plan.tile_n, tiles ? 4 : 8, kRows);
         CKV_HIP_TRY(hipGetLastError());
     }
     return CKV_OK;

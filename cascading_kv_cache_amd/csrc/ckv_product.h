@@ -16,38 +16,72 @@ struct ProductParams {
     Operand a, b;
     void* out;          // (M, N) contiguous, or the gated (M, N / 2)
     void* both;         // gated, optional: (M, N), gate and up columns
-    float* partial;     // (shares, M, N) where the sums are shared out, else null
+    float* partial;     // sums of the shares, tile by tile: (tiles shared out, shares, tile rows, tile columns)
     int64_t M, N, K;
     int64_t k_share;    // steps of a share
     int tiles_m, tiles_n;
+    int whole_tiles;    // tiles before the first that is shared out
+    int shares;
     bool a_vectors, b_vectors;   // float32 products: operands of whole, aligned pieces of 16 bytes
 };
 
 enum Epilogue { kStore, kGate };
 
-__device__ inline float gate_product(float g, float u) { return g / (1.f + expf(-g)) * u; }
+// silu(g) * u.  The exponential by the hardware's exp2, whose argument is rounded: |g| 2^-24 relative, of what is added to one.
+__device__ inline float gate_product(float g, float u) {
+    return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.44269504f)) * u;
+}
 
-// Tiles go round the eight XCDs: each gets a stretch of them, kHigh tiles of M high, so that the tiles of a stretch that run at a time share
-// operands in its L2.
+// Workgroups go round the eight XCDs: each gets a stretch of the tiles, and behind those one of the shares.  Tiles are numbered in bands
+// kHigh tiles of M high, so that the tiles of a stretch that run at a time share operands in its L2.
+__device__ inline int stretch(int block, int all) {
+    const int xcd = block % 8, many = all / 8, over = all % 8;
+    return xcd * many + min(xcd, over) + block / 8;
+}
 template <int kHigh>
-__device__ inline void tile_of(const ProductParams& p, int& tm, int& tn) {
-    const int all = p.tiles_m * p.tiles_n, xcd = blockIdx.x % 8, many = all / 8, over = all % 8;
-    const int tile = xcd * many + min(xcd, over) + blockIdx.x / 8;
+__device__ inline void place_of(const ProductParams& p, int tile, int& tm, int& tn) {
     const int band = tile / (kHigh * p.tiles_n), in = tile - band * kHigh * p.tiles_n;
     const int high = min(kHigh, p.tiles_m - band * kHigh);
     tm = band * kHigh + in % high;
     tn = in / high;
 }
+// This workgroup's tile, its share of it, and, where there are several, where the sums of the share go.
+template <int kHigh>
+__device__ inline float* work_of(const ProductParams& p, int tile_size, int& tm, int& tn, int& share) {
+    const int all = p.tiles_m * p.tiles_n, block = blockIdx.x;
+    const bool rest = block >= p.whole_tiles;
+    share = 0;
+    if (!rest || p.shares == 1) {
+        const int first = rest ? p.whole_tiles : 0;
+        place_of<kHigh>(p, first + stretch(block - first, rest ? all - first : p.whole_tiles), tm, tn);
+        return nullptr;
+    }
+    const int at = stretch(block - p.whole_tiles, (all - p.whole_tiles) * p.shares);
+    share = at % p.shares;
+    place_of<kHigh>(p, p.whole_tiles + at / p.shares, tm, tn);
+    return p.partial + (int64_t)at * tile_size;
+}
 
 // ---- 16-bit operands on the matrix instructions of their type, ckv_product_mfma.hip -------------------------------------------------------
 // Sizes and layouts it takes: whole pieces of 16 bytes everywhere (adjacent elements, strides, addresses; C's columns).
 struct TilePlan {
-    int tile_m, tile_n, tiles_m, tiles_n, shares;
+    int tile_m, tile_n, stages;
+    int tiles_m, tiles_n, whole_tiles, shares;
     int64_t k_share;
+    int64_t blocks() const { return whole_tiles + ((int64_t)tiles_m * tiles_n - whole_tiles) * shares; }
+    int64_t bytes() const {   // of the shares' sums
+        return shares > 1 ? align_up(((int64_t)tiles_m * tiles_n - whole_tiles) * shares * tile_m * tile_n * 4, 256) : 0;
+    }
+    void fill(ProductParams& p) const {
+        p.tiles_m = tiles_m;
+        p.tiles_n = tiles_n;
+        p.whole_tiles = whole_tiles;
+        p.shares = shares;
+        p.k_share = k_share;
+    }
 };
-TilePlan plan_tiles(int64_t M, int64_t N, int64_t K, bool a_along_k, bool gated, int cus);
-// p.partial is set where plan.shares > 1
+TilePlan plan_tiles(int64_t M, int64_t N, int64_t K, bool a_along_k, int cus);
 template <typename T>
-int run_tiles(ProductParams& p, const TilePlan& plan, bool a_along_k, bool b_along_k, Epilogue epilogue, hipStream_t stream);
+int run_tiles(const ProductParams& p, const TilePlan& plan, bool a_along_k, Epilogue epilogue, hipStream_t stream);
 
 }  // namespace ckv

@@ -1,30 +1,56 @@
-// C (M, N) = sum over k of A (m, k) B (n, k) of 16-bit operands on v_mfma_f32_32x32x16, with the gate of a gated MLP or shares of the
+// C (M, N) = sum over k of A (m, k) B (n, k) of 16-bit operands on v_mfma_f32_16x16x32, with the gate of a gated MLP or shares of the
 // sum behind it.
 //
-// A workgroup has a tile of C and brings 64 steps of both operands at a time into one of two stages of LDS by asynchronous copies, while
-// it works on the other: one barrier a stage.  An operand whose rows are adjacent along k lies in LDS as rows of 128 bytes, and an operand read
-// is 16 of them; one whose steps are adjacent along its rows lies as it is, and is turned on the way into registers (ds_read_b64_tr_b16).
-// Pieces of 16 bytes are permuted within a row as they are copied, so that an operand read meets every bank once.
+// A workgroup has a tile of C and brings 32 steps of both operands at a time into one of four stages of LDS by asynchronous copies, three
+// stages ahead: one barrier a stage.  An operand whose rows are adjacent along k lies in LDS as rows of 64 bytes, and an operand read is 16 of
+// them; one whose steps are adjacent along its rows lies as it is, and is turned on the way into registers (ds_read_b64_tr_b16).  Pieces of 16
+// bytes are permuted within a row as they are copied, so that an operand read meets every bank once.
+//
+// A wavefront of the large tile has 128 x 128 of it: with 64 x 128 each (eight wavefronts) the reads and copies of LDS alone take as long as the
+// products (a stage of 64 steps: 1536 + 512 of 2048 cycles).  One wavefront on a SIMD hides nothing behind another, so reads of the next
+// operands and copies stand between the products, one at a time.
 #include "ckv_product.h"
 
 #include <algorithm>
+#include <utility>
 
 namespace ckv {
 namespace {
 
+// f(0), f(1), ... f(kN - 1), the numbers known to the compiler
+template <typename F, int... kI>
+__device__ __attribute__((always_inline)) inline void each(F f, std::integer_sequence<int, kI...>) {
+    (f(std::integral_constant<int, kI>{}), ...);
+}
+template <int kN, typename F>
+__device__ __attribute__((always_inline)) inline void each(F f) {
+    each(f, std::make_integer_sequence<int, kN>{});
+}
+
 typedef __bf16 product_bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 product_f16x8 __attribute__((ext_vector_type(8)));
 typedef short product_s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t product_u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kSteps = 64;   // of a stage
+constexpr int kSteps = 32;   // of a stage, and of a matrix instruction
 
+// Written as an instruction, its sum in place: what the compiler makes of the builtin gives a sum another register than it had, and moves it
+// back, where there are as many as a wavefront of the large tile has.  Whoever reads a sum other than by the next product waits (sums_done).
 template <typename T>
-__device__ inline f32x16_t mma(uint4 a, uint4 b, f32x16_t c) {
+__device__ inline void mma(uint4 a, uint4 b, f32x4_t& c) {
     if constexpr (std::is_same<T, __hip_bfloat16>::value)
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(product_bf16x8, a), __builtin_bit_cast(product_bf16x8, b), c, 0, 0, 0);
+        asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(__builtin_bit_cast(product_bf16x8, a)), "v"(__builtin_bit_cast(product_bf16x8, b)));
     else
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(product_f16x8, a), __builtin_bit_cast(product_f16x8, b), c, 0, 0, 0);
+        asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(__builtin_bit_cast(product_f16x8, a)), "v"(__builtin_bit_cast(product_f16x8, b)));
+}
+template <int kM, int kN>
+__device__ inline void sums_done(f32x4_t (&c)[kM][kN]) {
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < kM; i++)
+#pragma unroll
+        for (int j = 0; j < kN; j++) asm volatile("" : "+a"(c[i][j]));   // nobody reads it earlier
 }
 
 template <typename T>
@@ -35,88 +61,95 @@ __device__ inline uint2 pack4(float a, float b, float c, float d) {
 // What steps behind the last one read: zeros of both operands (another row's number may be one times zero that is not zero).
 __device__ uint4 g_zeros[1];
 
-// One operand of a tile kRows rows high: copies of a wavefront, and where the lanes' operands lie.
+// Which bits of the number of a piece step k flips: a read that turns 8 steps (k..k+3 and k+8..k+11) of 16 rows meets every bank once.
+__device__ inline int turned_bits(int k) { return ((k & 3) << 2) | ((k >> 2) & 2); }
+
+// The same where rows lie along k: which of its four pieces stands first in row r.  A read of 16 bytes a lane goes in four parts, of lanes 0-3,
+// 12-15, 20-23 and 24-27 the first, of 4-11, 16-19 and 28-31 the second: rows 4 q.. of piece 0 for two q, of piece 1 for the two others.
+__device__ inline int first_piece(int r) { return ((r >> 2 << 1) ^ ((r >> 3 & 1) * 3)) & 3; }
+
+// One operand of a tile kRows rows high: copies of a wavefront, and where the lanes' pieces come from.
 template <int kRows, bool kAlongK, int kWaves>
 struct Side {
-    static constexpr int kCopies = kRows / 8 / kWaves;       // of 1 KiB a wavefront and stage
+    static constexpr int kCopies = kRows * kSteps / 512 / kWaves;   // of 1 KiB a wavefront and stage
     static constexpr int kBytes = kRows * kSteps * 2;
-    static constexpr int kRowBytes = kAlongK ? kSteps * 2 : kRows * 2;   // of LDS
-    const char* base[kCopies];   // uniform; with the gate the rows of a copy are all gate or all up rows
-    uint32_t voff[kCopies];
-    int step[kCopies];           // of the lane's piece, counted from the stage's first
+    const char* at;              // uniform: of the next stage to be copied
     int64_t advance;             // bytes a stage
+    uint32_t voff[kCopies];
 
-    // `first`, `rows`: the tile's first row and how many the operand has; kGated: rows kRows / 2 and up are row `first` of the second half
+    // `first`, `rows`: the tile's first row and how many the operand has; kGated: rows kRows / 2 and up, copied by the second half of the
+    // wavefronts, are row `first` of the operand's second half
     template <bool kGated>
     __device__ void init(const Operand& o, int64_t first, int64_t rows, int64_t k0, int wave, int lane) {
+        static_assert(!kGated || (kAlongK && kWaves % 2 == 0), "a wavefront's copies are all gate or all up rows");
         const int64_t row_bytes = 2 * o.stride;
+        const bool up = kGated && wave >= kWaves / 2;
         advance = kAlongK ? 2 * kSteps : kSteps * row_bytes;
+        at = kAlongK ? (const char*)o.p + ((up ? rows : 0) + first) * row_bytes + 2 * k0 : (const char*)o.p + k0 * row_bytes + 2 * first;
 #pragma unroll
         for (int c = 0; c < kCopies; c++) {
             const int copy = wave * kCopies + c;
             if constexpr (kAlongK) {
-                const bool up = kGated && 8 * copy >= kRows / 2;
-                const int row = 8 * copy + (lane >> 3), in_half = row - (up ? kRows / 2 : 0);
-                const int piece = (lane & 7) ^ ((row >> 1) & 7);
+                const int row = 16 * copy + (lane >> 2), in_half = row - (up ? kRows / 2 : 0);
+                const int piece = (lane & 3) ^ first_piece(row);
                 const int64_t left = rows - first - 1;
-                base[c] = (const char*)o.p + ((up ? rows : 0) + first) * row_bytes + 2 * k0;
                 voff[c] = (uint32_t)(min((int64_t)in_half, left) * row_bytes) + 16 * piece;
-                step[c] = 8 * piece;
             } else {
                 constexpr int kLanes = kRows / 8;   // of a step
                 const int k = copy * (64 / kLanes) + lane / kLanes;
-                const int piece = (lane % kLanes) ^ ((k & 3) << 2);
+                const int piece = (lane % kLanes) ^ turned_bits(k);
                 const int64_t left = rows - first - 8;
-                base[c] = (const char*)o.p + k0 * row_bytes + 2 * first;
                 voff[c] = (uint32_t)(k * row_bytes) + 2 * (uint32_t)min((int64_t)(8 * piece), left);
-                step[c] = k;
             }
         }
     }
-    __device__ void copy(int64_t stage, uint32_t lds, int wave) const {
-#pragma unroll
-        for (int c = 0; c < kCopies; c++) async_copy16(base[c] + stage * advance, voff[c], lds + (wave * kCopies + c) * 1024);
-    }
-    // the last stage, of which `left` steps are there
-    __device__ void copy_some(int64_t stage, uint32_t lds, int wave, int left) const {
-#pragma unroll
-        for (int c = 0; c < kCopies; c++) {
-            const char* from = base[c] + stage * advance + voff[c];
-            async_copy16_from(step[c] < left ? (const void*)from : (const void*)g_zeros, lds + (wave * kCopies + c) * 1024);
-        }
+    // lds: this wavefront's part of the stage
+    __device__ void copy(int c, uint32_t lds) const { async_copy16(at, voff[c], lds + c * 1024); }
+    // a stage of which only `left` steps are there
+    __device__ void copy_some(int c, uint32_t lds, int left, int wave, int lane) const {
+        const int copy = wave * kCopies + c;
+        const int step = kAlongK ? 8 * ((lane & 3) ^ first_piece(16 * copy + (lane >> 2))) : copy * (512 / kRows) + lane / (kRows / 8);
+        async_copy16_from(step < left ? (const void*)(at + voff[c]) : (const void*)g_zeros, lds + c * 1024);
     }
 };
 
-// Operands of kFrags blocks of 32 rows.  Element e of a lane: row lane % 32 of the block, step 16 s + 8 (lane / 32) + e.
-template <int kRows, bool kAlongK, int kFrags>
+// Operands of kFrags blocks of 16 rows.  Element e of a lane: row lane % 16 of the block, step 8 (lane / 16) + e.  A read's address is a
+// register and a constant: with an addition in front of every one the products of the large tile waited for their turn to be issued.
+template <int kRows, bool kAlongK, int kFrags, int kStage, int kStages>
 struct Reader {
-    uint32_t at[kAlongK ? kSteps / 16 : kFrags];
-    // block f's first row is f0 + 32 f, behind kSplit blocks f1 + 32 (f - kSplit)
-    __device__ void init(uint32_t lds, int f0, int lane) {
+    static constexpr int kReach = kStages / 2;   // stages that a read's constant reaches over, 64 KiB
+    uint32_t at[2][kAlongK ? 1 : kFrags];
+    __device__ void init(uint32_t lds, int first, int lane) {
+        static_assert(kReach * kStage <= 65536 && kStages % 2 == 0, "of 16 bits");
+        const int r = lane & 15, g = lane >> 4;
         if constexpr (kAlongK) {
-            const int r = lane & 31, h = lane >> 5;
-#pragma unroll
-            for (int s = 0; s < kSteps / 16; s++) at[s] = lds + (f0 + r) * (kSteps * 2) + (((2 * s + h) ^ ((r >> 1) & 7)) << 4);
+            at[0][0] = lds + (first + r) * (kSteps * 2) + ((g ^ first_piece(r)) << 4);
         } else {
-            const int rl = lane & 15, g = (lane >> 4) & 1, h = lane >> 5, k = 8 * h + (rl >> 2);
+            const int k = 8 * g + (r >> 2);   // and four further
 #pragma unroll
             for (int f = 0; f < kFrags; f++) {
-                const int piece = (f0 + 32 * f) / 8 + 2 * g + ((rl & 3) >> 1);
-                at[f] = lds + k * (kRows * 2) + ((piece ^ ((k & 3) << 2)) << 4) + 8 * (rl & 1);
+                const int piece = (first + 16 * f) / 8 + ((r & 3) >> 1);
+                at[0][f] = lds + k * (kRows * 2) + ((piece ^ turned_bits(k)) << 4) + 8 * (r & 1);
             }
         }
+#pragma unroll
+        for (int f = 0; f < (kAlongK ? 1 : kFrags); f++) {
+            at[1][f] = at[0][f] + kReach * kStage;
+            asm("" : "+v"(at[0][f]), "+v"(at[1][f]));   // kept, not worked out again
+        }
     }
-    // `jump`: bytes that the block lies further than 32 rows a block would put it
-    __device__ uint4 read(uint32_t stage, int s, int f, int jump) const {
+    // `jump`: bytes that the block lies further than 16 rows a block would put it
+    __device__ uint4 read(int stage, int f, int jump) const {
+        const int to = stage % kReach * kStage;
         if constexpr (kAlongK) {
-            const product_u32x4 v = *(const __attribute__((address_space(3))) product_u32x4*)(uintptr_t)(at[s] + stage + f * 32 * (kSteps * 2) + jump);
+            const product_u32x4 v = *(const __attribute__((address_space(3))) product_u32x4*)(uintptr_t)(at[stage / kReach][0] + (to + f * 16 * (kSteps * 2) + jump));
             return make_uint4(v[0], v[1], v[2], v[3]);
         } else {
             uint2 u[2];
 #pragma unroll
             for (int a = 0; a < 2; a++)
                 u[a] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) product_s16x4*)(uintptr_t)(
-                                                     at[f] + stage + (16 * s + 4 * a) * (kRows * 2))));
+                                                     at[stage / kReach][f] + (to + 4 * a * (kRows * 2)))));
             return make_uint4(u[0].x, u[0].y, u[1].x, u[1].y);
         }
     }
@@ -125,102 +158,150 @@ struct Reader {
 template <int kTileM, int kTileN>
 constexpr int kStageBytes = (kTileM + kTileN) * kSteps * 2;
 
-template <typename T, int kTileM, int kTileN, int kWavesM, int kWavesN, bool kAlongKA, bool kAlongKB, Epilogue kEpilogue>
-__global__ void __launch_bounds__(64 * kWavesM * kWavesN) tile_kernel(ProductParams p) {
+template <typename T, int kTileM, int kTileN, int kWavesM, int kWavesN, int kStages, bool kAlongKA, bool kAlongKB, Epilogue kEpilogue>
+__global__ void __launch_bounds__(64 * kWavesM * kWavesN, kTileM == 256 || kStages > 4 ? 1 : 2) tile_kernel(ProductParams p) {
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr bool kGated = kEpilogue == kGate;
-    constexpr int kWaves = kWavesM * kWavesN, kFragsM = kTileM / kWavesM / 32, kFragsN = kTileN / kWavesN / 32;
+    constexpr int kWaves = kWavesM * kWavesN, kFragsM = kTileM / kWavesM / 16, kFragsN = kTileN / kWavesN / 16;
     constexpr int kStage = kStageBytes<kTileM, kTileN>;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / kWavesN, wn = wave % kWavesN;
-    int tm, tn;
-    tile_of<4>(p, tm, tn);
+    int tm, tn, share;
+    float* sums = work_of<4>(p, kTileM * kTileN, tm, tn, share);
     const int64_t cols = kGated ? p.N / 2 : p.N;
     const int64_t m0 = (int64_t)tm * kTileM, n0 = (int64_t)tn * (kGated ? kTileN / 2 : kTileN);
-    const int64_t k0 = blockIdx.y * p.k_share, steps = min(p.K - k0, p.k_share);
+    const int64_t k0 = share * p.k_share, steps = sums ? min(p.K - k0, p.k_share) : p.K;
     const uint32_t lds = lds_address(smem);
 
     Side<kTileM, kAlongKA, kWaves> a;
     Side<kTileN, kAlongKB, kWaves> b;
     a.template init<false>(p.a, m0, p.M, k0, wave, lane);
     b.template init<kGated>(p.b, n0, cols, k0, wave, lane);
-    Reader<kTileM, kAlongKA, kFragsM> ra;
-    Reader<kTileN, kAlongKB, kFragsN> rb;
+    Reader<kTileM, kAlongKA, kFragsM, kStage, kStages> ra;
+    Reader<kTileN, kAlongKB, kFragsN, kStage, kStages> rb;
     ra.init(lds, wm * (kTileM / kWavesM), lane);
     rb.init(lds + Side<kTileM, kAlongKA, kWaves>::kBytes, kGated ? wn * (kTileN / kWavesN / 2) : wn * (kTileN / kWavesN), lane);
     // with the gate, a wavefront's second half of blocks are the up columns of its first
     constexpr int kJump = kGated ? (kTileN / 2 - kTileN / kWavesN / 2) * kSteps * 2 : 0;
 
-    const int64_t whole = steps / kSteps, stages = (steps + kSteps - 1) / kSteps;
-    auto copy = [&](int64_t stage) {
-        const uint32_t to = lds + (uint32_t)(stage & 1) * kStage, to_b = to + Side<kTileM, kAlongKA, kWaves>::kBytes;
-        if (stage < whole) {
-            a.copy(stage, to, wave);
-            b.copy(stage, to_b, wave);
-        } else {
-            const int left = (int)(steps - stage * kSteps);
-            a.copy_some(stage, to, wave, left);
-            b.copy_some(stage, to_b, wave, left);
-        }
+    using SideA = Side<kTileM, kAlongKA, kWaves>;
+    using SideB = Side<kTileN, kAlongKB, kWaves>;
+    const int whole = (int)(steps / (kStages * kSteps)) * kStages, left = (int)(steps % (kStages * kSteps));   // stages; steps behind them
+    constexpr int kCopiesA = SideA::kCopies, kCopies = kCopiesA + SideB::kCopies;
+    const uint32_t mine_a = lds + wave * (kCopiesA * 1024), mine_b = lds + SideA::kBytes + wave * (SideB::kCopies * 1024);
+    auto copy = [&](int c, uint32_t stage_at) {
+        if (c < kCopiesA) a.copy(c, mine_a + stage_at);
+        else b.copy(c - kCopiesA, mine_b + stage_at);
     };
-    f32x16_t acc[kFragsM][kFragsN] = {};
-    copy(0);
-    for (int64_t stage = 0; stage < stages; stage++) {
+    int ahead = 0;   // the stage that is copied next; behind the last whole one that one is brought again, to nobody's use
+    auto next = [&] {
+        ahead++;
+        a.at += ahead < whole ? a.advance : 0;
+        b.at += ahead < whole ? b.advance : 0;
+    };
+    f32x4_t acc[kFragsM][kFragsN] = {};
+    asm volatile("s_nop 7" ::: "memory");
+    uint4 av[2][kFragsM], bv[2][kFragsN];
+    constexpr int kReads = kFragsM + kFragsN, kProducts = kFragsM * kFragsN;
+    auto read = [&](int n, int buf, int stage) {   // in the order in which the products want them
+        if (n == 0) bv[buf][0] = rb.read(stage, 0, 0);
+        else if (n <= kFragsM) av[buf][n - 1] = ra.read(stage, n - 1, 0);
+        else bv[buf][n - kFragsM] = rb.read(stage, n - kFragsM, n - kFragsM >= kFragsN / 2 ? kJump : 0);
+    };
+    // The products of the stage whose operands are in registers, and between them the next one's operands and copies to its own place.
+    auto step = [&](auto stage_) {
+        constexpr int stage = decltype(stage_)::value, next_stage = (stage + 1) % kStages;
+        each<kProducts>([&](auto n_) {
+            constexpr int n = decltype(n_)::value, j = n / kFragsM, i = n % kFragsM;
+            mma<T>(bv[stage % 2][j], av[stage % 2][i], acc[i][j]);
+            constexpr int kEarly = kProducts * 3 / 4;
+            if constexpr (n < kEarly) {
+                constexpr int first = n * kReads / kEarly, end = (n + 1) * kReads / kEarly;
+                each<end - first>([&](auto x) { read(first + decltype(x)::value, next_stage % 2, next_stage); });
+            }
+            constexpr int from = n * kCopies / kProducts, to = (n + 1) * kCopies / kProducts;
+            each<to - from>([&](auto x) { copy(from + decltype(x)::value, stage * kStage); });
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        next();
+    };
+    if (whole > 0) {
+        each<kStages>([&](auto st) {
+            each<kCopies>([&](auto c) { copy(decltype(c)::value, decltype(st)::value * kStage); });
+            next();
+        });
+        wait_copies<(kStages - 1) * kCopies>();
+        __syncthreads();
+        each<kReads>([&](auto n) { read(decltype(n)::value, 0, 0); });
+        for (int stage = 0; stage < whole; stage += kStages)
+            each<kStages>([&](auto st) {
+                // Everybody has this stage's operands in registers, so it may be copied over, and the next one is there.
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                wait_copies<(kStages - 2) * kCopies>();
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                step(st);
+            });
+        sums_done(acc);
         wait_copies<0>();
-        __syncthreads();   // everybody's copies are there, and nobody reads the other stage any more
-        if (stage + 1 < stages) copy(stage + 1);
-        const uint32_t at = (uint32_t)(stage & 1) * kStage;
-#pragma unroll
-        for (int s = 0; s < kSteps / 16; s++) {
-            uint4 av[kFragsM], bv[kFragsN];
-#pragma unroll
-            for (int i = 0; i < kFragsM; i++) av[i] = ra.read(at, s, i, 0);
-#pragma unroll
-            for (int j = 0; j < kFragsN; j++) bv[j] = rb.read(at, s, j, j >= kFragsN / 2 ? kJump : 0);
-#pragma unroll
-            for (int i = 0; i < kFragsM; i++)
-#pragma unroll
-                for (int j = 0; j < kFragsN; j++) acc[i][j] = mma<T>(bv[j], av[i], acc[i][j]);
-        }
+        __syncthreads();
     }
-
-    // Accumulator element r of a lane: row lane % 32 of C's block, column 8 (r / 4) + 4 (lane / 32) + r % 4.
-    const int r32 = lane & 31, h = lane >> 5;
-    const int64_t mw = m0 + wm * (kTileM / kWavesM), nw = n0 + wn * (kGated ? kTileN / kWavesN / 2 : kTileN / kWavesN);
-    if (p.partial) {
+    if (left) {   // last stages, one of which may not be whole
+        if (whole > 0) {
+            a.at += a.advance;
+            b.at += b.advance;
+        }
 #pragma unroll
-        for (int i = 0; i < kFragsM; i++) {
-            const int64_t m = mw + 32 * i + r32;
-            float* row = p.partial + (blockIdx.y * p.M + m) * p.N;
+        for (int st = 0; st < kStages; st++) {
+            if (st * kSteps < left) {
 #pragma unroll
-            for (int j = 0; j < kFragsN; j++) {
-                const bool up = kGated && j >= kFragsN / 2;
-                const int64_t n = nw + 32 * (up ? j - kFragsN / 2 : j);
-#pragma unroll
-                for (int q = 0; q < 4; q++)
-                    if (m < p.M && n + 8 * q < cols)
-                        *reinterpret_cast<float4*>(row + (up ? cols : 0) + n + 8 * q + 4 * h) =
-                            make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+                for (int c = 0; c < kCopies; c++)
+                    if (c < kCopiesA) a.copy_some(c, mine_a + st * kStage, left - st * kSteps, wave, lane);
+                    else b.copy_some(c - kCopiesA, mine_b + st * kStage, left - st * kSteps, wave, lane);
+                a.at += a.advance;
+                b.at += b.advance;
             }
         }
+        wait_copies<0>();
+        __syncthreads();
+#pragma unroll
+        for (int st = 0; st < kStages; st++) {
+            if (st * kSteps < left) {
+#pragma unroll
+                for (int n = 0; n < kReads; n++) read(n, 0, st);
+#pragma unroll
+                for (int n = 0; n < kProducts; n++) mma<T>(bv[0][n / kFragsM], av[0][n % kFragsM], acc[n % kFragsM][n / kFragsM]);
+            }
+        }
+        sums_done(acc);
+    }
+
+    // Accumulator element r of a lane: row lane % 16 of C's block, column 4 (lane / 16) + r.
+    const int r16 = lane & 15, c4 = 4 * (lane >> 4);
+    const int64_t mw = m0 + wm * (kTileM / kWavesM), nw = n0 + wn * (kGated ? kTileN / kWavesN / 2 : kTileN / kWavesN);
+    if (sums) {
+        float* to = sums + (int64_t)(wm * (kTileM / kWavesM) + r16) * kTileN + (kGated ? wn * (kTileN / kWavesN / 2) : wn * (kTileN / kWavesN)) + c4;
+#pragma unroll
+        for (int i = 0; i < kFragsM; i++)
+#pragma unroll
+            for (int j = 0; j < kFragsN; j++)
+                *reinterpret_cast<float4*>(to + 16 * i * kTileN + 16 * j + (kGated && j >= kFragsN / 2 ? kTileN / 2 - kTileN / kWavesN / 2 : 0)) =
+                    make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
         return;
     }
-    // 32 rows at a time go through the wavefront's part of LDS, so that whole pieces of a row are written at a time.
+    // 16 rows at a time go through the wavefront's part of LDS, so that whole pieces of a row are written at a time.
     __syncthreads();
-    constexpr int kBlocks = kGated ? kFragsN / 2 : kFragsN, kPieces = kBlocks * 4, kPitch = kBlocks * 64 + 16;
-    unsigned char* mine = smem + wave * (32 * kPitch);
+    constexpr int kBlocks = kGated ? kFragsN / 2 : kFragsN, kPieces = kBlocks * 2, kPitch = kBlocks * 32 + 16;
+    unsigned char* mine = smem + wave * (16 * kPitch);
     auto write = [&](int i, auto value, void* out, int64_t stride, int64_t first) {
 #pragma unroll
         for (int j = 0; j < kBlocks; j++)
-#pragma unroll
-            for (int q = 0; q < 4; q++)
-                *reinterpret_cast<uint2*>(mine + r32 * kPitch + (32 * j + 8 * q + 4 * h) * 2) =
-                    pack4<T>(value(j, 4 * q), value(j, 4 * q + 1), value(j, 4 * q + 2), value(j, 4 * q + 3));
+            *reinterpret_cast<uint2*>(mine + r16 * kPitch + (16 * j + c4) * 2) = pack4<T>(value(j, 0), value(j, 1), value(j, 2), value(j, 3));
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         const int piece = lane % kPieces;
 #pragma unroll
-        for (int x = 0; x < 32 * kPieces / 64; x++) {
+        for (int x = 0; x < 16 * kPieces / 64; x++) {
             const int row = x * (64 / kPieces) + lane / kPieces;
-            const int64_t m = mw + 32 * i + row, n = nw + 8 * piece;
+            const int64_t m = mw + 16 * i + row, n = nw + 8 * piece;
             const uint4 v = *reinterpret_cast<const uint4*>(mine + row * kPitch + piece * 16);
             if (m < p.M && n < cols) *reinterpret_cast<uint4*>((T*)out + m * stride + first + n) = v;
         }
@@ -237,53 +318,74 @@ __global__ void __launch_bounds__(64 * kWavesM * kWavesN) tile_kernel(ProductPar
         } else {
             write(i, [&](int j, int r) { return acc[i][j][r]; }, p.out, p.N, 0);
         }
+        __builtin_amdgcn_sched_barrier(0);
     }
 }
 
-template <typename T, int kTileM, int kTileN, int kWavesM, int kWavesN, bool kAlongKA, bool kAlongKB, Epilogue kEpilogue>
+template <typename T, int kTileM, int kTileN, int kStages, bool kAlongKA, bool kAlongKB, Epilogue kEpilogue>
 int launch_tiles(const ProductParams& p, const TilePlan& plan, hipStream_t stream) {
-    auto kernel = tile_kernel<T, kTileM, kTileN, kWavesM, kWavesN, kAlongKA, kAlongKB, kEpilogue>;
-    constexpr int lds = 2 * kStageBytes<kTileM, kTileN>;
+    auto kernel = tile_kernel<T, kTileM, kTileN, 2, 2, kStages, kAlongKA, kAlongKB, kEpilogue>;
+    constexpr int lds = kStages * kStageBytes<kTileM, kTileN>;
     if (int rc = ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), lds)) return rc;
-    hipLaunchKernelGGL(kernel, dim3(plan.tiles_m * plan.tiles_n, plan.shares), dim3(64 * kWavesM * kWavesN), lds, stream, p);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)plan.blocks()), dim3(256), lds, stream, p);
     CKV_HIP_TRY(hipGetLastError());
     return CKV_OK;
 }
 
 template <typename T, bool kAlongKA, bool kAlongKB, Epilogue kEpilogue>
 int launch_tiles(const ProductParams& p, const TilePlan& plan, hipStream_t stream) {
-    if (plan.tile_m == 256) return launch_tiles<T, 256, 256, 4, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
-    if (plan.tile_m == 128) return launch_tiles<T, 128, 128, 2, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
-    if constexpr (kAlongKA) return launch_tiles<T, 64, 128, 2, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
+    if (plan.tile_m == 256) return launch_tiles<T, 256, 256, 4, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
+    if (plan.tile_m == 128 && plan.stages == 4) return launch_tiles<T, 128, 128, 4, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
+    if (plan.tile_m == 128) return launch_tiles<T, 128, 128, 8, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
+    if constexpr (kAlongKA) return launch_tiles<T, 64, 128, 8, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
     return CKV_ERR_UNSUPPORTED;
 }
 
+// A kind of tile, and microseconds that its workgroups take on a compute unit, `resident` of them at a time: a stage, and around the stages.
+struct Kind {
+    int tile_m, tile_n, stages, resident;
+    double stage_us, around_us;
+};
+constexpr Kind kKinds[] = {{256, 256, 4, 1, 0.73, 8.0}, {128, 128, 4, 2, 0.60, 1.8}, {128, 128, 8, 1, 0.33, 4.0}, {64, 128, 8, 1, 0.17, 3.0}};
+
 }  // namespace
 
-TilePlan plan_tiles(int64_t M, int64_t N, int64_t K, bool a_along_k, bool gated, int cus) {
-    TilePlan r;
-    auto tiles = [&](int tm, int tn) { return ((M + tm - 1) / tm) * ((N + tn - 1) / tn); };
-    r.tile_m = a_along_k && M <= 64 ? 64 : tiles(256, 256) < cus ? 128 : 256;
-    r.tile_n = r.tile_m == 256 ? 256 : 128;
-    r.tiles_m = (int)((M + r.tile_m - 1) / r.tile_m);
-    r.tiles_n = (int)(((gated ? N / 2 : N) + r.tile_n / (gated ? 2 : 1) - 1) / (r.tile_n / (gated ? 2 : 1)));
-    const int64_t all = (int64_t)r.tiles_m * r.tiles_n;
-    const int64_t shares = std::max<int64_t>(1, std::min<int64_t>(2 * cus / all, K / 512));
-    r.k_share = ((K + shares - 1) / shares + kSteps - 1) / kSteps * kSteps;
-    r.shares = (int)((K + r.k_share - 1) / r.k_share);
-    return r;
+// Tiles fill the compute units round by round; those of the last round may be shared out along k, which costs their sums a trip to memory (4
+// TB/s both ways, 3 us the launch that adds them up).
+TilePlan plan_tiles(int64_t M, int64_t N, int64_t K, bool a_along_k, int cus) {
+    TilePlan best = {};
+    double best_us = 0;
+    const double stages = (double)((K + kSteps - 1) / kSteps);
+    for (const Kind& kind : kKinds) {
+        if (kind.tile_m == 64 && !a_along_k) continue;
+        const int64_t tiles_m = (M + kind.tile_m - 1) / kind.tile_m, tiles_n = (N + kind.tile_n - 1) / kind.tile_n, all = tiles_m * tiles_n;
+        const int64_t places = (int64_t)cus * kind.resident, rest = all % places;
+        for (int shares = 1; shares <= 8; shares++) {
+            if (shares > 1 && (rest == 0 || K / shares < 256)) break;
+            const int64_t k_share = shares == 1 ? K : ((K + shares - 1) / shares + kSteps * kind.stages - 1) / (kSteps * kind.stages) * (kSteps * kind.stages);
+            const int real = (int)((K + k_share - 1) / k_share);
+            if (real != shares) continue;
+            // several to a unit: the last of them run beside each other
+            double rounds = kind.resident == 1 ? (double)((rest * shares + cus - 1) / cus) : std::max(0.5, (double)rest * shares / places);
+            if (rest == 0) rounds = 0;
+            double us = (double)(all / places) * (stages * kind.stage_us + kind.around_us) + rounds * ((double)k_share / kSteps * kind.stage_us + kind.around_us);
+            if (shares > 1) us += 3.0 + (double)(rest * shares) * kind.tile_m * kind.tile_n * 8 / 4e6;
+            if (best_us == 0 || us < best_us) {
+                best_us = us;
+                best = TilePlan{kind.tile_m, kind.tile_n, kind.stages, (int)tiles_m, (int)tiles_n, (int)(all - rest), shares, k_share};
+            }
+        }
+    }
+    return best;
 }
 
 template <typename T>
-int run_tiles(ProductParams& p, const TilePlan& plan, bool a_along_k, bool b_along_k, Epilogue epilogue, hipStream_t stream) {
-    p.tiles_m = plan.tiles_m;
-    p.tiles_n = plan.tiles_n;
-    p.k_share = plan.k_share;
+int run_tiles(const ProductParams& p, const TilePlan& plan, bool a_along_k, Epilogue epilogue, hipStream_t stream) {
     if (epilogue == kGate) return launch_tiles<T, true, true, kGate>(p, plan, stream);
     if (a_along_k) return launch_tiles<T, true, false, kStore>(p, plan, stream);
     return launch_tiles<T, false, false, kStore>(p, plan, stream);
 }
-template int run_tiles<__half>(ProductParams&, const TilePlan&, bool, bool, Epilogue, hipStream_t);
-template int run_tiles<__hip_bfloat16>(ProductParams&, const TilePlan&, bool, bool, Epilogue, hipStream_t);
+template int run_tiles<__half>(const ProductParams&, const TilePlan&, bool, Epilogue, hipStream_t);
+template int run_tiles<__hip_bfloat16>(const ProductParams&, const TilePlan&, bool, Epilogue, hipStream_t);
 
 }  // namespace ckv

@@ -56,7 +56,7 @@ def inputs(m, k, i, dtype, seed=0):
 
 SIZES = [  # rows, k, inter
     (1, 1, 1), (3, 7, 5), (2, 64, 16), (1, 256, 512), (17, 130, 66), (65, 129, 63), (129, 512, 64), (16, 4096, 32), (130, 72, 200),
-    (255, 1000, 136), (1030, 136, 8200), (4104, 4104, 72), (77, 4104, 2056), (300, 64, 1000), (64, 4096, 264), (513, 264, 520), (5, 2056, 8), (257, 8, 256), (1000, 2048, 16), (9, 520, 2048),
+    (255, 1000, 136), (1030, 136, 8200), (4104, 4104, 72), (77, 4104, 2056), (513, 2056, 4104), (40, 3592, 9480), (130, 1544, 9480), (300, 64, 1000), (64, 4096, 264), (513, 264, 520), (5, 2056, 8), (257, 8, 256), (1000, 2048, 16), (9, 520, 2048),
 ]
 
 
