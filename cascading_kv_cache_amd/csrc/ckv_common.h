@@ -70,6 +70,11 @@ __device__ inline T gated(T gate, T up) {
     return Elem<T>::from_float(s * Elem<T>::to_float(up));
 }
 
+// silu(g) * u.  The exponential by the hardware's exp2, whose argument is rounded: |g| 2^-24 relative, of what is added to one.
+__device__ inline float gate_product(float g, float u) {
+    return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.44269504f)) * u;
+}
+
 // stage timing hooks (ckv_profile_enable / ckv_profile_read); no-ops while disabled
 void prof_begin(int stage, hipStream_t stream);
 void prof_end(int stage, hipStream_t stream);

@@ -298,6 +298,8 @@ int run_product(ProductParams& p, const DeviceInfo& di, void* workspace, int64_t
     return CKV_OK;
 }
 
+constexpr int64_t kFewRows = 16, kFewBytes = 118 << 10;
+
 int check_sizes(int64_t rows, int64_t inter, int64_t k, int64_t x_stride, int32_t dtype) {
     if (dtype != CKV_F32 && dtype != CKV_F16 && dtype != CKV_BF16) return CKV_ERR_DTYPE;
     if (rows < 0 || inter <= 0 || k <= 0 || x_stride < k) return CKV_ERR_SHAPE;
@@ -308,6 +310,13 @@ int check_sizes(int64_t rows, int64_t inter, int64_t k, int64_t x_stride, int32_
 template <typename T>
 int run_forward(const void* x, const void* w, void* out, void* gate_up, int64_t rows, int64_t inter, int64_t k, int64_t x_stride, void* workspace,
                 int64_t bytes, const DeviceInfo& di, hipStream_t stream) {
+    // A few rows wait for the weights, and the kernel of a decoding step's products streams them through LDS beside the rows (28672 x 4096, a
+    // row: 39.3 us, tiles 52; twelve rows 43 and 53; sixteen, whose rows leave no room for the streams, 59 and 49; sixteen of 3584: 47 and 61).
+    if (sizeof(T) == 2 && rows <= kFewRows && rows * (2 * k + 16) <= kFewBytes && !gate_up && inter % 8 == 0 && k % 64 == 0 && (rows == 1 || x_stride % 8 == 0) &&
+        ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(out)) & 15) == 0) {
+        const int rc = ckv_linear_rows(x, w, nullptr, nullptr, nullptr, 0.f, out, rows, 2 * inter, k, rows == 1 ? k : x_stride, 2, 1, 1, Elem<T>::code, stream);
+        if (rc != CKV_ERR_UNSUPPORTED) return rc;   // rows too long for LDS
+    }
     ProductParams p = {};
     p.a = Operand{x, x_stride};
     p.b = Operand{w, k};

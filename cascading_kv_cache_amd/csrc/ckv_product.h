@@ -27,11 +27,6 @@ struct ProductParams {
 
 enum Epilogue { kStore, kGate };
 
-// silu(g) * u.  The exponential by the hardware's exp2, whose argument is rounded: |g| 2^-24 relative, of what is added to one.
-__device__ inline float gate_product(float g, float u) {
-    return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.44269504f)) * u;
-}
-
 // Workgroups go round the eight XCDs: each gets a stretch of the tiles, and behind those one of the shares.  Tiles are numbered in bands
 // kHigh tiles of M high, so that the tiles of a stretch that run at a time share operands in its L2.
 __device__ inline int stretch(int block, int all) {

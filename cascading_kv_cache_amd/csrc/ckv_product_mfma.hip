@@ -172,19 +172,19 @@ __global__ void __launch_bounds__(64 * kWavesM * kWavesN, kTileM == 256 || kStag
     const int64_t k0 = share * p.k_share, steps = sums ? min(p.K - k0, p.k_share) : p.K;
     const uint32_t lds = lds_address(smem);
 
-    Side<kTileM, kAlongKA, kWaves> a;
-    Side<kTileN, kAlongKB, kWaves> b;
+    using SideA = Side<kTileM, kAlongKA, kWaves>;
+    using SideB = Side<kTileN, kAlongKB, kWaves>;
+    SideA a;
+    SideB b;
     a.template init<false>(p.a, m0, p.M, k0, wave, lane);
     b.template init<kGated>(p.b, n0, cols, k0, wave, lane);
     Reader<kTileM, kAlongKA, kFragsM, kStage, kStages> ra;
     Reader<kTileN, kAlongKB, kFragsN, kStage, kStages> rb;
     ra.init(lds, wm * (kTileM / kWavesM), lane);
-    rb.init(lds + Side<kTileM, kAlongKA, kWaves>::kBytes, kGated ? wn * (kTileN / kWavesN / 2) : wn * (kTileN / kWavesN), lane);
+    rb.init(lds + SideA::kBytes, kGated ? wn * (kTileN / kWavesN / 2) : wn * (kTileN / kWavesN), lane);
     // with the gate, a wavefront's second half of blocks are the up columns of its first
     constexpr int kJump = kGated ? (kTileN / 2 - kTileN / kWavesN / 2) * kSteps * 2 : 0;
 
-    using SideA = Side<kTileM, kAlongKA, kWaves>;
-    using SideB = Side<kTileN, kAlongKB, kWaves>;
     const int whole = (int)(steps / (kStages * kSteps)) * kStages, left = (int)(steps % (kStages * kSteps));   // stages; steps behind them
     constexpr int kCopiesA = SideA::kCopies, kCopies = kCopiesA + SideB::kCopies;
     const uint32_t mine_a = lds + wave * (kCopiesA * 1024), mine_b = lds + SideA::kBytes + wave * (SideB::kCopies * 1024);
@@ -192,11 +192,18 @@ __global__ void __launch_bounds__(64 * kWavesM * kWavesN, kTileM == 256 || kStag
         if (c < kCopiesA) a.copy(c, mine_a + stage_at);
         else b.copy(c - kCopiesA, mine_b + stage_at);
     };
-    int ahead = 0;   // the stage that is copied next; behind the last whole one that one is brought again, to nobody's use
+    // The stage that is copied next.  Behind the last whole one comes the first again (to nobody's use, where that is where it began).  Few rows
+    // wait for the bytes of B, and workgroups that go through its rows side by side ask for the same few channels of memory at a time: they begin
+    // in different places (32 x 28672 x 4096: 62.7 -> 55.2 us.  Where B's steps are its rows, which they share, not: 58 -> 67).
+    int ahead = kStages > 4 && kAlongKB && whole > 0 ? (int)((blockIdx.x * 2654435761u >> 8) % (uint32_t)whole) : 0;
+    const int64_t back_a = (1 - whole) * a.advance, back_b = (1 - whole) * b.advance;
+    a.at += ahead * a.advance;
+    b.at += ahead * b.advance;
     auto next = [&] {
-        ahead++;
-        a.at += ahead < whole ? a.advance : 0;
-        b.at += ahead < whole ? b.advance : 0;
+        const bool last = ahead + 1 >= whole;
+        a.at += last ? back_a : a.advance;
+        b.at += last ? back_b : b.advance;
+        ahead = last ? 0 : ahead + 1;
     };
     f32x4_t acc[kFragsM][kFragsN] = {};
     asm volatile("s_nop 7" ::: "memory");
@@ -246,10 +253,8 @@ __global__ void __launch_bounds__(64 * kWavesM * kWavesN, kTileM == 256 || kStag
         __syncthreads();
     }
     if (left) {   // last stages, one of which may not be whole
-        if (whole > 0) {
-            a.at += a.advance;
-            b.at += b.advance;
-        }
+        a.at += (whole - ahead) * a.advance;
+        b.at += (whole - ahead) * b.advance;
 #pragma unroll
         for (int st = 0; st < kStages; st++) {
             if (st * kSteps < left) {
@@ -336,17 +341,18 @@ template <typename T, bool kAlongKA, bool kAlongKB, Epilogue kEpilogue>
 int launch_tiles(const ProductParams& p, const TilePlan& plan, hipStream_t stream) {
     if (plan.tile_m == 256) return launch_tiles<T, 256, 256, 4, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
     if (plan.tile_m == 128 && plan.stages == 4) return launch_tiles<T, 128, 128, 4, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
-    if (plan.tile_m == 128) return launch_tiles<T, 128, 128, 8, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
-    if constexpr (kAlongKA) return launch_tiles<T, 64, 128, 8, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
+    if constexpr (kAlongKA)
+        return plan.tile_m == 128 ? launch_tiles<T, 128, 128, 8, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream)
+                                  : launch_tiles<T, 64, 128, 8, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
     return CKV_ERR_UNSUPPORTED;
 }
 
 // A kind of tile, and microseconds that its workgroups take on a compute unit, `resident` of them at a time: a stage, and around the stages.
 struct Kind {
     int tile_m, tile_n, stages, resident;
-    double stage_us, around_us;
+    double stage_us, around_us, first_us;   // first_us: where others hide what is around the stages, once a launch
 };
-constexpr Kind kKinds[] = {{256, 256, 4, 1, 0.73, 8.0}, {128, 128, 4, 2, 0.60, 1.8}, {128, 128, 8, 1, 0.33, 4.0}, {64, 128, 8, 1, 0.17, 3.0}};
+constexpr Kind kKinds[] = {{256, 256, 4, 1, 0.73, 8.5, 0}, {128, 128, 4, 2, 0.65, 1.0, 8.0}, {128, 128, 8, 1, 0.33, 4.0, 0}, {64, 128, 8, 1, 0.17, 3.0, 0}};
 
 }  // namespace
 
@@ -357,18 +363,21 @@ TilePlan plan_tiles(int64_t M, int64_t N, int64_t K, bool a_along_k, int cus) {
     double best_us = 0;
     const double stages = (double)((K + kSteps - 1) / kSteps);
     for (const Kind& kind : kKinds) {
-        if (kind.tile_m == 64 && !a_along_k) continue;
+        const bool few = kind.stages > 4;   // rows, all of them in a tile: bound by the bytes of B, for which there are more stages
+        if (few && (!a_along_k || M > kind.tile_m)) continue;
         const int64_t tiles_m = (M + kind.tile_m - 1) / kind.tile_m, tiles_n = (N + kind.tile_n - 1) / kind.tile_n, all = tiles_m * tiles_n;
         const int64_t places = (int64_t)cus * kind.resident, rest = all % places;
         for (int shares = 1; shares <= 8; shares++) {
-            if (shares > 1 && (rest == 0 || K / shares < 256)) break;
+            // Behind full rounds of products compute units may idle: the others' clock rises (2048 x 37888 x 3584, 4.6 rounds: 457 us, 485 with the
+            // rest in three shares), unless it is bytes they wait for (77 x 37888 x 3584, 1.2 rounds: 82 us, 69 in five).
+            if (shares > 1 && (rest == 0 || K / shares < 256 || (!few && all > places))) break;
             const int64_t k_share = shares == 1 ? K : ((K + shares - 1) / shares + kSteps * kind.stages - 1) / (kSteps * kind.stages) * (kSteps * kind.stages);
             const int real = (int)((K + k_share - 1) / k_share);
             if (real != shares) continue;
-            // several to a unit: the last of them run beside each other
-            double rounds = kind.resident == 1 ? (double)((rest * shares + cus - 1) / cus) : std::max(0.5, (double)rest * shares / places);
-            if (rest == 0) rounds = 0;
-            double us = (double)(all / places) * (stages * kind.stage_us + kind.around_us) + rounds * ((double)k_share / kSteps * kind.stage_us + kind.around_us);
+            double rounds = (double)((rest * shares + cus - 1) / cus);
+            if (kind.resident > 1)   // they start as others end; one alone on a unit is the faster for it
+                rounds = rest * shares <= cus && all < places ? 0.55 : all > places ? (double)rest / places : std::max(1.0, (double)rest * shares / places);
+            double us = kind.first_us + (double)(all / places) * (stages * kind.stage_us + kind.around_us) + rounds * ((double)k_share / kSteps * kind.stage_us + kind.around_us);
             if (shares > 1) us += 3.0 + (double)(rest * shares) * kind.tile_m * kind.tile_n * 8 / 4e6;
             if (best_us == 0 || us < best_us) {
                 best_us = us;

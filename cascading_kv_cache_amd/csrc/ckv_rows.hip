@@ -37,6 +37,7 @@ struct RowsParams {
     const void* norm;       // (K) weights of the RMSNorm in front, or null
     void* out;              // (rows, N); gated: (rows, N / 2)
     float eps;
+    bool once;              // gated: the product is rounded, and not what it is made of
     int rows, N, K;
     int64_t x_stride;
     // kCut: tiles of cut_groups groups from tile cut_first on are cut, see cut_of
@@ -235,7 +236,7 @@ __global__ void __launch_bounds__(64 * kMostWaves<kParts>) rows_kernel(RowsParam
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             const float up = __shfl_xor(acc[e], 32);
-            o.v[e] = gated<T>(Elem<T>::from_float(acc[e]), Elem<T>::from_float(up));
+            o.v[e] = p.once ? Elem<T>::from_float(gate_product(acc[e], up)) : gated<T>(Elem<T>::from_float(acc[e]), Elem<T>::from_float(up));
         }
         if (live && r < p.rows && q < 2) *reinterpret_cast<Out*>((T*)p.out + (int64_t)r * (p.N / 2) + group * 8 + 4 * q) = o;
     } else {
@@ -344,6 +345,7 @@ extern "C" int ckv_linear_rows(const void* x, const void* w, const void* bias, c
     RowsParams p;
     p.x = x; p.w = w; p.bias = bias; p.residual = residual; p.norm = norm; p.out = out;
     p.eps = eps;
+    p.once = gated == 2;
     p.rows = (int)rows; p.N = (int)n; p.K = (int)k;
     p.x_stride = x_stride;
     p.cut_groups = 1; p.cut_first = 0; p.cut_span = 0; p.cut_length = 1;

@@ -322,7 +322,8 @@ int ckv_gated_silu(const void* gate_up, void* out, int64_t rows, int64_t inter, 
 /* out = x W^T of a few rows (a decoding step's projections), x (rows <= 16, k), W (n, k) contiguous, 16-bit, n % 16 == 0, k % 64 == 0,
  * x and W 16-byte aligned.  Optional: `norm` (k): RMSNorm of the rows with `eps` in front, rounded to the tensor dtype; `bias` (n), added
  * in float32; `residual` (rows, n), added to the rounded product; `gated`: W holds n / 2 gate rows and n / 2 up rows, out
- * (rows, n / 2) = silu(gate) * up as ckv_gated_silu has it (no bias or residual then; parts 1).  The float32 sum of an output is made of
+ * (rows, n / 2) = silu(gate) * up as ckv_gated_silu has it, or with 2 rounded once as ckv_gated_linear has it (no bias or residual then;
+ * parts 1).  The float32 sum of an output is made of
  * `parts` chains of matrix instructions, added in order: part p takes stretches p, p + parts, ... of `unit` * 64 elements; (parts, unit)
  * is (1, 1), (2, 2), (4, 1) or (4, 2).  (1, 1 + 256 runs) and (4, 1 + 256 runs), not gated: as a library sums up that deals tiles of 256
  * rows of W and 64 elements (four parts: of 32 rows and 256 elements) out over `runs` <= 1024 workgroups, n of at least `runs` tiles,
