@@ -17,53 +17,48 @@ namespace {
 
 constexpr int kTile = 128, kStep = 16, kPitch = kTile + 4;
 
-// A thread's eight elements of a tile of 128 rows and 16 steps: along k of one row, or along the rows of one step.
+// A thread's four elements of a tile of 128 rows and 16 steps: along k of one row, or along the rows of one step.  Inside the operand they are
+// read at a time, from whatever address (an odd number of float32 a row: 1023 columns, 509 rows and 5462, 64 us by elements and 52 so).
 template <typename T, bool kAlongK>
 struct Piece {
+    struct __attribute__((packed, aligned(sizeof(T)))) Four {
+        T v[4];
+    };
     int row, step;   // of the first
-    float v[8];
+    float v[4];
     __device__ Piece() {
-        row = kAlongK ? threadIdx.x >> 1 : (threadIdx.x & 15) * 8;
-        step = kAlongK ? (threadIdx.x & 1) * 8 : threadIdx.x >> 4;
+        row = kAlongK ? threadIdx.x >> 2 : (threadIdx.x & 31) * 4;
+        step = kAlongK ? (threadIdx.x & 3) * 4 : threadIdx.x >> 5;
     }
     // base: the operand's row 0; `first` the tile's first row, counted from base; rows behind `rows` and steps behind `end` are zeros
-    __device__ void load(const T* base, int64_t stride, int64_t first, int64_t rows, int64_t k, int64_t end, bool vectors) {
+    __device__ void load(const T* base, int64_t stride, int64_t first, int64_t rows, int64_t k, int64_t end) {
         const int64_t r = first + row, s = k + step;
         const T* at = base + (kAlongK ? r * stride + s : s * stride + r);
-        const bool whole = kAlongK ? r < rows && s + 8 <= end : s < end && r + 8 <= rows;
-        if (vectors && whole) {
-            struct alignas(16) Sixteen {
-                T v[16 / sizeof(T)];
-            };
-            constexpr int kPer = 16 / sizeof(T);
+        if (kAlongK ? r < rows && s + 4 <= end : s < end && r + 4 <= rows) {
+            const Four x = *reinterpret_cast<const Four*>(at);
 #pragma unroll
-            for (int i = 0; i < 8 / kPer; i++) {
-                const Sixteen x = reinterpret_cast<const Sixteen*>(at)[i];
-#pragma unroll
-                for (int e = 0; e < kPer; e++) v[i * kPer + e] = Elem<T>::to_float(x.v[e]);
-            }
+            for (int i = 0; i < 4; i++) v[i] = Elem<T>::to_float(x.v[i]);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
+            for (int i = 0; i < 4; i++) {
                 const bool there = kAlongK ? r < rows && s + i < end : s < end && r + i < rows;
                 v[i] = there ? Elem<T>::to_float(at[i]) : 0.f;
             }
         }
     }
-    __device__ void store(float (*tile)[kPitch], int row_in_tile) const {
+    __device__ void store(float (*tile)[kPitch]) const {
         if constexpr (kAlongK) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) tile[step + i][row_in_tile] = v[i];
+            for (int i = 0; i < 4; i++) tile[step + i][row] = v[i];
         } else {
-            float4* to = reinterpret_cast<float4*>(&tile[step][row_in_tile]);
-            to[0] = make_float4(v[0], v[1], v[2], v[3]);
-            to[1] = make_float4(v[4], v[5], v[6], v[7]);
+            *reinterpret_cast<float4*>(&tile[step][row]) = make_float4(v[0], v[1], v[2], v[3]);
         }
     }
 };
 
+// Eight wavefronts of 32 x 64, two on a SIMD: one's loads and stores stand beside the other's products.
 template <typename T, bool kAlongKA, bool kAlongKB, Epilogue kEpilogue>
-__global__ void __launch_bounds__(256) product_kernel(ProductParams p) {
+__global__ void __launch_bounds__(512) product_kernel(ProductParams p) {
     __shared__ __align__(16) float as[2][kStep][kPitch], bs[2][kStep][kPitch];
     int tm, tn, share;
     float* sums = work_of<8>(p, kTile * kTile, tm, tn, share);
@@ -79,70 +74,64 @@ __global__ void __launch_bounds__(256) product_kernel(ProductParams p) {
     // gated: rows 0..63 of B's tile are gate rows, 64..127 up rows
     const bool up = kGated && pb.row >= kTile / 2;
     auto load = [&](int64_t k) {
-        pa.load(a, p.a.stride, m0, p.M, k, k1, p.a_vectors);
-        if constexpr (kGated) pb.load(b + (up ? inter * p.b.stride : 0), p.b.stride, n0 - (up ? kTile / 2 : 0), inter, k, k1, p.b_vectors);
-        else pb.load(b, p.b.stride, n0, p.N, k, k1, p.b_vectors);
+        pa.load(a, p.a.stride, m0, p.M, k, k1);
+        if constexpr (kGated) pb.load(b + (up ? inter * p.b.stride : 0), p.b.stride, n0 - (up ? kTile / 2 : 0), inter, k, k1);
+        else pb.load(b, p.b.stride, n0, p.N, k, k1);
     };
-    auto store = [&](int at) {
-        pa.store(as[at], pa.row);
-        pb.store(bs[at], pb.row);
-    };
-    f32x16_t acc[2][2] = {};
+    const bool there = m0 + wm * 32 < p.M;   // of a few rows most of the products would be of none: 64 x 5632 x 1024, 33 -> 25 us
+    f32x16_t acc[2] = {};
     load(k0);
-    store(0);
+    pa.store(as[0]);
+    pb.store(bs[0]);
     __syncthreads();
     int at = 0;
     for (int64_t k = k0; k < k1; k += kStep) {
         const bool more = k + kStep < k1;
         if (more) load(k + kStep);
+        if (there)
 #pragma unroll
         for (int s = 0; s < kStep; s += 2) {
-            float av[2], bv[2];
+            const float av = as[at][s + half][wm * 32 + l];
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                av[i] = as[at][s + half][wm * 64 + i * 32 + l];
-                bv[i] = bs[at][s + half][kGated ? i * 64 + wn * 32 + l : wn * 64 + i * 32 + l];
-            }
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(av[i], bv[j], acc[i][j], 0, 0, 0);
+            for (int j = 0; j < 2; j++)
+                acc[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(av, bs[at][s + half][kGated ? j * 64 + wn * 32 + l : wn * 64 + j * 32 + l], acc[j], 0, 0, 0);
         }
-        if (more) store(at ^ 1);
+        if (more) {
+            pa.store(as[at ^ 1]);
+            pb.store(bs[at ^ 1]);
+        }
         __syncthreads();
         at ^= 1;
     }
     // element r of an accumulator: row 8 (r / 4) + 4 half + r % 4, column l
 #pragma unroll
-    for (int i = 0; i < 2; i++)
+    for (int r = 0; r < 16; r++) {
+        const int row = wm * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
+        const int64_t m = m0 + row;
+        if (sums) {
 #pragma unroll
-        for (int r = 0; r < 16; r++) {
-            const int row = wm * 64 + i * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
-            const int64_t m = m0 + row;
-            if (sums) {
-#pragma unroll
-                for (int j = 0; j < 2; j++) sums[row * kTile + (kGated ? j * 64 + wn * 32 : wn * 64 + j * 32) + l] = acc[i][j][r];
-                continue;
+            for (int j = 0; j < 2; j++) sums[row * kTile + (kGated ? j * 64 + wn * 32 : wn * 64 + j * 32) + l] = acc[j][r];
+            continue;
+        }
+        if (m >= p.M) continue;
+        if constexpr (kGated) {
+            const int64_t n = n0 + wn * 32 + l;
+            if (n >= inter) continue;
+            const float g = acc[0][r], u = acc[1][r];
+            ((T*)p.out)[m * inter + n] = Elem<T>::from_float(gate_product(g, u));
+            if (p.both) {
+                T* to = (T*)p.both + m * p.N + n;
+                to[0] = Elem<T>::from_float(g);
+                to[inter] = Elem<T>::from_float(u);
             }
-            if (m >= p.M) continue;
-            if constexpr (kGated) {
-                const int64_t n = n0 + wn * 32 + l;
-                if (n >= inter) continue;
-                const float g = acc[i][0][r], u = acc[i][1][r];
-                ((T*)p.out)[m * inter + n] = Elem<T>::from_float(gate_product(g, u));
-                if (p.both) {
-                    T* to = (T*)p.both + m * p.N + n;
-                    to[0] = Elem<T>::from_float(g);
-                    to[inter] = Elem<T>::from_float(u);
-                }
-            } else {
+        } else {
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const int64_t n = n0 + wn * 64 + j * 32 + l;
-                    if (n < p.N) ((T*)p.out)[m * p.N + n] = Elem<T>::from_float(acc[i][j][r]);
-                }
+            for (int j = 0; j < 2; j++) {
+                const int64_t n = n0 + wn * 64 + j * 32 + l;
+                if (n < p.N) ((T*)p.out)[m * p.N + n] = Elem<T>::from_float(acc[j][r]);
             }
         }
+    }
 }
 
 // Sums of the shares of a tile, in their order, and what the product's own epilogue does.  A workgroup has some rows of a tile, a thread four
@@ -244,7 +233,7 @@ bool fits_tiles(const ProductParams& p, bool along_a, bool along_b, bool gated) 
 }
 
 // Where the tiles of float32 products leave compute units idle, the steps are shared out over as many workgroups as come to one each, none with
-// fewer than 256.
+// fewer than 128.
 TilePlan plan_float(int64_t M, int64_t N, int64_t K, int cus) {
     TilePlan r;
     r.tile_m = r.tile_n = kTile;
@@ -252,7 +241,7 @@ TilePlan plan_float(int64_t M, int64_t N, int64_t K, int cus) {
     r.tiles_m = (int)((M + kTile - 1) / kTile);
     r.tiles_n = (int)((N + kTile - 1) / kTile);
     const int64_t tiles = (int64_t)r.tiles_m * r.tiles_n;
-    const int64_t shares = std::max<int64_t>(1, std::min<int64_t>(cus / tiles, K / 256));
+    const int64_t shares = std::max<int64_t>(1, std::min<int64_t>(cus / tiles, K / 128));
     r.k_share = ((K + shares - 1) / shares + kStep - 1) / kStep * kStep;
     r.shares = (int)((K + r.k_share - 1) / r.k_share);
     r.whole_tiles = r.shares > 1 ? 0 : (int)std::min<int64_t>(tiles, 0x7fffffff);
@@ -283,10 +272,7 @@ int run_product(ProductParams& p, const DeviceInfo& di, void* workspace, int64_t
         if constexpr (sizeof(T) == 2)
             if (int rc = run_tiles<T>(p, plan, kAlongKA, kEpilogue, stream)) return rc;
     } else {
-        auto vectors = [](const Operand& o) { return reinterpret_cast<uintptr_t>(o.p) % 16 == 0 && o.stride % (16 / (int64_t)sizeof(T)) == 0; };
-        p.a_vectors = vectors(p.a);
-        p.b_vectors = vectors(p.b);
-        hipLaunchKernelGGL((product_kernel<T, kAlongKA, kAlongKB, kEpilogue>), dim3((unsigned)plan.blocks()), dim3(256), 0, stream, p);
+        hipLaunchKernelGGL((product_kernel<T, kAlongKA, kAlongKB, kEpilogue>), dim3((unsigned)plan.blocks()), dim3(512), 0, stream, p);
         CKV_HIP_TRY(hipGetLastError());
     }
     if (plan.shares > 1) {

@@ -22,7 +22,6 @@ struct ProductParams {
     int tiles_m, tiles_n;
     int whole_tiles;    // tiles before the first that is shared out
     int shares;
-    bool a_vectors, b_vectors;   // float32 products: operands of whole, aligned pieces of 16 bytes
 };
 
 enum Epilogue { kStore, kGate };
