@@ -4,15 +4,16 @@
 //   top-k keeps the first k, top-p what has less than p of their mass before it, min-p what has w_i >= min_p; the first one stays.
 //   The token is the first whose running kept mass exceeds u times all of it.
 //
-// Every one of these sets is a beginning of the order, so nothing needs sorting but the elements around three borders: rows are laid into
-// bins of x, 1/64 wide up to 32 (below that a weight is 2^-45 of the first one's: nothing), each with its count and mass; running sums say in
-// which bins the borders lie, and the elements of those bins alone are collected and sorted.  Where they are too many to be (ties), the row is
-// read again a byte of the order at a time.
+// Every one of these sets is a beginning of the order, so nothing needs sorting but the elements around four borders: rows are laid into
+// bins of x, ln 2 / 64 wide up to 32 (a weight of 2^-46: what lies further is nothing), running sums say in which bins the borders lie, and
+// the elements of those bins alone are collected and sorted.  Where they are too many to be (ties), the row is read again a byte of the order
+// at a time.
 //
-// Masses are whole numbers, of 2^-44: sums are exact, whatever the order of the atomics that add them up, and a row means the same
-// however many workgroups share it.  x is worked out in double (a logit of float32 less another has more digits than that, and a
-// running sum over 10^5 tokens has as many borders that u may fall next to); of the exponential, 2^(-n/64) is a table in double and
-// the rest, below 0.0055, a float32 polynomial: 2^-31 relative.
+// A weight is 2^(-n / 64), its bin's, times 1 + q, which is no more than 0.0055 from one: a bin adds up q in whole numbers of 2^-31 and counts,
+// both in one 64-bit atomic, so that sums are exact whatever the order of the atomics.  Masses of bins, or of beginnings of one, are rounded to
+// whole numbers of 2^-44: running sums over bins and over elements agree to the last digit (in double, an empty bin between two threads' sums
+// had a mass of 10^-16).  x is worked out in double (a logit of float32 less another has more digits than that, and a running sum over 10^5
+// tokens has as many borders that u may fall next to); q is a float32 polynomial: 2^-31 relative to the weight.
 //
 // A row is one workgroup's where there are rows enough to fill the chip, one launch with everything in LDS; fewer rows are shared out in
 // slices over three launches (maximum; bins, and the last workgroup of a row to arrive finds the borders; elements, and the last one draws).
@@ -23,27 +24,31 @@
 namespace ckv {
 namespace {
 
-constexpr int kBins = 2048;
-constexpr double kBinsPerUnit = 64.0, kFar = 32.0;   // kBins / kBinsPerUnit
+constexpr double kFar = 32.0;
+constexpr float kBinsPerUnit = 92.332482618935f;     // 64 / ln 2
+constexpr double kBinWidth = 0.010830424696249145;
+constexpr int kBins = 2956;                          // kFar of them, the last rounded up
 constexpr int kListMax = 2048;                       // a power of two: the list is sorted in place
 constexpr int kMaxSlices = 64;
-constexpr int kMaxVocab = (1 << 20) - 1;             // of masses up to 2^44 each in 64 bits
-constexpr uint64_t kOne = 1ull << 44;
+constexpr int kThreads = 1024;
+constexpr int kMaxVocab = (1 << 19) - 1;             // of numbers below 2^25 in the lower 44 bits of a bin, and their count in the upper 20
+constexpr int kCountShift = 44;
+constexpr uint64_t kOne = 1ull << 44;                // the mass of the first token
+constexpr uint32_t kBias = 1u << 24;                 // makes q's whole number positive
 
 // Which bins have to be looked at element by element, and what is known of the borders without that.
 struct Borders {
-    int from[3], to[3];   // top-k, top-p, the token; from > to: none
+    int from[4], to[4];   // top-k, top-p, min-p, the token; from > to: none
     int partial_k;        // the k-th element lies inside its bin
     int many;             // more elements in those bins than the list holds
     uint64_t mass_k;      // of the first k, unless partial
-    uint64_t mass_min;    // of what min-p keeps
 };
 
 struct RowSpace {   // of a row that several workgroups share
-    uint64_t mass[kBins + 1];
+    unsigned long long bins[kBins];
+    unsigned long long mass[kBins + 1];
     uint32_t count[kBins + 1];
-    uint32_t maxima[kMaxSlices];
-    uint64_t mass_min;
+    float maxima[kMaxSlices];
     uint32_t arrived[2], listed;
     Borders borders;
     uint64_t list[kListMax];
@@ -66,7 +71,7 @@ struct SampleParams {
 };
 
 struct Settings {
-    double inv_t, far_min, p, u;   // far_min: the largest x that min-p keeps
+    double inv_t, far_min, p, u;   // far_min: the largest x that min-p keeps, above kFar: no limit
     int k;
 };
 
@@ -84,33 +89,35 @@ __device__ inline Settings settings_of(const SampleParams& s, int64_t row) {
     return r;
 }
 
-// Rising with the value, zeros of either sign alike; NaN below everything.
+// Rising with the value, zeros of either sign alike.
 __device__ inline uint32_t key_of(float l) {
-    if (l != l) return 0;
     const uint32_t u = __float_as_uint(l + 0.f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ inline float value_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
-constexpr uint32_t kMinusInfinity = 0x007fffffu;
 
 // x of a logit, or false: nothing of it counts
 __device__ inline bool distance(float l, float m, double inv_t, double& x) {
     x = l == m ? 0.0 : ((double)m - (double)l) * inv_t;
     return x < kFar;
 }
-__device__ inline int bin_of(double x) { return (int)(x * kBinsPerUnit); }
+__device__ inline float bin_of(double x) { return rintf((float)x * kBinsPerUnit); }   // a whole number; rises with x
 
 __device__ inline void fill_table(double* table) {
     if (threadIdx.x < 64) table[threadIdx.x] = exp2(-(double)threadIdx.x / 64.0);
 }
+__device__ inline double bin_weight(int n, const double* table) { return __longlong_as_double(__double_as_longlong(table[n & 63]) - (int64_t)(n >> 6) * (1ll << 52)); }
 
-__device__ inline uint64_t mass_of(double x, const double* table) {
-    const float n = rintf((float)x * 92.332482618935f);                     // 64 / ln 2
-    const float r = (float)__builtin_fma(-(double)n, 0.010830424696249145, x);
+// q of a weight in its bin, in whole numbers of 2^-31 and biased
+__device__ inline uint32_t rest_of(double x, float n) {
+    const float r = (float)__builtin_fma(-(double)n, kBinWidth, x);
     const float q = r * (-1.f + r * (0.5f + r * (-0.16666667f + r * 0.041666668f)));   // exp(-r) - 1
-    const int i = (int)n;
-    const double t = __longlong_as_double(__double_as_longlong(table[i & 63]) + (44 - (i >> 6)) * (1ll << 52));
-    return (uint64_t)__double_as_longlong(__builtin_fma(t, (double)q, t) + 4503599627370496.0) & 0xfffffffffffffull;   // + 2^52: rounded to a whole number
+    return (uint32_t)((int)rintf(q * 2147483648.f) + (int)kBias);
+}
+// The mass of some weights of bin n: their count in the upper bits, the sum of their rests in the lower ones.
+__device__ inline uint64_t mass_of(int n, uint64_t some, const double* table) {
+    const int64_t count = (int64_t)(some >> kCountShift), rests = (int64_t)(some & ((1ull << kCountShift) - 1));
+    return (uint64_t)rint(bin_weight(n, table) * (double)((count << 31) + rests - count * (int64_t)kBias) * 8192.0);   // 2^44 / 2^31
 }
 
 // fn(index, value) for a slice of a row: vectors of 16 bytes between what lies in front of the first aligned one and behind the last.
@@ -165,58 +172,65 @@ __device__ inline V before_me(V v, V* waves, V* all) {
     return front + s - v;
 }
 
-__device__ inline uint32_t block_max(uint32_t v, uint32_t* waves) {
+// The largest of all in front of this thread; 0 if there is none.
+__device__ inline uint32_t latest_before_me(uint32_t v, uint32_t* waves) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t s = v;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
+    for (int o = 1; o < CKV_WAVE; o <<= 1) {
+        const uint32_t other = __shfl_up(s, o);
+        if (lane >= o) s = max(s, other);
+    }
+    __syncthreads();
+    if (lane == 63) waves[wave] = s;
+    const uint32_t before = __shfl_up(s, 1);
+    __syncthreads();
+    uint32_t front = lane ? before : 0;
+    for (int w = 0; w < wave; w++) front = max(front, waves[w]);
+    return front;
+}
+
+__device__ inline float block_max(float v, float* waves) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
     __syncthreads();
     if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
     __syncthreads();
     v = waves[0];
-    for (int w = 1; w < (int)(blockDim.x >> 6); w++) v = max(v, waves[w]);
+    for (int w = 1; w < (int)(blockDim.x >> 6); w++) v = fmaxf(v, waves[w]);
     return v;
 }
 
 struct Shared {
-    uint64_t mass[kBins + 1];    // of a bin, then of all bins in front of it
+    unsigned long long mass[kBins + 1];   // of all bins in front of one; first the bins themselves
     uint32_t count[kBins + 1];
     double table[64];
     uint64_t wide[16];
     uint32_t narrow[16];
-    uint64_t mass_min;
+    float tops[16];
     uint32_t listed, last;
     Borders borders;
-    uint64_t answer[3];
+    unsigned long long answer[3];
 };
 
 struct Lists {
     uint64_t list[kListMax];     // order: (falling value, rising index)
-    uint64_t running[kListMax];
+    uint64_t before[kListMax];   // counts and rests of all in front
 };
 
 // ---- the bins --------------------------------------------------------------------------------------------------------------------------
 
 template <typename T>
 __device__ inline void fill_bins(Shared& sh, const T* row, const SampleParams& s, const Settings& set, float m, int slice) {
-    for (int i = threadIdx.x; i <= kBins; i += blockDim.x) {
-        sh.mass[i] = 0;
-        sh.count[i] = 0;
-    }
-    if (threadIdx.x == 0) sh.mass_min = 0;
+    for (int i = threadIdx.x; i < kBins; i += blockDim.x) sh.mass[i] = 0;
     fill_table(sh.table);
     __syncthreads();
-    uint64_t kept = 0;
     for_each(row, s.vocab, slice, s.slices, [&](int, float l) {
         double x;
         if (!distance(l, m, set.inv_t, x)) return;
-        const uint64_t q = mass_of(x, sh.table);
-        const int b = bin_of(x);
-        atomicAdd((unsigned long long*)&sh.mass[b], (unsigned long long)q);
-        atomicAdd(&sh.count[b], 1u);
-        if (x <= set.far_min) kept += q;
+        const float n = bin_of(x);
+        atomicAdd(&sh.mass[(int)n], (1ull << kCountShift) | rest_of(x, n));
     });
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) kept += __shfl_xor(kept, o);
-    if ((threadIdx.x & 63) == 0) atomicAdd((unsigned long long*)&sh.mass_min, (unsigned long long)kept);
     __syncthreads();
 }
 
@@ -241,23 +255,26 @@ __device__ inline uint64_t draw_below(double u, uint64_t mass) {
 
 // Bins become running sums, and the borders are looked up in them.
 __device__ inline void find_borders(Shared& sh, const Settings& set) {
-    constexpr int kMost = 8;
-    const int each = kBins / blockDim.x;   // 2 or 8
-    uint64_t m[kMost], all_m;
-    uint32_t c[kMost], all_c;
-    uint64_t sm = 0;
-    uint32_t sc = 0;
-    for (int i = 0; i < each; i++) {
-        m[i] = sh.mass[threadIdx.x * each + i];
-        c[i] = sh.count[threadIdx.x * each + i];
+    constexpr int kEach = (kBins + kThreads - 1) / kThreads;
+    uint64_t m[kEach], sm = 0, all_m;
+    uint32_t c[kEach], sc = 0, all_c;
+    const int first = threadIdx.x * kEach;
+#pragma unroll
+    for (int i = 0; i < kEach; i++) {
+        const uint64_t b = first + i < kBins ? sh.mass[first + i] : 0;
+        m[i] = first + i < kBins ? mass_of(first + i, b, sh.table) : 0;
+        c[i] = (uint32_t)(b >> kCountShift);
         sm += m[i];
         sc += c[i];
     }
-    uint64_t fm = before_me(sm, sh.wide, &all_m);
+    uint64_t fm = before_me(sm, sh.wide, &all_m);   // its barriers let everybody read the bins first
     uint32_t fc = before_me(sc, sh.narrow, &all_c);
-    for (int i = 0; i < each; i++) {
-        sh.mass[threadIdx.x * each + i] = fm;
-        sh.count[threadIdx.x * each + i] = fc;
+#pragma unroll
+    for (int i = 0; i < kEach; i++) {
+        if (first + i < kBins) {
+            sh.mass[first + i] = fm;
+            sh.count[first + i] = fc;
+        }
         fm += m[i];
         fc += c[i];
     }
@@ -268,15 +285,17 @@ __device__ inline void find_borders(Shared& sh, const Settings& set) {
     __syncthreads();
     Borders r;
     r.partial_k = 0;
-    r.mass_min = sh.mass_min;
-    r.from[0] = r.from[1] = 1;
-    r.to[0] = r.to[1] = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        r.from[i] = 1;
+        r.to[i] = 0;
+    }
     uint64_t low = all_m, high = all_m;   // of what is kept
     if (set.k < (int)all_c) {
         const int b = first_bin(sh, [&](int e) { return sh.count[e] >= (uint32_t)set.k; });
         low = high = sh.mass[b + 1];
         if (sh.count[b + 1] != (uint32_t)set.k) {
-            low = max(sh.mass[b], kOne);
+            low = max((uint64_t)sh.mass[b], kOne);
             r.partial_k = 1;
             r.from[0] = r.to[0] = b;
         }
@@ -286,16 +305,21 @@ __device__ inline void find_borders(Shared& sh, const Settings& set) {
         const double t0 = set.p * (double)low, t1 = set.p * (double)high;
         r.from[1] = first_bin(sh, [&](int e) { return (double)sh.mass[e] >= t0; });
         r.to[1] = first_bin(sh, [&](int e) { return (double)sh.mass[e] >= t1; });
-        low = min(low, max(sh.mass[r.from[1]], kOne));
-        high = min(high, sh.mass[r.to[1] + 1]);
+        low = min(low, max((uint64_t)sh.mass[r.from[1]], kOne));
+        high = min(high, (uint64_t)sh.mass[r.to[1] + 1]);
     }
-    low = min(low, r.mass_min);
-    high = min(high, r.mass_min);
+    if (set.far_min < kFar) {
+        const int b = (int)bin_of(set.far_min);
+        r.from[2] = r.to[2] = b;
+        low = min(low, max((uint64_t)sh.mass[b], kOne));
+        high = min(high, (uint64_t)sh.mass[b + 1]);
+    }
     const uint64_t d0 = draw_below(set.u, low), d1 = draw_below(set.u, high);
-    r.from[2] = first_bin(sh, [&](int e) { return sh.mass[e] > d0; });
-    r.to[2] = first_bin(sh, [&](int e) { return sh.mass[e] > d1; });
+    r.from[3] = first_bin(sh, [&](int e) { return sh.mass[e] > d0; });
+    r.to[3] = first_bin(sh, [&](int e) { return sh.mass[e] > d1; });
     uint32_t many = 0;
-    for (int i = 0; i < 3; i++)
+#pragma unroll
+    for (int i = 0; i < 4; i++)
         if (r.from[i] <= r.to[i]) many += sh.count[r.to[i] + 1] - sh.count[r.from[i]];
     r.many = many > (uint32_t)kListMax;
     __syncthreads();
@@ -304,11 +328,28 @@ __device__ inline void find_borders(Shared& sh, const Settings& set) {
 }
 
 __device__ inline bool wanted(const Borders& r, int b) {
-    return (b >= r.from[0] && b <= r.to[0]) || (b >= r.from[1] && b <= r.to[1]) || (b >= r.from[2] && b <= r.to[2]);
+    return (b >= r.from[0] && b <= r.to[0]) || (b >= r.from[1] && b <= r.to[1]) || (b >= r.from[2] && b <= r.to[2]) || (b >= r.from[3] && b <= r.to[3]);
 }
 
 __device__ inline uint64_t order_of(float l, int i) { return ((uint64_t)~key_of(l) << 32) | (uint32_t)i; }
 __device__ inline float logit_of(uint64_t order) { return value_of(~(uint32_t)(order >> 32)); }
+
+// The elements of the borders' bins.  The bins of a border are a stretch of values: one comparison passes most of a row over.
+template <typename T, typename Fn>
+__device__ inline void for_wanted(const T* row, const SampleParams& s, const Settings& set, float m, const Borders& r, int slice, int slices, Fn fn) {
+    int last = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (r.from[i] <= r.to[i]) last = max(last, r.to[i]);
+    // a bin further than the last one, and rounded down twice: below it nothing is wanted
+    const double lowest = (double)m - (last + 1.5) * kBinWidth / set.inv_t;
+    const float floor = lowest > -3.4e38 ? (float)lowest - fabsf((float)lowest) * 2.4e-7f : -__builtin_huge_valf();
+    for_each(row, s.vocab, slice, slices, [&](int i, float l) {
+        if (l < floor) return;
+        double x;
+        if (distance(l, m, set.inv_t, x) && wanted(r, (int)bin_of(x))) fn(order_of(l, i));
+    });
+}
 
 // ---- the token -------------------------------------------------------------------------------------------------------------------------
 
@@ -338,125 +379,108 @@ __device__ inline void draw_from_list(Shared& sh, Lists& li, const SampleParams&
             }
             __syncthreads();
         }
-    // Running mass up to and with each element; the bins between are added where the next one starts.
-    const int each = (n + blockDim.x - 1) / blockDim.x, first = min(n, (int)threadIdx.x * each), end = min(n, first + each);
-    auto bin_at = [&](int i) {
-        double x;
-        distance(logit_of(li.list[i]), m, set.inv_t, x);
-        return bin_of(x);
-    };
-    uint64_t sum = 0, all;
-    uint32_t rank = 0, all_rank;
-    int prev = first > 0 && first < n ? bin_at(first - 1) : -1;
-    const int prev0 = prev;
-    auto step = [&](int i, uint64_t& mass, uint32_t& place) {
-        double x;
-        distance(logit_of(li.list[i]), m, set.inv_t, x);
-        const int b = bin_of(x);
-        if (b != prev) {
-            mass += sh.mass[b] - sh.mass[prev + 1];
-            place += sh.count[b] - sh.count[prev + 1];
-            prev = b;
+    // A thread has two neighbours at most.  The running mass up to an element is that of the bins in front of its own and of the beginning of its
+    // bin up to it: the weights between, counts and rests, are added up over the list, and the element where the bin begins is looked up.
+    static_assert(kListMax <= 2 * kThreads, "two a thread");
+    const int each = n > (int)blockDim.x ? 2 : 1, first = threadIdx.x * each;
+    double x[2] = {};
+    uint64_t some[2] = {}, run[2] = {};
+    int bin[2] = {-1, -1};
+    uint32_t begin[2] = {};   // of its bin, 1-based, in this thread
+    int before = -1;
+    if (first > 0 && first < n) {
+        double xb;
+        distance(logit_of(li.list[first - 1]), m, set.inv_t, xb);
+        before = (int)bin_of(xb);
+    }
+    uint32_t latest = 0;
+    for (int e = 0; e < each; e++)
+        if (first + e < n) {
+            distance(logit_of(li.list[first + e]), m, set.inv_t, x[e]);
+            const float b = bin_of(x[e]);
+            bin[e] = (int)b;
+            some[e] = (1ull << kCountShift) | rest_of(x[e], b);
+            if (bin[e] != before) latest = first + e + 1;
+            before = bin[e];
+            begin[e] = latest;
         }
-        const uint64_t q = mass_of(x, sh.table);
-        mass += q;
-        place += 1;
-        return q;
-    };
-    for (int i = first; i < end; i++) step(i, sum, rank);
-    const uint64_t front = before_me(sum, sh.wide, &all);
-    const uint32_t front_rank = before_me(rank, sh.narrow, &all_rank);
+    uint64_t all;
+    uint64_t front = before_me(some[0] + some[1], sh.wide, &all);
+    const uint32_t begun = latest_before_me(latest, sh.narrow);
+    for (int e = 0; e < each; e++)
+        if (first + e < n) {
+            li.before[first + e] = front;
+            front += some[e];
+        }
     if (threadIdx.x == 0) {
         sh.answer[0] = r.mass_k;
-        sh.answer[1] = kOne;
-        sh.answer[2] = (uint64_t)(n - 1);
+        sh.answer[1] = sh.answer[2] = kOne;
+        sh.listed = 0;
     }
     __syncthreads();
-    // top-k
-    prev = prev0;
-    uint64_t at = front;
-    uint32_t place = front_rank;
-    for (int i = first; i < end; i++) {
-        step(i, at, place);
-        li.running[i] = at;
-        if (r.partial_k && place == (uint32_t)set.k) sh.answer[0] = at;
-    }
+    for (int e = 0; e < each; e++)
+        if (first + e < n) {
+            const uint32_t from = (begin[e] ? begin[e] : begun) - 1;
+            const uint64_t in_front = li.before[first + e] - li.before[from];
+            run[e] = sh.mass[bin[e]] + mass_of(bin[e], in_front + some[e], sh.table);
+            some[e] = sh.mass[bin[e]] + mass_of(bin[e], in_front, sh.table);   // and before it
+            if (r.partial_k && sh.count[bin[e]] + (first + e - from) + 1 == (uint32_t)set.k) sh.answer[0] = run[e];
+            if (x[e] <= set.far_min) atomicMax(&sh.answer[2], (unsigned long long)run[e]);
+        }
     __syncthreads();
     uint64_t kept = sh.answer[0];
     if (set.p < 1.0) {   // the last one that has less than p of that before it
         const double t = set.p * (double)kept;
-        prev = prev0;
-        at = front;
-        place = 0;
-        for (int i = first; i < end; i++) {
-            const uint64_t q = step(i, at, place);
-            if ((double)(at - q) < t) atomicMax((unsigned long long*)&sh.answer[1], (unsigned long long)at);
-        }
+        for (int e = 0; e < each; e++)
+            if (first + e < n && (double)some[e] < t) atomicMax(&sh.answer[1], (unsigned long long)run[e]);
         __syncthreads();
-        kept = min(kept, sh.answer[1]);
+        kept = min(kept, (uint64_t)sh.answer[1]);
     }
-    kept = min(kept, r.mass_min);
+    if (set.far_min < kFar) kept = min(kept, max((uint64_t)sh.answer[2], (uint64_t)sh.mass[r.from[2]]));
     const uint64_t d = draw_below(set.u, kept);
-    for (int i = first; i < end; i++)
-        if (li.running[i] > d && (i == 0 || li.running[i - 1] <= d)) sh.answer[2] = (uint64_t)i;
+    for (int e = 0; e < each; e++)
+        if (first + e < n && run[e] > d && some[e] <= d) sh.listed = first + e;
     __syncthreads();
-    if (threadIdx.x == 0) answer(s, row, set, m, li.list[sh.answer[2]], kept);
+    if (threadIdx.x == 0) answer(s, row, set, m, li.list[sh.listed], kept);
 }
 
 // Without a list: the row is read once for every byte of the order.  In one bin, the first element at which `reached(count, mass)`, of all
 // up to and with it, holds; returns the running mass there and the element.
 template <typename T, typename Fn>
 __device__ inline uint64_t search_row(Shared& sh, Lists& li, const T* row, const SampleParams& s, const Settings& set, float m, int bin, Fn reached,
-                                      uint64_t& element) {
-    uint64_t* masses = li.list;                                    // 256
-    uint32_t* counts = reinterpret_cast<uint32_t*>(li.running);   // 256
-    uint64_t prefix = 0, mass = sh.mass[bin];
-    uint32_t count = sh.count[bin];
+                                    uint64_t& element) {
+    unsigned long long* digits = reinterpret_cast<unsigned long long*>(li.list);   // 256
+    uint64_t prefix = 0, front = 0;
     for (int shift = 56; shift >= 0; shift -= 8) {
         __syncthreads();
-        for (int i = threadIdx.x; i < 256; i += blockDim.x) {
-            masses[i] = 0;
-            counts[i] = 0;
-        }
+        for (int i = threadIdx.x; i < 256; i += blockDim.x) digits[i] = 0;
         __syncthreads();
         for_each(row, s.vocab, 0, 1, [&](int i, float l) {
             double x;
-            if (!distance(l, m, set.inv_t, x) || bin_of(x) != bin) return;
+            if (!distance(l, m, set.inv_t, x)) return;
+            const float n = bin_of(x);
+            if ((int)n != bin) return;
             const uint64_t o = order_of(l, i);
             if (shift < 56 && (o >> (shift + 8)) != (prefix >> (shift + 8))) return;
-            const int digit = (int)(o >> shift) & 255;
-            atomicAdd((unsigned long long*)&masses[digit], (unsigned long long)mass_of(x, sh.table));
-            atomicAdd(&counts[digit], 1u);
+            atomicAdd(&digits[(int)(o >> shift) & 255], (1ull << kCountShift) | rest_of(x, n));
         });
         __syncthreads();
-        // every thread walks over the 256 sums alike
-        int digit = 0, last = 0;
-        uint64_t last_mass = mass;
-        uint32_t last_count = count;
-        bool found = false;
-        for (; digit < 256; digit++) {
-            if (!counts[digit]) continue;
-            last = digit;
-            last_mass = mass;
-            last_count = count;
-            if (reached(count + counts[digit], mass + masses[digit])) {
-                found = true;
-                break;
-            }
-            mass += masses[digit];
-            count += counts[digit];
-        }
-        if (!found) {   // rounding of a border at the bin's end: the last one
-            digit = last;
-            mass = last_mass;
-            count = last_count;
+        // every thread walks over the 256 sums alike; if none reaches (rounding, at the bin's end), the last one that is there does
+        int digit = 0;
+        uint64_t some = front;
+        for (int i = 0; i < 256; i++) {
+            if (!digits[i]) continue;
+            digit = i;
+            front = some;
+            some += digits[i];
+            if (reached(sh.count[bin] + (uint32_t)(some >> kCountShift), sh.mass[bin] + mass_of(bin, some, sh.table))) break;
         }
         prefix |= (uint64_t)digit << shift;
-        if (shift == 0) mass += masses[digit];
+        if (shift == 0) front = some;
     }
     element = prefix;
     __syncthreads();
-    return mass;
+    return sh.mass[bin] + mass_of(bin, front, sh.table);
 }
 
 template <typename T>
@@ -470,7 +494,20 @@ __device__ inline void draw_from_row(Shared& sh, Lists& li, const T* row_logits,
         const int b = first_bin(sh, [&](int e) { return (double)sh.mass[e] >= t; });
         kept = min(kept, max(kOne, search_row(sh, li, row_logits, s, set, m, b, [&](uint32_t, uint64_t q) { return (double)q >= t; }, element)));
     }
-    kept = min(kept, r.mass_min);
+    if (set.far_min < kFar) {   // what of its bin min-p keeps
+        unsigned long long* sum = reinterpret_cast<unsigned long long*>(li.list);
+        __syncthreads();
+        if (threadIdx.x == 0) *sum = 0;
+        __syncthreads();
+        for_each(row_logits, s.vocab, 0, 1, [&](int, float l) {
+            double x;
+            if (!distance(l, m, set.inv_t, x) || x > set.far_min) return;
+            const float n = bin_of(x);
+            if ((int)n == r.from[2]) atomicAdd(sum, (1ull << kCountShift) | rest_of(x, n));
+        });
+        __syncthreads();
+        kept = min(kept, max(kOne, sh.mass[r.from[2]] + mass_of(r.from[2], *sum, sh.table)));
+    }
     const uint64_t d = draw_below(set.u, kept);
     const int b = first_bin(sh, [&](int e) { return sh.mass[e] > d; });
     search_row(sh, li, row_logits, s, set, m, b, [&](uint32_t, uint64_t q) { return q > d; }, element);
@@ -485,20 +522,19 @@ __device__ inline void no_answer(const SampleParams& s, int64_t row) {   // no l
 // ---- a workgroup a row -----------------------------------------------------------------------------------------------------------------
 
 template <typename T>
-__global__ void __launch_bounds__(1024) sample_row_kernel(SampleParams s) {
+__global__ void __launch_bounds__(kThreads) sample_row_kernel(SampleParams s) {
     __shared__ Shared sh;
     __shared__ Lists li;
     const int64_t row = blockIdx.x;
     const T* logits = (const T*)s.logits + row * s.stride;
     const Settings set = settings_of(s, row);
-    uint32_t top = 0;
-    for_each(logits, s.vocab, 0, 1, [&](int, float l) { top = max(top, key_of(l)); });
-    top = block_max(top, sh.narrow);
-    if (top <= kMinusInfinity) {
+    float m = -__builtin_huge_valf();
+    for_each(logits, s.vocab, 0, 1, [&](int, float l) { m = fmaxf(m, l); });   // NaN is passed over
+    m = block_max(m, sh.tops);
+    if (!(m > -__builtin_huge_valf())) {
         if (threadIdx.x == 0) no_answer(s, row);
         return;
     }
-    const float m = value_of(top);
     fill_bins(sh, logits, s, set, m, 0);
     find_borders(sh, set);
     const Borders r = sh.borders;
@@ -508,51 +544,44 @@ __global__ void __launch_bounds__(1024) sample_row_kernel(SampleParams s) {
     }
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
-    for_each(logits, s.vocab, 0, 1, [&](int i, float l) {
-        double x;
-        if (distance(l, m, set.inv_t, x) && wanted(r, bin_of(x))) li.list[atomicAdd(&sh.listed, 1u)] = order_of(l, i);
-    });
+    for_wanted(logits, s, set, m, r, 0, 1, [&](uint64_t o) { li.list[atomicAdd(&sh.listed, 1u)] = o; });
     __syncthreads();
-    draw_from_list(sh, li, s, row, set, m, (int)sh.listed);
+    const int n = (int)sh.listed;
+    __syncthreads();
+    draw_from_list(sh, li, s, row, set, m, n);
 }
 
 // ---- several workgroups a row ----------------------------------------------------------------------------------------------------------
 
 template <typename T>
-__global__ void __launch_bounds__(256) sample_max_kernel(SampleParams s) {
-    __shared__ uint32_t waves[4];
+__global__ void __launch_bounds__(kThreads) sample_max_kernel(SampleParams s) {
+    __shared__ float waves[kThreads / 64];
     const int64_t row = blockIdx.y;
     RowSpace& space = s.space[row];
-    for (int i = blockIdx.x * 256 + threadIdx.x; i <= kBins; i += gridDim.x * 256) {
-        space.mass[i] = 0;
-        space.count[i] = 0;
-    }
-    if (blockIdx.x == 0 && threadIdx.x == 0) {
-        space.mass_min = 0;
-        space.arrived[0] = space.arrived[1] = space.listed = 0;
-    }
-    uint32_t top = 0;
-    for_each((const T*)s.logits + row * s.stride, s.vocab, blockIdx.x, s.slices, [&](int, float l) { top = max(top, key_of(l)); });
-    top = block_max(top, waves);
-    if (threadIdx.x == 0) space.maxima[blockIdx.x] = top;
+    for (int i = blockIdx.x * kThreads + threadIdx.x; i < kBins; i += gridDim.x * kThreads) space.bins[i] = 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) space.arrived[0] = space.arrived[1] = space.listed = 0;
+    float m = -__builtin_huge_valf();
+    for_each((const T*)s.logits + row * s.stride, s.vocab, blockIdx.x, s.slices, [&](int, float l) { m = fmaxf(m, l); });
+    m = block_max(m, waves);
+    if (threadIdx.x == 0) space.maxima[blockIdx.x] = m;
 }
 
-__device__ inline uint32_t top_of(const RowSpace& space, int slices) {
-    uint32_t top = (int)(threadIdx.x & 63) < slices ? space.maxima[threadIdx.x & 63] : 0;
+__device__ inline float top_of(const RowSpace& space, int slices) {
+    float m = (int)(threadIdx.x & 63) < slices ? space.maxima[threadIdx.x & 63] : -__builtin_huge_valf();
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
-    return top;
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    return m;
 }
 
-// Is this the last of the row's workgroups to arrive?  Then what the others wrote before is there to be read.
+// Is this the last of the row's workgroups to arrive?  Then what the others wrote before is there to be read.  Everything that goes from one to
+// another is written by atomics of the device's scope and read by such loads, past the caches of an XCD, so their end is all there is to wait
+// for: a fence would have every wavefront write back and invalidate the L2.
 __device__ inline bool last_to_arrive(uint32_t* arrived, int slices, uint32_t* shared) {
-    __threadfence();
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (threadIdx.x == 0) *shared = atomicAdd(arrived, 1u) == (uint32_t)slices - 1;
+    if (threadIdx.x == 0) *shared = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)slices - 1;
     __syncthreads();
-    if (!*shared) return false;
-    __threadfence();
-    return true;
+    return *shared;
 }
 
 template <typename V>
@@ -561,29 +590,21 @@ __device__ inline V read_through(const V* p) {   // past what this compute unit 
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) sample_bins_kernel(SampleParams s) {
+__global__ void __launch_bounds__(kThreads) sample_bins_kernel(SampleParams s) {
     __shared__ Shared sh;
     const int64_t row = blockIdx.y;
     RowSpace& space = s.space[row];
-    const uint32_t top = top_of(space, s.slices);
-    if (top <= kMinusInfinity) return;   // all of the row's workgroups
+    const float m = top_of(space, s.slices);
+    if (!(m > -__builtin_huge_valf())) return;   // all of the row's workgroups
     const Settings set = settings_of(s, row);
-    fill_bins(sh, (const T*)s.logits + row * s.stride, s, set, value_of(top), blockIdx.x);
-    for (int b = threadIdx.x; b < kBins; b += 256)
-        if (sh.count[b]) {
-            atomicAdd((unsigned long long*)&space.mass[b], (unsigned long long)sh.mass[b]);
-            atomicAdd(&space.count[b], sh.count[b]);
-        }
-    if (threadIdx.x == 0) atomicAdd((unsigned long long*)&space.mass_min, (unsigned long long)sh.mass_min);
+    fill_bins(sh, (const T*)s.logits + row * s.stride, s, set, m, blockIdx.x);
+    for (int b = threadIdx.x; b < kBins; b += kThreads)
+        if (sh.mass[b]) (void)__hip_atomic_fetch_add(&space.bins[b], sh.mass[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (!last_to_arrive(&space.arrived[0], s.slices, &sh.last)) return;
-    for (int b = threadIdx.x; b < kBins; b += 256) {
-        sh.mass[b] = read_through(&space.mass[b]);
-        sh.count[b] = read_through(&space.count[b]);
-    }
-    if (threadIdx.x == 0) sh.mass_min = read_through(&space.mass_min);
+    for (int b = threadIdx.x; b < kBins; b += kThreads) sh.mass[b] = read_through(&space.bins[b]);
     __syncthreads();
     find_borders(sh, set);
-    for (int b = threadIdx.x; b <= kBins; b += 256) {
+    for (int b = threadIdx.x; b <= kBins; b += kThreads) {
         space.mass[b] = sh.mass[b];
         space.count[b] = sh.count[b];
     }
@@ -591,28 +612,32 @@ __global__ void __launch_bounds__(256) sample_bins_kernel(SampleParams s) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) sample_draw_kernel(SampleParams s) {
+__global__ void __launch_bounds__(kThreads) sample_draw_kernel(SampleParams s) {
     __shared__ Shared sh;
     __shared__ Lists li;
     const int64_t row = blockIdx.y;
     RowSpace& space = s.space[row];
     const T* logits = (const T*)s.logits + row * s.stride;
-    const uint32_t top = top_of(space, s.slices);
-    if (top <= kMinusInfinity) {
+    const float m = top_of(space, s.slices);
+    if (!(m > -__builtin_huge_valf())) {
         if (blockIdx.x == 0 && threadIdx.x == 0) no_answer(s, row);
         return;
     }
-    const float m = value_of(top);
     const Settings set = settings_of(s, row);
     const Borders r = space.borders;
-    if (!r.many)
-        for_each(logits, s.vocab, blockIdx.x, s.slices, [&](int i, float l) {
-            double x;
-            if (distance(l, m, set.inv_t, x) && wanted(r, bin_of(x)))
-                __hip_atomic_store(&space.list[atomicAdd(&space.listed, 1u)], order_of(l, i), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        });
+    if (!r.many) {   // a slice's elements are collected here and take their place in the row's list together
+        if (threadIdx.x == 0) sh.listed = 0;
+        __syncthreads();
+        for_wanted(logits, s, set, m, r, blockIdx.x, s.slices, [&](uint64_t o) { li.list[atomicAdd(&sh.listed, 1u)] = o; });
+        __syncthreads();
+        const uint32_t n = sh.listed;
+        if (threadIdx.x == 0) sh.last = n ? __hip_atomic_fetch_add(&space.listed, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+        __syncthreads();
+        const uint32_t at = sh.last;
+        for (uint32_t i = threadIdx.x; i < n; i += kThreads) __hip_atomic_store(&space.list[at + i], li.list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
     if (!last_to_arrive(&space.arrived[1], s.slices, &sh.last)) return;
-    for (int b = threadIdx.x; b <= kBins; b += 256) {
+    for (int b = threadIdx.x; b <= kBins; b += kThreads) {
         sh.mass[b] = space.mass[b];
         sh.count[b] = space.count[b];
     }
@@ -624,31 +649,31 @@ __global__ void __launch_bounds__(256) sample_draw_kernel(SampleParams s) {
         return;
     }
     const int n = (int)read_through(&space.listed);
-    for (int i = threadIdx.x; i < n; i += 256) li.list[i] = read_through(&space.list[i]);
+    for (int i = threadIdx.x; i < n; i += kThreads) li.list[i] = read_through(&space.list[i]);
     __syncthreads();
     draw_from_list(sh, li, s, row, set, m, n);
 }
 
-// Slices of a row: four workgroups of four wavefronts to a compute unit over all rows, none with less than 2048 elements; one where the rows
-// alone are as many as half of the compute units.
+// Slices of a row: one workgroup to a compute unit over all rows, none with less than 4096 elements; one where the rows alone are as many as
+// half of the compute units.
 int slices_of(int64_t rows, int64_t vocab, int cus) {
     if (2 * rows >= cus) return 1;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(kMaxSlices, 2 * cus / rows), vocab / 2048));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(kMaxSlices, cus / rows), vocab / 4096));
 }
 
 template <typename T>
 int run_sample(const SampleParams& s, int64_t rows, hipStream_t stream) {
     if (s.slices == 1) {
-        hipLaunchKernelGGL((sample_row_kernel<T>), dim3((unsigned)rows), dim3(1024), 0, stream, s);
+        hipLaunchKernelGGL((sample_row_kernel<T>), dim3((unsigned)rows), dim3(kThreads), 0, stream, s);
         CKV_HIP_TRY(hipGetLastError());
         return CKV_OK;
     }
     const dim3 grid(s.slices, (unsigned)rows);
-    hipLaunchKernelGGL((sample_max_kernel<T>), grid, dim3(256), 0, stream, s);
+    hipLaunchKernelGGL((sample_max_kernel<T>), grid, dim3(kThreads), 0, stream, s);
     CKV_HIP_TRY(hipGetLastError());
-    hipLaunchKernelGGL((sample_bins_kernel<T>), grid, dim3(256), 0, stream, s);
+    hipLaunchKernelGGL((sample_bins_kernel<T>), grid, dim3(kThreads), 0, stream, s);
     CKV_HIP_TRY(hipGetLastError());
-    hipLaunchKernelGGL((sample_draw_kernel<T>), grid, dim3(256), 0, stream, s);
+    hipLaunchKernelGGL((sample_draw_kernel<T>), grid, dim3(kThreads), 0, stream, s);
     CKV_HIP_TRY(hipGetLastError());
     return CKV_OK;
 }

@@ -12,7 +12,7 @@ import torch
 from . import _abi
 from .cascading_cache import _require_device, on_device, raw_stream
 
-MAX_VOCAB = (1 << 20) - 1
+MAX_VOCAB = (1 << 19) - 1
 
 #: setting: (field of one number, field of one a row, type of the array)
 _SETTINGS = {"temperature": ("temperature", "temperatures", torch.float32), "top_k": ("top_k", "top_ks", torch.int64),

@@ -406,8 +406,8 @@ int ckv_gated_linear_bwd(const void* x, const void* w, const void* gate_up, cons
  * logarithm of its share of the kept mass.  Settings are numbers for all rows or arrays with one a row.  temperature that is
  * not above 0: the first one.  top_k <= 0, top_p >= 1, min_p <= 0: no limit; top_p <= 0, min_p >= 1: the first one and (min_p)
  * its equals.  A uniform at or above 1 takes the last kept token, one below 0 the first.  Logits of NaN and minus infinity
- * are no tokens, one of plus infinity is the only one besides its equals; a row without tokens gives -1 and NaN.  Masses are
- * whole numbers of 2^-44 of the first one's: the same call gives the same tokens.  vocab < 2^20.
+ * are no tokens, one of plus infinity is the only one besides its equals; a row without tokens gives -1 and NaN.  Sums are
+ * of whole numbers: the same call gives the same tokens.  vocab < 2^19.
  * ---------------------------------------------------------------------------------------- */
 typedef struct ckv_sample_args {
     const void* logits;            /* (rows, vocab), elements of a row adjacent           */
