@@ -76,16 +76,20 @@ struct Settings {
 };
 
 __device__ inline Settings settings_of(const SampleParams& s, int64_t row) {
+    // all loads first, of something where there is no array: one trip to memory instead of five
+    const float u = s.uniforms[row], t_row = (s.temperature ? s.temperature : s.uniforms)[row], p_row = (s.top_p ? s.top_p : s.uniforms)[row],
+                least_row = (s.min_p ? s.min_p : s.uniforms)[row];
+    const int64_t k_row = s.top_k ? s.top_k[row] : s.top_k_all;
     Settings r;
-    const double t = s.temperature ? (double)s.temperature[row] : s.temperature_all;
-    const int64_t k = s.top_k ? s.top_k[row] : s.top_k_all;
+    const double t = s.temperature ? (double)t_row : s.temperature_all;
+    const int64_t k = k_row;
     r.k = k <= 0 || k > s.vocab ? s.vocab : (int)k;
     if (!(t > 0.0)) r.k = 1;   // the first one
     r.inv_t = t > 0.0 ? 1.0 / fmax(t, 1e-300) : 1.0;
-    r.p = s.top_p ? (double)s.top_p[row] : s.top_p_all;
-    const double least = s.min_p ? (double)s.min_p[row] : s.min_p_all;
+    r.p = s.top_p ? (double)p_row : s.top_p_all;
+    const double least = s.min_p ? (double)least_row : s.min_p_all;
     r.far_min = least > 0.0 ? (least < 1.0 ? -log(least) : 0.0) : 2 * kFar;
-    r.u = (double)s.uniforms[row];
+    r.u = (double)u;
     return r;
 }
 
@@ -209,6 +213,7 @@ struct Shared {
     uint32_t narrow[16];
     float tops[16];
     uint32_t listed, last;
+    int first[2], counted[2];
     Borders borders;
     unsigned long long answer[3];
 };
@@ -234,16 +239,22 @@ __device__ inline void fill_bins(Shared& sh, const T* row, const SampleParams& s
     __syncthreads();
 }
 
-// The first bin at whose end `reached` holds, which it then does behind every later one; the last bin if nowhere.
+// The first bins at whose ends `low` and `high` hold, which they then do behind every later one; the last bin if nowhere.
+template <typename Low, typename High>
+__device__ inline int2 first_bins(Shared& sh, Low low, High high) {
+    __syncthreads();
+    if (threadIdx.x == 0) sh.first[0] = sh.first[1] = kBins - 1;
+    __syncthreads();
+    for (int b = threadIdx.x; b < kBins; b += blockDim.x) {
+        if (low(b + 1) && (b == 0 || !low(b))) sh.first[0] = b;
+        if (high(b + 1) && (b == 0 || !high(b))) sh.first[1] = b;
+    }
+    __syncthreads();
+    return make_int2(sh.first[0], sh.first[1]);
+}
 template <typename Fn>
 __device__ inline int first_bin(Shared& sh, Fn reached) {
-    __syncthreads();
-    if (threadIdx.x == 0) sh.last = kBins - 1;
-    __syncthreads();
-    for (int b = threadIdx.x; b < kBins; b += blockDim.x)
-        if (reached(b + 1) && (b == 0 || !reached(b))) sh.last = b;
-    __syncthreads();
-    return sh.last;
+    return first_bins(sh, reached, [](int) { return false; }).x;
 }
 
 // u times a mass, as a whole number below it
@@ -303,8 +314,9 @@ __device__ inline void find_borders(Shared& sh, const Settings& set) {
     r.mass_k = high;
     if (set.p < 1.0) {
         const double t0 = set.p * (double)low, t1 = set.p * (double)high;
-        r.from[1] = first_bin(sh, [&](int e) { return (double)sh.mass[e] >= t0; });
-        r.to[1] = first_bin(sh, [&](int e) { return (double)sh.mass[e] >= t1; });
+        const int2 b = first_bins(sh, [&](int e) { return (double)sh.mass[e] >= t0; }, [&](int e) { return (double)sh.mass[e] >= t1; });
+        r.from[1] = b.x;
+        r.to[1] = b.y;
         low = min(low, max((uint64_t)sh.mass[r.from[1]], kOne));
         high = min(high, (uint64_t)sh.mass[r.to[1] + 1]);
     }
@@ -315,8 +327,9 @@ __device__ inline void find_borders(Shared& sh, const Settings& set) {
         high = min(high, (uint64_t)sh.mass[b + 1]);
     }
     const uint64_t d0 = draw_below(set.u, low), d1 = draw_below(set.u, high);
-    r.from[3] = first_bin(sh, [&](int e) { return sh.mass[e] > d0; });
-    r.to[3] = first_bin(sh, [&](int e) { return sh.mass[e] > d1; });
+    const int2 drawn = first_bins(sh, [&](int e) { return sh.mass[e] > d0; }, [&](int e) { return sh.mass[e] > d1; });
+    r.from[3] = drawn.x;
+    r.to[3] = drawn.y;
     uint32_t many = 0;
 #pragma unroll
     for (int i = 0; i < 4; i++)
@@ -334,18 +347,22 @@ __device__ inline bool wanted(const Borders& r, int b) {
 __device__ inline uint64_t order_of(float l, int i) { return ((uint64_t)~key_of(l) << 32) | (uint32_t)i; }
 __device__ inline float logit_of(uint64_t order) { return value_of(~(uint32_t)(order >> 32)); }
 
-// The elements of the borders' bins.  The bins of a border are a stretch of values: one comparison passes most of a row over.
+// The elements of the borders' bins.  All of them lie in one stretch of values: two comparisons pass most of a row over.
 template <typename T, typename Fn>
 __device__ inline void for_wanted(const T* row, const SampleParams& s, const Settings& set, float m, const Borders& r, int slice, int slices, Fn fn) {
-    int last = 0;
+    int low = kBins, high = 0;
 #pragma unroll
     for (int i = 0; i < 4; i++)
-        if (r.from[i] <= r.to[i]) last = max(last, r.to[i]);
-    // a bin further than the last one, and rounded down twice: below it nothing is wanted
-    const double lowest = (double)m - (last + 1.5) * kBinWidth / set.inv_t;
-    const float floor = lowest > -3.4e38 ? (float)lowest - fabsf((float)lowest) * 2.4e-7f : -__builtin_huge_valf();
+        if (r.from[i] <= r.to[i]) {
+            low = min(low, r.from[i]);
+            high = max(high, r.to[i]);
+        }
+    // a bin further on either side, and rounded outwards twice over
+    const double least = (double)m - (high + 1.5) * kBinWidth / set.inv_t, most = (double)m - (low - 1.5) * kBinWidth / set.inv_t;
+    const float floor = least > -3.4e38 ? (float)least - fabsf((float)least) * 2.4e-7f : -__builtin_huge_valf();
+    const float ceiling = most < 3.4e38 ? (float)most + fabsf((float)most) * 2.4e-7f : __builtin_huge_valf();
     for_each(row, s.vocab, slice, slices, [&](int i, float l) {
-        if (l < floor) return;
+        if (l < floor || l > ceiling) return;
         double x;
         if (distance(l, m, set.inv_t, x) && wanted(r, (int)bin_of(x))) fn(order_of(l, i));
     });
@@ -363,22 +380,40 @@ __device__ inline void answer(const SampleParams& s, int64_t row, const Settings
 // From the elements of the borders' bins, n of them.
 __device__ inline void draw_from_list(Shared& sh, Lists& li, const SampleParams& s, int64_t row, const Settings& set, float m, int n) {
     const Borders r = sh.borders;
-    int size = 2;
-    while (size < n) size <<= 1;
-    for (int i = n + threadIdx.x; i < size; i += blockDim.x) li.list[i] = ~0ull;
-    __syncthreads();
-    for (int k = 2; k <= size; k <<= 1)
-        for (int j = k >> 1; j > 0; j >>= 1) {
-            for (int i = threadIdx.x; i < size / 2; i += blockDim.x) {
-                const int a = 2 * i - (i & (j - 1)), b = a + j;
-                const uint64_t va = li.list[a], vb = li.list[b];
-                if ((va > vb) == ((a & k) == 0)) {
-                    li.list[a] = vb;
-                    li.list[b] = va;
+    if (n <= kThreads / 2) {   // an element's place is the number of smaller ones, counted by as many threads as there are for each
+        int log = 1;
+        while (log < 6 && (n << (log + 1)) <= kThreads) log++;
+        const int element = threadIdx.x >> log, part = threadIdx.x & ((1 << log) - 1);
+        const uint64_t mine = element < n ? li.list[element] : 0;
+        int place = 0;
+        if ((int)((threadIdx.x & ~63u) >> log) < n)
+            for (int i = part; i < n; i += 1 << log) place += li.list[i] < mine;
+        for (int o = (1 << log) >> 1; o > 0; o >>= 1) place += __shfl_xor(place, o);
+        __syncthreads();
+        if (element < n && part == 0) li.list[place] = mine;
+        __syncthreads();
+    } else {
+        // A thread compares one pair a step, a wavefront those of 128 neighbours: steps within them need no other wavefront.
+        int size = kThreads;
+        while (size < n) size <<= 1;
+        for (int i = n + threadIdx.x; i < size; i += kThreads) li.list[i] = ~0ull;
+        __syncthreads();
+        for (int k = 2; k <= size; k <<= 1)
+            for (int j = k >> 1; j > 0; j >>= 1) {
+                if (j >= 2 * CKV_WAVE) __syncthreads();
+                if ((int)threadIdx.x < size / 2) {
+                    const int i = threadIdx.x, a = 2 * i - (i & (j - 1)), b = a + j;
+                    const uint64_t va = li.list[a], vb = li.list[b];
+                    if ((va > vb) == ((a & k) == 0)) {
+                        li.list[a] = vb;
+                        li.list[b] = va;
+                    }
                 }
+                if (j >= 2 * CKV_WAVE) __syncthreads();
+                else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             }
-            __syncthreads();
-        }
+        __syncthreads();
+    }
     // A thread has two neighbours at most.  The running mass up to an element is that of the bins in front of its own and of the beginning of its
     // bin up to it: the weights between, counts and rests, are added up over the list, and the element where the bin begins is looked up.
     static_assert(kListMax <= 2 * kThreads, "two a thread");
@@ -415,31 +450,48 @@ __device__ inline void draw_from_list(Shared& sh, Lists& li, const SampleParams&
     if (threadIdx.x == 0) {
         sh.answer[0] = r.mass_k;
         sh.answer[1] = sh.answer[2] = kOne;
+        sh.counted[0] = sh.counted[1] = 0;
         sh.listed = 0;
     }
     __syncthreads();
-    for (int e = 0; e < each; e++)
-        if (first + e < n) {
+    // How many of the list, which are its first ones: top-p and min-p keep beginnings of it.
+    auto count = [&](int which, bool a, bool b) {
+        const int many = __popcll(__ballot(a)) + __popcll(__ballot(b));
+        if ((threadIdx.x & 63) == 0 && many) atomicAdd(&sh.counted[which], many);
+    };
+    const bool there[2] = {first < n, each == 2 && first + 1 < n};
+#pragma unroll
+    for (int e = 0; e < 2; e++)
+        if (there[e]) {
             const uint32_t from = (begin[e] ? begin[e] : begun) - 1;
             const uint64_t in_front = li.before[first + e] - li.before[from];
             run[e] = sh.mass[bin[e]] + mass_of(bin[e], in_front + some[e], sh.table);
             some[e] = sh.mass[bin[e]] + mass_of(bin[e], in_front, sh.table);   // and before it
             if (r.partial_k && sh.count[bin[e]] + (first + e - from) + 1 == (uint32_t)set.k) sh.answer[0] = run[e];
-            if (x[e] <= set.far_min) atomicMax(&sh.answer[2], (unsigned long long)run[e]);
         }
+    if (set.far_min < kFar) count(0, there[0] && x[0] <= set.far_min, there[1] && x[1] <= set.far_min);
     __syncthreads();
     uint64_t kept = sh.answer[0];
-    if (set.p < 1.0) {   // the last one that has less than p of that before it
+    if (set.p < 1.0) {   // those that have less than p of that before them
         const double t = set.p * (double)kept;
-        for (int e = 0; e < each; e++)
-            if (first + e < n && (double)some[e] < t) atomicMax(&sh.answer[1], (unsigned long long)run[e]);
-        __syncthreads();
-        kept = min(kept, (uint64_t)sh.answer[1]);
+        count(1, there[0] && (double)some[0] < t, there[1] && (double)some[1] < t);
     }
-    if (set.far_min < kFar) kept = min(kept, max((uint64_t)sh.answer[2], (uint64_t)sh.mass[r.from[2]]));
+    if (set.p < 1.0 || set.far_min < kFar) {
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+            if (there[e]) {
+                if (first + e + 1 == sh.counted[1]) sh.answer[1] = run[e];
+                if (first + e + 1 == sh.counted[0]) sh.answer[2] = run[e];
+            }
+        __syncthreads();
+        if (set.p < 1.0) kept = min(kept, (uint64_t)sh.answer[1]);
+        if (set.far_min < kFar) kept = min(kept, max((uint64_t)sh.answer[2], (uint64_t)sh.mass[r.from[2]]));
+    }
     const uint64_t d = draw_below(set.u, kept);
-    for (int e = 0; e < each; e++)
-        if (first + e < n && run[e] > d && some[e] <= d) sh.listed = first + e;
+#pragma unroll
+    for (int e = 0; e < 2; e++)
+        if (there[e] && run[e] > d && some[e] <= d) sh.listed = first + e;
     __syncthreads();
     if (threadIdx.x == 0) answer(s, row, set, m, li.list[sh.listed], kept);
 }
