@@ -15,6 +15,9 @@
 namespace ckv {
 namespace {
 
+constexpr int kMaxHeadDim = 256;
+constexpr int kMostBlocks = 2048, kMostChunks = 64;   // of a backward launch
+
 struct NormSide {
     const void* x;
     const void* weight;     // (D) or null: no norm
@@ -109,6 +112,23 @@ struct Share {
                 }
             }
     }
+    // The same in two steps: the loads, which the next head's work is put behind, and the conversion.
+    using Raw = Vec<T, kVec>[kSlots][2];
+    __device__ void fetch(const T* row, Raw& v) const {
+#pragma unroll
+        for (int i = 0; i < kSlots; i++)
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+                if (at[i][u] >= 0) v[i][u] = *reinterpret_cast<const Vec<T, kVec>*>(row + at[i][u]);
+    }
+    __device__ void convert(const Raw& raw, float (&v)[kSlots][2][kVec]) const {
+#pragma unroll
+        for (int i = 0; i < kSlots; i++)
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int e = 0; e < kVec; e++) v[i][u][e] = at[i][u] >= 0 ? Elem<T>::to_float(raw[i][u].v[e]) : 0.f;
+    }
     __device__ void store(T* row, const float (&v)[kSlots][2][kVec]) const {
 #pragma unroll
         for (int i = 0; i < kSlots; i++)
@@ -183,7 +203,7 @@ __global__ void __launch_bounds__(256) norm_rotate_kernel(NormParams p) {
 // order, no atomics.
 template <typename T, int kVec, int kSlots>
 __global__ void __launch_bounds__(256) norm_rotate_bwd_kernel(NormParams p) {
-    __shared__ float sums[256];
+    __shared__ float sums[4][kMaxHeadDim];
     const bool keys = blockIdx.y >= (unsigned)p.side[0].chunks;
     const NormSide& side = p.side[keys];
     const int chunk = blockIdx.y - (keys ? p.side[0].chunks : 0);
@@ -202,10 +222,17 @@ __global__ void __launch_bounds__(256) norm_rotate_bwd_kernel(NormParams p) {
         const T* from = (const T*)side.x + b * side.x_stride[0] + t * side.x_stride[2];
         const T* grad = (const T*)side.grad + b * side.grad_stride[0] + t * side.grad_stride[2];
         T* to = (T*)side.out + b * side.out_stride[0] + t * side.out_stride[2];
+        typename Share<T, kVec, kSlots>::Raw raw_x = {}, raw_g = {};
+        share.fetch(grad + h0 * side.grad_stride[1], raw_g);
+        if (side.weight) share.fetch(from + h0 * side.x_stride[1], raw_x);
         for (int h = h0; h < h1; h++) {
             float x[kSlots][2][kVec], g[kSlots][2][kVec];
-            share.load(grad + h * side.grad_stride[1], g);
-            if (side.weight) share.load(from + h * side.x_stride[1], x);
+            share.convert(raw_g, g);
+            if (side.weight) share.convert(raw_x, x);
+            if (h + 1 < h1) {   // in flight while this head is worked on
+                share.fetch(grad + (h + 1) * side.grad_stride[1], raw_g);
+                if (side.weight) share.fetch(from + (h + 1) * side.x_stride[1], raw_x);
+            }
 #pragma unroll
             for (int i = 0; i < kSlots; i++)
                 if (share.turned[i]) {
@@ -249,6 +276,7 @@ __global__ void __launch_bounds__(256) norm_rotate_bwd_kernel(NormParams p) {
     }
     if (!side.weight) return;
     float* row = side.partial + ((int64_t)blockIdx.x * side.chunks + chunk) * p.D;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
     for (int i = 0; i < kSlots; i++)
 #pragma unroll
@@ -257,13 +285,10 @@ __global__ void __launch_bounds__(256) norm_rotate_bwd_kernel(NormParams p) {
             for (int e = 0; e < kVec; e++) {
                 float s = dw[i][u][e];
                 for (int o = lanes; o < CKV_WAVE; o <<= 1) s += __shfl_xor(s, o);
-                const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-                __syncthreads();
-                if (lane < lanes) sums[wave * 64 + lane] = s;
-                __syncthreads();
-                if (threadIdx.x < (unsigned)lanes && share.at[i][u] >= 0)
-                    row[share.at[i][u] + e] = (sums[lane] + sums[64 + lane]) + (sums[128 + lane] + sums[192 + lane]);
+                if (lane < lanes && share.at[i][u] >= 0) sums[wave][share.at[i][u] + e] = s;
             }
+    __syncthreads();
+    for (int d = threadIdx.x; d < p.D; d += 256) row[d] = (sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d]);
 }
 
 struct WeightGradients {
@@ -273,26 +298,30 @@ struct WeightGradients {
     int D;
 };
 
-// Column sums of the blocks' rows: 32 columns a workgroup, 32 threads a column.
+// Column sums of the blocks' rows: 8 columns a workgroup, 128 threads a column, four rows in flight a thread.
 template <typename T>
 __global__ void __launch_bounds__(1024) weight_gradient_kernel(WeightGradients p) {
-    __shared__ float sums[32][33];
-    const int col = threadIdx.x & 31, part = threadIdx.x >> 5, side = blockIdx.y;
-    const int at = blockIdx.x * 32 + col;
-    float s = 0.f;
+    __shared__ float sums[16][8];
+    const int col = threadIdx.x & 7, part = threadIdx.x >> 3, side = blockIdx.y;
+    const int at = blockIdx.x * 8 + col, rows = p.rows[side];
+    float s[4] = {};
     if (at < p.D)
-        for (int r = part; r < p.rows[side]; r += 32) s += p.partial[side][(int64_t)r * p.D + at];
-    sums[part][col] = s;
+        for (int r = part; r < rows; r += 512) {
+            const float* from = p.partial[side] + (int64_t)r * p.D + at;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (r + i * 128 < rows) s[i] += from[(int64_t)i * 128 * p.D];
+        }
+    float all = (s[0] + s[1]) + (s[2] + s[3]);
+    for (int o = 8; o < CKV_WAVE; o <<= 1) all += __shfl_xor(all, o);
+    if ((threadIdx.x & 63) < 8) sums[threadIdx.x >> 6][col] = all;
     __syncthreads();
-    if (part == 0 && at < p.D) {
-        float all = 0.f;
-        for (int i = 0; i < 32; i++) all += sums[i][col];
+    if (threadIdx.x < 8 && at < p.D) {
+        all = 0.f;
+        for (int i = 0; i < 16; i++) all += sums[i][col];
         ((T*)p.out[side])[at] = Elem<T>::from_float(all);
     }
 }
-
-constexpr int kMaxHeadDim = 256;
-constexpr int kMostBlocks = 1024, kMostChunks = 64;   // of a backward launch
 
 bool vectors_fit(const ckv_norm_rotate_args* a, bool backward, int vec) {
     const int64_t bytes = vec * elem_bytes(a->dtype);
@@ -326,7 +355,8 @@ int launch_norm(NormParams& p, const ckv_norm_rotate_args* a, bool backward, int
         CKV_HIP_TRY(hipGetLastError());
         return CKV_OK;
     }
-    const int gx = (int)std::min<int64_t>(blocks, std::max(1, kMostBlocks / chunks));
+    const int64_t most = std::max(1, kMostBlocks / chunks), rounds = (blocks + most - 1) / most;
+    const int gx = (int)((blocks + rounds - 1) / rounds);   // so that no block has a round more than most of the others
     p.side[0].partial = (float*)a->workspace;
     p.side[1].partial = p.side[0].partial + (int64_t)gx * p.side[0].chunks * p.D;
     hipLaunchKernelGGL((norm_rotate_bwd_kernel<T, kVec, kSlots>), dim3(gx, chunks), dim3(256), 0, stream, p);
@@ -340,7 +370,7 @@ int launch_norm(NormParams& p, const ckv_norm_rotate_args* a, bool backward, int
     g.out[0] = a->dq_weight;
     g.out[1] = a->dk_weight;
     g.D = p.D;
-    hipLaunchKernelGGL((weight_gradient_kernel<T>), dim3((p.D + 31) / 32, 2), dim3(1024), 0, stream, g);
+    hipLaunchKernelGGL((weight_gradient_kernel<T>), dim3((p.D + 7) / 8, 2), dim3(1024), 0, stream, g);
     CKV_HIP_TRY(hipGetLastError());
     return CKV_OK;
 }

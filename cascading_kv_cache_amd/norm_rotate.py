@@ -19,70 +19,99 @@ from .cascading_cache import _require_device, on_device, raw_stream
 MAX_HEAD_DIM = 256
 
 
-def _describe(q, k, q_weight, k_weight, positions, inv_freq, eps):
-    a = _abi.NormRotateArgs()
+# What is known of a call by its tensors' sizes, strides, types and devices alone: that the checks passed, and the argument block without
+# pointers.  Nothing of a tensor's address or contents.  A single token's call is bound by the host: 19 us with all of this every time.
+_LAYOUTS = {}
+
+
+class _Layout:
+    def __init__(self, q, k, q_weight, k_weight, positions, inv_freq, out):
+        a = _abi.NormRotateArgs()
+        self._strides(a, q_stride=q, k_stride=k)
+        if inv_freq is not None:
+            a.pos_stride = positions.stride(0) if positions.ndim == 2 and positions.size(0) > 1 else 0
+            a.rot = 2 * inv_freq.numel()
+        a.B, a.H, a.n, a.D = q.shape
+        a.KVH = k.size(1)
+        a.dtype = _abi.dtype_code(q.dtype)
+        self.common = bytes(a)
+        # not torch.empty_like: the inputs are usually parts of one wider buffer, and may be expanded
+        self._strides(a, **dict(zip(("q_out_stride", "k_out_stride"), out or (q.new_empty(q.shape), k.new_empty(k.shape)))))
+        self.forward = bytes(a)
+        self.backward = {}
+        self.scratch = _abi.lib().ckv_norm_rotate_workspace_bytes(a.D)
+
+    @staticmethod
+    def _strides(a, **tensors):
+        for field, t in tensors.items():
+            array = getattr(a, field)
+            _abi.set_strides(array, t)
+            array[3] = 1   # of a single head dim torch may say anything
+
+    def block(self, grads=None, dq=None, dk=None):
+        """A copy of the block (the backward runs on a thread of autograd's own)."""
+        if grads is None:
+            return _abi.NormRotateArgs.from_buffer_copy(self.forward)
+        key = (grads[0].stride(), grads[1].stride())
+        known = self.backward.get(key)
+        if known is None:
+            a = _abi.NormRotateArgs.from_buffer_copy(self.common)
+            self._strides(a, q_grad_stride=grads[0], k_grad_stride=grads[1], dq_stride=dq, dk_stride=dk)
+            if len(self.backward) > 64:
+                self.backward.clear()
+            known = self.backward[key] = bytes(a)
+        return _abi.NormRotateArgs.from_buffer_copy(known)
+
+
+def _point(a, q, k, q_weight, k_weight, positions, inv_freq, eps):
     a.q, a.k = q.data_ptr(), k.data_ptr()
-    _abi.set_strides(a.q_stride, q)
-    _abi.set_strides(a.k_stride, k)
-    a.q_stride[3] = a.k_stride[3] = 1   # of a single head dim torch may say anything
     if q_weight is not None:
         a.q_weight, a.k_weight = q_weight.data_ptr(), k_weight.data_ptr()
     if inv_freq is not None:
         a.positions, a.inv_freq = positions.data_ptr(), inv_freq.data_ptr()
-        a.pos_stride = positions.stride(0) if positions.ndim == 2 and positions.size(0) > 1 else 0
-        a.rot = 2 * inv_freq.numel()
-    a.B, a.H, a.n, a.D = q.shape
-    a.KVH = k.size(1)
-    a.eps = float(eps)
-    a.dtype = _abi.dtype_code(q.dtype)
-    return a
+    a.eps = eps
 
 
-def _forward(q, k, q_weight, k_weight, positions, inv_freq, eps, out=None):
-    # not torch.empty_like: the inputs are usually parts of one wider buffer, and may be expanded
-    q_out, k_out = out or (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
-    a = _describe(q, k, q_weight, k_weight, positions, inv_freq, eps)
+def _forward(layout, q, k, q_weight, k_weight, positions, inv_freq, eps, out=None):
+    q_out, k_out = out or (q.new_empty(q.shape), k.new_empty(k.shape))
+    a = layout.block()
+    _point(a, q, k, q_weight, k_weight, positions, inv_freq, eps)
     a.q_out, a.k_out = q_out.data_ptr(), k_out.data_ptr()
-    _abi.set_strides(a.q_out_stride, q_out)
-    _abi.set_strides(a.k_out_stride, k_out)
-    a.q_out_stride[3] = a.k_out_stride[3] = 1
-    with on_device(q.device):
-        _abi.check(_abi.lib().ckv_norm_rotate(C.byref(a), C.c_void_p(raw_stream(q.device))), "ckv_norm_rotate")
+    device = q.device
+    with on_device(device):
+        _abi.check(_abi.lib().ckv_norm_rotate(C.byref(a), raw_stream(device)), "ckv_norm_rotate")
     return q_out, k_out
 
 
 class _NormRotate(torch.autograd.Function):
 
     @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, positions, inv_freq, eps):
+    def forward(ctx, layout, eps, q, k, q_weight, k_weight, positions, inv_freq):
         ctx.save_for_backward(q, k, q_weight, k_weight, positions, inv_freq)
-        ctx.eps = eps
-        return _forward(q, k, q_weight, k_weight, positions, inv_freq, eps)
+        ctx.layout, ctx.eps = layout, eps
+        return _forward(layout, q, k, q_weight, k_weight, positions, inv_freq, eps)
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, q_grad, k_grad):
+    def backward(ctx, *grads):
         q, k, q_weight, k_weight, positions, inv_freq = ctx.saved_tensors
         # a gradient may be an expanded scalar, or in an order of its own
-        q_grad, k_grad = (g if g.stride(-1) == 1 or g.size(-1) == 1 else g.contiguous() for g in (q_grad.to(q.dtype), k_grad.to(q.dtype)))
-        a = _describe(q, k, q_weight, k_weight, positions, inv_freq, ctx.eps)
-        a.q_grad, a.k_grad = q_grad.data_ptr(), k_grad.data_ptr()
-        dq, dk = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
-        a.dq, a.dk = dq.data_ptr(), dk.data_ptr()
-        for field, t in ((a.q_grad_stride, q_grad), (a.k_grad_stride, k_grad), (a.dq_stride, dq), (a.dk_stride, dk)):
-            _abi.set_strides(field, t)
-            field[3] = 1
+        q_grad, k_grad = (g if g.stride(-1) == 1 or g.size(-1) == 1 else g.contiguous() for g in grads)
+        dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
+        a = ctx.layout.block((q_grad, k_grad), dq, dk)
+        _point(a, q, k, q_weight, k_weight, positions, inv_freq, ctx.eps)
+        a.q_grad, a.k_grad, a.dq, a.dk = q_grad.data_ptr(), k_grad.data_ptr(), dq.data_ptr(), dk.data_ptr()
         dqw = dkw = None
-        lib = _abi.lib()
-        with on_device(q.device):
+        device = q.device
+        with on_device(device):
             if q_weight is not None:
-                dqw, dkw = torch.empty_like(q_weight), torch.empty_like(k_weight)
+                dqw, dkw = q_weight.new_empty(q_weight.shape), k_weight.new_empty(k_weight.shape)
                 a.dq_weight, a.dk_weight = dqw.data_ptr(), dkw.data_ptr()
                 # of this call alone: a graph that records it must share its scratch with nobody
-                ws = torch.empty(lib.ckv_norm_rotate_workspace_bytes(a.D), dtype=torch.uint8, device=q.device)
-                a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-            _abi.check(lib.ckv_norm_rotate_bwd(C.byref(a), C.c_void_p(raw_stream(q.device))), "ckv_norm_rotate_bwd")
-        return dq, dk, dqw, dkw, None, None, None
+                ws = torch.empty(ctx.layout.scratch, dtype=torch.uint8, device=device)
+                a.workspace, a.workspace_bytes = ws.data_ptr(), ctx.layout.scratch
+            _abi.check(_abi.lib().ckv_norm_rotate_bwd(C.byref(a), raw_stream(device)), "ckv_norm_rotate_bwd")
+        return None, None, dq, dk, dqw, dkw, None, None
 
 
 def _check(q, k, q_weight, k_weight, positions, inv_freq):
@@ -138,17 +167,28 @@ def norm_rotate(q, k, q_weight=None, k_weight=None, positions=None, inv_freq=Non
     weights of the norm, or None for no norm.  ``positions`` int64 ``(n,)`` or ``(B, n)`` and ``inv_freq`` float32 ``(R / 2,)``: the first
     R <= D dims are rotated, dim j with dim j + R / 2 by ``position * inv_freq[j]``; or None for no rotation.  Gradients go back to q, k
     and the weights (once: not a second time).  Works under graph capture; nothing is kept between calls."""
-    _check(q, k, q_weight, k_weight, positions, inv_freq)
-    q, k = (t if t.stride(-1) == 1 or t.size(-1) == 1 else t.contiguous() for t in (q, k))
-    q_weight, k_weight, inv_freq = (None if t is None else t.contiguous() for t in (q_weight, k_weight, inv_freq))
-    if positions is not None and positions.stride(-1) != 1:
-        positions = positions.contiguous()
-    followed = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight))
+    tensors = q, k, q_weight, k_weight, positions, inv_freq
+    followed = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors[:4])
     if out is not None:
         if followed:
             raise ValueError("no gradients go through out")
-        _check_out(out, q, k)
-        return _forward(q, k, q_weight, k_weight, positions, inv_freq, eps, tuple(out))
+        out = tuple(out)
+    key = [(t.shape, t.stride(), t.dtype, t.device) if t is not None else None for t in (tensors if out is None else tensors + out)]
+    key = tuple(key)
+    layout = _LAYOUTS.get(key)
+    if layout is None or (inv_freq is not None and inv_freq.requires_grad):
+        _check(*tensors)
+        if out is not None:
+            _check_out(out, q, k)
+        q, k = (t if t.stride(-1) == 1 or t.size(-1) == 1 else t.contiguous() for t in (q, k))
+        q_weight, k_weight, inv_freq = (None if t is None else t.contiguous() for t in (q_weight, k_weight, inv_freq))
+        if positions is not None and positions.stride(-1) != 1:
+            positions = positions.contiguous()
+        layout = _Layout(q, k, q_weight, k_weight, positions, inv_freq, out)
+        if all(a is b for a, b in zip(tensors, (q, k, q_weight, k_weight, positions, inv_freq))):   # nothing to lay out at the next call either
+            if len(_LAYOUTS) > 256:
+                _LAYOUTS.clear()
+            _LAYOUTS[key] = layout
     if followed:
-        return _NormRotate.apply(q, k, q_weight, k_weight, positions, inv_freq, float(eps))
-    return _forward(q, k, q_weight, k_weight, positions, inv_freq, eps)
+        return _NormRotate.apply(layout, float(eps), q, k, q_weight, k_weight, positions, inv_freq)
+    return _forward(layout, q, k, q_weight, k_weight, positions, inv_freq, float(eps), out)
