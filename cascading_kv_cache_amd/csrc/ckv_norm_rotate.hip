@@ -167,9 +167,12 @@ __global__ void __launch_bounds__(256) norm_rotate_kernel(NormParams p) {
     share.angles(p, b, t, sn, cs);
     const T* from = (const T*)side.x + b * side.x_stride[0] + t * side.x_stride[2];
     T* to = (T*)side.out + b * side.out_stride[0] + t * side.out_stride[2];
+    typename Share<T, kVec, kSlots>::Raw raw = {};
+    share.fetch(from + h0 * side.x_stride[1], raw);
     for (int h = h0; h < h1; h++) {
         float x[kSlots][2][kVec];
-        share.load(from + h * side.x_stride[1], x);
+        share.convert(raw, x);
+        if (h + 1 < h1) share.fetch(from + (h + 1) * side.x_stride[1], raw);   // in flight while this head is worked on
         if (side.weight) {
             float s = 0.f;
 #pragma unroll
