@@ -13,73 +13,118 @@
 namespace ckv {
 namespace {
 
-// ---- any type, stride and size: float32 products on v_mfma_f32_32x32x2 -----------------------------------------------------------------
+// ---- any type, stride and size: float32 products on v_mfma_f32_16x16x4 -----------------------------------------------------------------
 
-constexpr int kTile = 128, kStep = 16, kPitch = kTile + 4;
+// kTile 128: eight wavefronts of 32 x 64, two on a SIMD: one's loads and stores stand beside the other's products.  64: four of 32 x 32, of
+// which several workgroups share a compute unit.
+constexpr int kStep = 32;
+template <int kTile>
+constexpr int kThreads = kTile == 128 ? 512 : 256;
 
-// A thread's four elements of a tile of 128 rows and 16 steps: along k of one row, or along the rows of one step.  Inside the operand they are
-// read at a time, from whatever address (an odd number of float32 a row: 1023 columns, 509 rows and 5462, 64 us by elements and 52 so).
-template <typename T, bool kAlongK>
-struct Piece {
-    struct __attribute__((packed, aligned(sizeof(T)))) Four {
-        T v[4];
-    };
-    int row, step;   // of the first
-    float v[4];
-    __device__ Piece() {
-        row = kAlongK ? threadIdx.x >> 2 : (threadIdx.x & 31) * 4;
-        step = kAlongK ? (threadIdx.x & 3) * 4 : threadIdx.x >> 5;
-    }
-    // base: the operand's row 0; `first` the tile's first row, counted from base; rows behind `rows` and steps behind `end` are zeros
-    __device__ void load(const T* base, int64_t stride, int64_t first, int64_t rows, int64_t k, int64_t end) {
-        const int64_t r = first + row, s = k + step;
-        const T* at = base + (kAlongK ? r * stride + s : s * stride + r);
-        if (kAlongK ? r < rows && s + 4 <= end : s < end && r + 4 <= rows) {
-            const Four x = *reinterpret_cast<const Four*>(at);
-#pragma unroll
-            for (int i = 0; i < 4; i++) v[i] = Elem<T>::to_float(x.v[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const bool there = kAlongK ? r < rows && s + i < end : s < end && r + i < rows;
-                v[i] = there ? Elem<T>::to_float(at[i]) : 0.f;
-            }
-        }
-    }
-    __device__ void store(float (*tile)[kPitch]) const {
+// A tile of kTile rows and 32 steps in LDS.  A product takes four steps, one from each quarter of a wavefront's lanes; which ones does not matter as
+// long as both operands' are the same.
+//
+// Of an operand along k, four steps of a row are a piece of 16 bytes, which a lane reads for four products.  Rows are 16 steps long, the other 16 half
+// the banks on; a row's four pieces change places from four rows to the next, so that the sixteen lanes that read at a time, of two quarters and
+// eight rows each, meet in no bank.  Of one along its rows, a step's rows lie together, as they are loaded, and a step is 4 banks from the next: the
+// quarters' steps, four apart, meet in no bank either.
+template <bool kAlongK, int kTile>
+struct Stage {
+    static constexpr int kHalf = kTile * 16 + 32, kPitch = kTile + 4;
+    float v[kAlongK ? 2 * kHalf : kStep * kPitch];
+    __device__ static int place(int row, int piece) { return (piece >> 2) * kHalf + row * 16 + (((piece & 3) ^ (0x78 >> ((row >> 1) & 6) & 3)) << 2); }
+    __device__ f32x4_t read(int row, int piece) const {
         if constexpr (kAlongK) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) tile[step + i][row] = v[i];
+            return *reinterpret_cast<const f32x4_t*>(v + place(row, piece));
         } else {
-            *reinterpret_cast<float4*>(&tile[step][row]) = make_float4(v[0], v[1], v[2], v[3]);
+            f32x4_t r;
+#pragma unroll
+            for (int e = 0; e < 4; e++) r[e] = v[(4 * piece + e) * kPitch + row];
+            return r;
         }
     }
 };
 
-// Eight wavefronts of 32 x 64, two on a SIMD: one's loads and stores stand beside the other's products.
-template <typename T, bool kAlongKA, bool kAlongKB, Epilogue kEpilogue>
-__global__ void __launch_bounds__(512) product_kernel(ProductParams p) {
-    __shared__ __align__(16) float as[2][kStep][kPitch], bs[2][kStep][kPitch];
+// A thread's two pieces of a tile: four adjacent elements, along k of a row or along the rows of a step.  Inside the operand they are read at a
+// time, from whatever address: rows of an odd number of elements have no better one.
+template <typename T, bool kAlongK, int kTile>
+struct Pieces {
+    struct __attribute__((packed, aligned(sizeof(T)))) Four {
+        T v[4];
+    };
+    static constexpr int kAcross = kAlongK ? kStep / 4 : kTile / 4;   // pieces side by side
+    const T* at[2];
+    int left[2];   // rows from the first element's on
+    float v[2][4];
+    __device__ static int row(int i) {
+        return kAlongK ? (int)(threadIdx.x / kAcross) + i * (kThreads<kTile> / kAcross) : (int)(threadIdx.x % kAcross) * 4;
+    }
+    __device__ static int step(int i) {
+        return kAlongK ? (int)(threadIdx.x % kAcross) * 4 : (int)(threadIdx.x / kAcross) + i * (kThreads<kTile> / kAcross);
+    }
+    // r: the row of the operand that piece i begins with, of `rows`
+    __device__ void set(int i, const T* base, int64_t stride, int64_t r, int64_t rows, int64_t k) {
+        at[i] = base + (kAlongK ? r * stride + k + step(i) : (k + step(i)) * stride + r);
+        left[i] = (int)max((int64_t)0, min((int64_t)kTile, rows - r));
+    }
+    // steps behind `more` and rows behind the last are zeros
+    __device__ void load(int64_t stride, int64_t more) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            if (left[i] >= (kAlongK ? 1 : 4) && (more >= kStep || step(i) + (kAlongK ? 4 : 1) <= more)) {
+                const Four x = *reinterpret_cast<const Four*>(at[i]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[i][e] = Elem<T>::to_float(x.v[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const bool there = kAlongK ? left[i] > 0 && step(i) + e < more : left[i] > e && step(i) < more;
+                    v[i][e] = there ? Elem<T>::to_float(at[i][e]) : 0.f;
+                }
+            }
+            at[i] += kAlongK ? kStep : kStep * stride;
+        }
+    }
+    __device__ void store(Stage<kAlongK, kTile>& stage) const {
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            *reinterpret_cast<f32x4_t*>(stage.v + (kAlongK ? stage.place(row(i), step(i) / 4) : step(i) * stage.kPitch + row(i))) =
+                f32x4_t{v[i][0], v[i][1], v[i][2], v[i][3]};
+    }
+};
+
+template <typename T, bool kAlongKA, bool kAlongKB, Epilogue kEpilogue, int kTile>
+__global__ void __launch_bounds__(kThreads<kTile>) product_kernel(ProductParams p) {
+    __shared__ __align__(16) Stage<kAlongKA, kTile> as[2];
+    __shared__ __align__(16) Stage<kAlongKB, kTile> bs[2];
     int tm, tn, share;
     float* sums = work_of<8>(p, kTile * kTile, tm, tn, share);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1, half = lane >> 5, l = lane & 31;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1, quarter = lane >> 4, l = lane & 15;
     constexpr bool kGated = kEpilogue == kGate;
+    constexpr int kAcross = kTile / 32;   // products of a wavefront side by side; gated, the second half are up columns of the first's gates
     const int64_t inter = p.N / 2;
     const int64_t m0 = (int64_t)tm * kTile, n0 = (int64_t)tn * (kGated ? kTile / 2 : kTile);
     const int64_t k0 = share * p.k_share, k1 = sums ? min(p.K, k0 + p.k_share) : p.K;
-    Piece<T, kAlongKA> pa;
-    Piece<T, kAlongKB> pb;
+    Pieces<T, kAlongKA, kTile> pa;
+    Pieces<T, kAlongKB, kTile> pb;
     const T* a = (const T*)p.a.p;
     const T* b = (const T*)p.b.p;
-    // gated: rows 0..63 of B's tile are gate rows, 64..127 up rows
-    const bool up = kGated && pb.row >= kTile / 2;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        pa.set(i, a, p.a.stride, m0 + pa.row(i), p.M, k0);
+        // gated: the first half of the rows of B's tile are gate rows, the others up rows
+        const int row = pb.row(i), up = kGated && row >= kTile / 2;
+        pb.set(i, b + (up ? inter * p.b.stride : 0), p.b.stride, n0 + row - (up ? kTile / 2 : 0), kGated ? inter : p.N, k0);
+    }
     auto load = [&](int64_t k) {
-        pa.load(a, p.a.stride, m0, p.M, k, k1);
-        if constexpr (kGated) pb.load(b + (up ? inter * p.b.stride : 0), p.b.stride, n0 - (up ? kTile / 2 : 0), inter, k, k1);
-        else pb.load(b, p.b.stride, n0, p.N, k, k1);
+        pa.load(p.a.stride, k1 - k);
+        pb.load(p.b.stride, k1 - k);
+    };
+    auto column = [&](int j) {   // of the tile's, the first of a product
+        return kGated ? (j / (kAcross / 2)) * (kTile / 2) + wn * (kTile / 4) + j % (kAcross / 2) * 16 : wn * (kTile / 2) + j * 16;
     };
     const bool there = m0 + wm * 32 < p.M;   // of a few rows most of the products would be of none: 64 x 5632 x 1024, 33 -> 25 us
-    f32x16_t acc[2] = {};
+    f32x4_t acc[2][kAcross] = {};
     load(k0);
     pa.store(as[0]);
     pb.store(bs[0]);
@@ -90,11 +135,18 @@ __global__ void __launch_bounds__(512) product_kernel(ProductParams p) {
         if (more) load(k + kStep);
         if (there)
 #pragma unroll
-        for (int s = 0; s < kStep; s += 2) {
-            const float av = as[at][s + half][wm * 32 + l];
+        for (int h = 0; h < 2; h++) {
+            f32x4_t av[2], bv[kAcross];
 #pragma unroll
-            for (int j = 0; j < 2; j++)
-                acc[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(av, bs[at][s + half][kGated ? j * 64 + wn * 32 + l : wn * 64 + j * 32 + l], acc[j], 0, 0, 0);
+            for (int i = 0; i < 2; i++) av[i] = as[at].read(wm * 32 + i * 16 + l, h * 4 + quarter);
+#pragma unroll
+            for (int j = 0; j < kAcross; j++) bv[j] = bs[at].read(column(j) + l, h * 4 + quarter);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+                for (int j = 0; j < kAcross; j++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(av[i][e], bv[j][e], acc[i][j], 0, 0, 0);
         }
         if (more) {
             pa.store(as[at ^ 1]);
@@ -103,35 +155,40 @@ __global__ void __launch_bounds__(512) product_kernel(ProductParams p) {
         __syncthreads();
         at ^= 1;
     }
-    // element r of an accumulator: row 8 (r / 4) + 4 half + r % 4, column l
+    // element r of a sum: row 4 quarter + r, column l
 #pragma unroll
-    for (int r = 0; r < 16; r++) {
-        const int row = wm * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
-        const int64_t m = m0 + row;
-        if (sums) {
+    for (int i = 0; i < 2; i++)
 #pragma unroll
-            for (int j = 0; j < 2; j++) sums[row * kTile + (kGated ? j * 64 + wn * 32 : wn * 64 + j * 32) + l] = acc[j][r];
-            continue;
-        }
-        if (m >= p.M) continue;
-        if constexpr (kGated) {
-            const int64_t n = n0 + wn * 32 + l;
-            if (n >= inter) continue;
-            const float g = acc[0][r], u = acc[1][r];
-            ((T*)p.out)[m * inter + n] = Elem<T>::from_float(gate_product(g, u));
-            if (p.both) {
-                T* to = (T*)p.both + m * p.N + n;
-                to[0] = Elem<T>::from_float(g);
-                to[inter] = Elem<T>::from_float(u);
+        for (int r = 0; r < 4; r++) {
+            const int row = wm * 32 + i * 16 + 4 * quarter + r;
+            const int64_t m = m0 + row;
+            if (sums) {
+#pragma unroll
+                for (int j = 0; j < kAcross; j++) sums[row * kTile + column(j) + l] = acc[i][j][r];
+                continue;
             }
-        } else {
+            if (m >= p.M) continue;
+            if constexpr (kGated) {
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const int64_t n = n0 + wn * 64 + j * 32 + l;
-                if (n < p.N) ((T*)p.out)[m * p.N + n] = Elem<T>::from_float(acc[j][r]);
+                for (int j = 0; j < kAcross / 2; j++) {
+                    const int64_t n = n0 + column(j) + l;
+                    if (n >= inter) continue;
+                    const float g = acc[i][j][r], u = acc[i][j + kAcross / 2][r];
+                    ((T*)p.out)[m * inter + n] = Elem<T>::from_float(gate_product(g, u));
+                    if (p.both) {
+                        T* to = (T*)p.both + m * p.N + n;
+                        to[0] = Elem<T>::from_float(g);
+                        to[inter] = Elem<T>::from_float(u);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < kAcross; j++) {
+                    const int64_t n = n0 + column(j) + l;
+                    if (n < p.N) ((T*)p.out)[m * p.N + n] = Elem<T>::from_float(acc[i][j][r]);
+                }
             }
         }
-    }
 }
 
 // Sums of the shares of a tile, in their order, and what the product's own epilogue does.  A workgroup has some rows of a tile, a thread four
@@ -232,30 +289,46 @@ bool fits_tiles(const ProductParams& p, bool along_a, bool along_b, bool gated) 
            ((reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.both)) & 15) == 0;
 }
 
-// Where the tiles of float32 products leave compute units idle, the steps are shared out over as many workgroups as come to one each, none with
-// fewer than 128.
-TilePlan plan_float(int64_t M, int64_t N, int64_t K, int cus) {
-    TilePlan r;
-    r.tile_m = r.tile_n = kTile;
-    r.stages = 2;
-    r.tiles_m = (int)((M + kTile - 1) / kTile);
-    r.tiles_n = (int)((N + kTile - 1) / kTile);
-    const int64_t tiles = (int64_t)r.tiles_m * r.tiles_n;
-    const int64_t shares = std::max<int64_t>(1, std::min<int64_t>(cus / tiles, K / 128));
-    r.k_share = ((K + shares - 1) / shares + kStep - 1) / kStep * kStep;
-    r.shares = (int)((K + r.k_share - 1) / r.k_share);
-    r.whole_tiles = r.shares > 1 ? 0 : (int)std::min<int64_t>(tiles, 0x7fffffff);
-    return r;
-}
-
 // Columns of B's tiles are gate and up columns by halves, so there may be tiles with few of either.
 int64_t tiled_columns(int64_t N, bool gated, int tile_n) {
     return gated ? (N / 2 + tile_n / 2 - 1) / (tile_n / 2) * tile_n : N;
 }
 
+// Tiles of float32 products and the shares of their steps, by the time they are estimated to take: of the compute unit that has the most of them,
+// 32 steps of r tiles at a time 0.4 + 1.95 r us of 128 x 128, two at a time, and 1.1 + 0.35 r of 64 x 64, four at a time (one has the
+// unit wait for its loads); and of adding shares up 3 us, 0.25 a share and 2.5 MB/us.  509 x 5462 x 1023 in tiles of 64 and 128: 79 and 87 us;
+// 2048 x 16384 x 4096: 2531 and 2209; 509 x 1023 x 5462 by 16 shares: 87 and 79, by one: 274 and 528.
+TilePlan plan_float(int64_t M, int64_t N, int64_t K, bool gated, int cus) {
+    TilePlan best;
+    double least = 0;
+    for (int tile : {128, 64}) {
+        const int64_t at_a_time = tile == 128 ? 2 : 4;
+        auto time_of = [&](int64_t r) { return r == 0 ? 0. : tile == 128 ? 0.4 + 1.95 * r : 1.1 + 0.35 * r; };
+        TilePlan r;
+        r.tile_m = r.tile_n = tile;
+        r.stages = 2;
+        r.tiles_m = (int)((M + tile - 1) / tile);
+        r.tiles_n = (int)((tiled_columns(N, gated, tile) + tile - 1) / tile);
+        const int64_t tiles = (int64_t)r.tiles_m * r.tiles_n;
+        const int64_t most = std::max<int64_t>(1, std::min<int64_t>(K / 128, at_a_time * cus / tiles + 1));
+        for (int64_t shares = 1; shares <= most; shares++) {
+            r.k_share = ((K + shares - 1) / shares + kStep - 1) / kStep * kStep;
+            r.shares = (int)((K + r.k_share - 1) / r.k_share);
+            r.whole_tiles = r.shares > 1 ? 0 : (int)std::min<int64_t>(tiles, 0x7fffffff);
+            const int64_t each = (tiles * r.shares + cus - 1) / cus;
+            const double time = (r.k_share / kStep) * ((each / at_a_time) * time_of(at_a_time) + time_of(each % at_a_time)) + (r.shares > 1 ? 3 + 0.25 * r.shares + r.bytes() / 2.5e6 : 0);
+            if (least == 0 || time < least) {
+                least = time;
+                best = r;
+            }
+        }
+    }
+    return best;
+}
+
 // Scratch of a product, whichever kernel takes it.
 int64_t product_bytes(int64_t M, int64_t N, int64_t K, bool a_along_k, bool gated, int cus) {
-    return std::max(plan_tiles(M, tiled_columns(N, gated, 128), K, a_along_k, cus).bytes(), plan_float(M, tiled_columns(N, gated, kTile), K, cus).bytes());
+    return std::max(plan_tiles(M, tiled_columns(N, gated, 128), K, a_along_k, cus).bytes(), plan_float(M, N, K, gated, cus).bytes());
 }
 
 template <typename T, bool kAlongKA, bool kAlongKB, Epilogue kEpilogue>
@@ -263,7 +336,7 @@ int run_product(ProductParams& p, const DeviceInfo& di, void* workspace, int64_t
     constexpr bool kGated = kEpilogue == kGate;
     const bool tiles = fits_tiles<T>(p, kAlongKA, kAlongKB, kGated);
     const TilePlan plan = tiles ? plan_tiles(p.M, tiled_columns(p.N, kGated, 128), p.K, kAlongKA, di.cus)
-                                : plan_float(p.M, tiled_columns(p.N, kGated, kTile), p.K, di.cus);
+                                : plan_float(p.M, p.N, p.K, kGated, di.cus);
     if (plan.bytes() && (!workspace || plan.bytes() > bytes || reinterpret_cast<uintptr_t>(workspace) & 15)) return CKV_ERR_WORKSPACE;
     if ((int64_t)plan.tiles_m * plan.tiles_n > 0x3fffffff || plan.blocks() > 0x7fffffff) return CKV_ERR_UNSUPPORTED;
     plan.fill(p);
@@ -272,7 +345,9 @@ int run_product(ProductParams& p, const DeviceInfo& di, void* workspace, int64_t
         if constexpr (sizeof(T) == 2)
             if (int rc = run_tiles<T>(p, plan, kAlongKA, kEpilogue, stream)) return rc;
     } else {
-        hipLaunchKernelGGL((product_kernel<T, kAlongKA, kAlongKB, kEpilogue>), dim3((unsigned)plan.blocks()), dim3(512), 0, stream, p);
+        if (plan.tile_m == 128)
+            hipLaunchKernelGGL((product_kernel<T, kAlongKA, kAlongKB, kEpilogue, 128>), dim3((unsigned)plan.blocks()), dim3(kThreads<128>), 0, stream, p);
+        else hipLaunchKernelGGL((product_kernel<T, kAlongKA, kAlongKB, kEpilogue, 64>), dim3((unsigned)plan.blocks()), dim3(kThreads<64>), 0, stream, p);
         CKV_HIP_TRY(hipGetLastError());
     }
     if (plan.shares > 1) {

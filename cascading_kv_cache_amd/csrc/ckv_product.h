@@ -5,7 +5,7 @@
 
 namespace ckv {
 
-typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 struct Operand {
     const void* p;
