@@ -289,11 +289,6 @@ bool fits_tiles(const ProductParams& p, bool along_a, bool along_b, bool gated) 
            ((reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.both)) & 15) == 0;
 }
 
-// Columns of B's tiles are gate and up columns by halves, so there may be tiles with few of either.
-int64_t tiled_columns(int64_t N, bool gated, int tile_n) {
-    return gated ? (N / 2 + tile_n / 2 - 1) / (tile_n / 2) * tile_n : N;
-}
-
 // Tiles of float32 products and the shares of their steps, by the time they are estimated to take: of the compute unit that has the most of them,
 // 32 steps of r tiles at a time 0.4 + 1.95 r us of 128 x 128, two at a time, and 1.1 + 0.35 r of 64 x 64, four at a time (one has the
 // unit wait for its loads); and of adding shares up 3 us, 0.25 a share and 2.5 MB/us.  509 x 5462 x 1023 in tiles of 64 and 128: 79 and 87 us;
@@ -308,7 +303,7 @@ TilePlan plan_float(int64_t M, int64_t N, int64_t K, bool gated, int cus) {
         r.tile_m = r.tile_n = tile;
         r.stages = 2;
         r.tiles_m = (int)((M + tile - 1) / tile);
-        r.tiles_n = (int)((tiled_columns(N, gated, tile) + tile - 1) / tile);
+        r.tiles_n = (int)tiles_across(N, tile, gated);
         const int64_t tiles = (int64_t)r.tiles_m * r.tiles_n;
         const int64_t most = std::max<int64_t>(1, std::min<int64_t>(K / 128, at_a_time * cus / tiles + 1));
         for (int64_t shares = 1; shares <= most; shares++) {
@@ -328,14 +323,14 @@ TilePlan plan_float(int64_t M, int64_t N, int64_t K, bool gated, int cus) {
 
 // Scratch of a product, whichever kernel takes it.
 int64_t product_bytes(int64_t M, int64_t N, int64_t K, bool a_along_k, bool gated, int cus) {
-    return std::max(plan_tiles(M, tiled_columns(N, gated, 128), K, a_along_k, cus).bytes(), plan_float(M, N, K, gated, cus).bytes());
+    return std::max(plan_tiles(M, N, K, a_along_k, gated, cus).bytes(), plan_float(M, N, K, gated, cus).bytes());
 }
 
 template <typename T, bool kAlongKA, bool kAlongKB, Epilogue kEpilogue>
 int run_product(ProductParams& p, const DeviceInfo& di, void* workspace, int64_t bytes, hipStream_t stream) {
     constexpr bool kGated = kEpilogue == kGate;
     const bool tiles = fits_tiles<T>(p, kAlongKA, kAlongKB, kGated);
-    const TilePlan plan = tiles ? plan_tiles(p.M, tiled_columns(p.N, kGated, 128), p.K, kAlongKA, di.cus)
+    const TilePlan plan = tiles ? plan_tiles(p.M, p.N, p.K, kAlongKA, kGated, di.cus)
                                 : plan_float(p.M, p.N, p.K, kGated, di.cus);
     if (plan.bytes() && (!workspace || plan.bytes() > bytes || reinterpret_cast<uintptr_t>(workspace) & 15)) return CKV_ERR_WORKSPACE;
     if ((int64_t)plan.tiles_m * plan.tiles_n > 0x3fffffff || plan.blocks() > 0x7fffffff) return CKV_ERR_UNSUPPORTED;

@@ -74,7 +74,9 @@ struct TilePlan {
         p.k_share = k_share;
     }
 };
-TilePlan plan_tiles(int64_t M, int64_t N, int64_t K, bool a_along_k, int cus);
+// Gated, a tile's columns are gate and up columns by halves, so there may be tiles with few of either.
+inline int64_t tiles_across(int64_t N, int tile_n, bool gated) { return gated ? (N / 2 + tile_n / 2 - 1) / (tile_n / 2) : (N + tile_n - 1) / tile_n; }
+TilePlan plan_tiles(int64_t M, int64_t N, int64_t K, bool a_along_k, bool gated, int cus);
 template <typename T>
 int run_tiles(const ProductParams& p, const TilePlan& plan, bool a_along_k, Epilogue epilogue, hipStream_t stream);
 

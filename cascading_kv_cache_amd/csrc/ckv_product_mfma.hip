@@ -302,13 +302,12 @@ __global__ void __launch_bounds__(64 * kWavesM * kWavesN, kTileM == 256 || kStag
         for (int j = 0; j < kBlocks; j++)
             *reinterpret_cast<uint2*>(mine + r16 * kPitch + (16 * j + c4) * 2) = pack4<T>(value(j, 0), value(j, 1), value(j, 2), value(j, 3));
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        const int piece = lane % kPieces;
 #pragma unroll
-        for (int x = 0; x < 16 * kPieces / 64; x++) {
-            const int row = x * (64 / kPieces) + lane / kPieces;
+        for (int x = 0; x < (16 * kPieces + 63) / 64; x++) {
+            const int at = x * 64 + lane, row = at / kPieces, piece = at % kPieces;
             const int64_t m = mw + 16 * i + row, n = nw + 8 * piece;
-            const uint4 v = *reinterpret_cast<const uint4*>(mine + row * kPitch + piece * 16);
-            if (m < p.M && n < cols) *reinterpret_cast<uint4*>((T*)out + m * stride + first + n) = v;
+            if (row >= 16 || m >= p.M || n >= cols) continue;
+            *reinterpret_cast<uint4*>((T*)out + m * stride + first + n) = *reinterpret_cast<const uint4*>(mine + row * kPitch + piece * 16);
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     };
@@ -340,6 +339,8 @@ int launch_tiles(const ProductParams& p, const TilePlan& plan, hipStream_t strea
 template <typename T, bool kAlongKA, bool kAlongKB, Epilogue kEpilogue>
 int launch_tiles(const ProductParams& p, const TilePlan& plan, hipStream_t stream) {
     if (plan.tile_m == 256) return launch_tiles<T, 256, 256, 4, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
+    if constexpr (kEpilogue == kGate)
+        if (plan.tile_n == 192) return launch_tiles<T, 128, 192, 6, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
     if (plan.tile_m == 128 && plan.stages == 4) return launch_tiles<T, 128, 128, 4, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
     if constexpr (kAlongKA)
         return plan.tile_m == 128 ? launch_tiles<T, 128, 128, 8, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream)
@@ -352,20 +353,21 @@ struct Kind {
     int tile_m, tile_n, stages, resident;
     double stage_us, around_us, first_us;   // first_us: where others hide what is around the stages, once a launch
 };
-constexpr Kind kKinds[] = {{256, 256, 4, 1, 0.73, 8.5, 0}, {128, 128, 4, 2, 0.65, 1.0, 8.0}, {128, 128, 8, 1, 0.33, 4.0, 0}, {64, 128, 8, 1, 0.17, 3.0, 0}};
+constexpr Kind kKinds[] = {{256, 256, 4, 1, 0.73, 8.5, 0}, {128, 128, 4, 2, 0.65, 1.0, 8.0}, {128, 128, 8, 1, 0.33, 4.0, 0}, {64, 128, 8, 1, 0.17, 3.0, 0}, {128, 192, 6, 1, 0.43, 6.0, 0}};
 
 }  // namespace
 
 // Tiles fill the compute units round by round; those of the last round may be shared out along k, which costs their sums a trip to memory (4
 // TB/s both ways, 3 us the launch that adds them up).
-TilePlan plan_tiles(int64_t M, int64_t N, int64_t K, bool a_along_k, int cus) {
+TilePlan plan_tiles(int64_t M, int64_t N, int64_t K, bool a_along_k, bool gated, int cus) {
     TilePlan best = {};
     double best_us = 0;
     const double stages = (double)((K + kSteps - 1) / kSteps);
     for (const Kind& kind : kKinds) {
         const bool few = kind.stages > 4;   // rows, all of them in a tile: bound by the bytes of B, for which there are more stages
         if (few && (!a_along_k || M > kind.tile_m)) continue;
-        const int64_t tiles_m = (M + kind.tile_m - 1) / kind.tile_m, tiles_n = (N + kind.tile_n - 1) / kind.tile_n, all = tiles_m * tiles_n;
+        if (kind.tile_n == 192 && !gated) continue;
+        const int64_t tiles_m = (M + kind.tile_m - 1) / kind.tile_m, tiles_n = tiles_across(N, kind.tile_n, gated), all = tiles_m * tiles_n;
         const int64_t places = (int64_t)cus * kind.resident, rest = all % places;
         for (int shares = 1; shares <= 8; shares++) {
             // Behind full rounds of products compute units may idle: the others' clock rises (2048 x 37888 x 3584, 4.6 rounds: 457 us, 485 with the
