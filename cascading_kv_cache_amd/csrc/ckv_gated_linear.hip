@@ -301,7 +301,7 @@ TilePlan plan_float(int64_t M, int64_t N, int64_t K, bool gated, int cus) {
         auto time_of = [&](int64_t r) { return r == 0 ? 0. : tile == 128 ? 0.4 + 1.95 * r : 1.1 + 0.35 * r; };
         TilePlan r;
         r.tile_m = r.tile_n = tile;
-        r.stages = 2;
+        r.deep = 1;
         r.tiles_m = (int)((M + tile - 1) / tile);
         r.tiles_n = (int)tiles_across(N, tile, gated);
         const int64_t tiles = (int64_t)r.tiles_m * r.tiles_n;

@@ -59,7 +59,7 @@ __device__ inline float* work_of(const ProductParams& p, int tile_size, int& tm,
 // ---- 16-bit operands on the matrix instructions of their type, ckv_product_mfma.hip -------------------------------------------------------
 // Sizes and layouts it takes: whole pieces of 16 bytes everywhere (adjacent elements, strides, addresses; C's columns).
 struct TilePlan {
-    int tile_m, tile_n, stages;
+    int tile_m, tile_n, deep;   // deep: 64 steps a stage instead of 32
     int tiles_m, tiles_n, whole_tiles, shares;
     int64_t k_share;
     int64_t blocks() const { return whole_tiles + ((int64_t)tiles_m * tiles_n - whole_tiles) * shares; }

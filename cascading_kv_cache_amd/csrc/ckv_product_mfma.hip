@@ -6,6 +6,10 @@
 // them; one whose steps are adjacent along its rows lies as it is, and is turned on the way into registers (ds_read_b64_tr_b16).  Pieces of 16
 // bytes are permuted within a row as they are copied, so that an operand read meets every bank once.
 //
+// Few rows wait for the bytes of B: their stages have 64 steps, whose rows are whole lines of 128 bytes (77 x 28672 x 4096 by halves of lines 53 us,
+// 44 so: 5.3 TB/s).  Many are bound by the products: 4096 x 28672 x 4096 takes 720 us, 1.34 PFLOP/s, which is what the library's product alone,
+// without the gate, takes on the same card.
+//
 // A wavefront of the large tile has 128 x 128 of it: with 64 x 128 each (eight wavefronts) the reads and copies of LDS alone take as long as the
 // products (a stage of 64 steps: 1536 + 512 of 2048 cycles).  One wavefront on a SIMD hides nothing behind another, so reads of the next
 // operands and copies stand between the products, one at a time.
@@ -33,7 +37,7 @@ typedef short product_s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t product_u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kSteps = 32;   // of a stage, and of a matrix instruction
+constexpr int kSteps = 32;   // of a matrix instruction; a stage has kDeep times as many
 
 // Written as an instruction, its sum in place: what the compiler makes of the builtin gives a sum another register than it had, and moves it
 // back, where there are as many as a wavefront of the large tile has.  Whoever reads a sum other than by the next product waits (sums_done).
@@ -64,15 +68,20 @@ __device__ uint4 g_zeros[1];
 // Which bits of the number of a piece step k flips: a read that turns 8 steps (k..k+3 and k+8..k+11) of 16 rows meets every bank once.
 __device__ inline int turned_bits(int k) { return ((k & 3) << 2) | ((k >> 2) & 2); }
 
-// The same where rows lie along k: which of its four pieces stands first in row r.  A read of 16 bytes a lane goes in four parts, of lanes 0-3,
-// 12-15, 20-23 and 24-27 the first, of 4-11, 16-19 and 28-31 the second: rows 4 q.. of piece 0 for two q, of piece 1 for the two others.
-__device__ inline int first_piece(int r) { return ((r >> 2 << 1) ^ ((r >> 3 & 1) * 3)) & 3; }
+// The same where rows lie along k, of kPieces pieces: which bits of the number of a piece row r flips.  A read of 16 bytes a lane goes in four
+// parts, of lanes 0-3, 12-15, 20-23 and 24-27 the first, of 4-11, 16-19 and 28-31 the second: rows 4 q.. of piece 0 for two q, of piece 1 for the
+// two others.
+template <int kPieces>
+__device__ inline int first_piece(int r) {
+    return kPieces == 4 ? ((r >> 2 << 1) ^ ((r >> 3 & 1) * 3)) & 3 : (r >> 1) & 7;
+}
 
 // One operand of a tile kRows rows high: copies of a wavefront, and where the lanes' pieces come from.
-template <int kRows, bool kAlongK, int kWaves>
+template <int kRows, bool kAlongK, int kWaves, int kDeep>
 struct Side {
-    static constexpr int kCopies = kRows * kSteps / 512 / kWaves;   // of 1 KiB a wavefront and stage
-    static constexpr int kBytes = kRows * kSteps * 2;
+    static constexpr int kStageSteps = kSteps * kDeep, kPieces = kStageSteps / 8;   // of a row along k
+    static constexpr int kCopies = kRows * kStageSteps / 512 / kWaves;   // of 1 KiB a wavefront and stage
+    static constexpr int kBytes = kRows * kStageSteps * 2;
     const char* at;              // uniform: of the next stage to be copied
     int64_t advance;             // bytes a stage
     uint32_t voff[kCopies];
@@ -84,14 +93,14 @@ struct Side {
         static_assert(!kGated || (kAlongK && kWaves % 2 == 0), "a wavefront's copies are all gate or all up rows");
         const int64_t row_bytes = 2 * o.stride;
         const bool up = kGated && wave >= kWaves / 2;
-        advance = kAlongK ? 2 * kSteps : kSteps * row_bytes;
+        advance = kAlongK ? 2 * kStageSteps : kStageSteps * row_bytes;
         at = kAlongK ? (const char*)o.p + ((up ? rows : 0) + first) * row_bytes + 2 * k0 : (const char*)o.p + k0 * row_bytes + 2 * first;
 #pragma unroll
         for (int c = 0; c < kCopies; c++) {
             const int copy = wave * kCopies + c;
             if constexpr (kAlongK) {
-                const int row = 16 * copy + (lane >> 2), in_half = row - (up ? kRows / 2 : 0);
-                const int piece = (lane & 3) ^ first_piece(row);
+                const int row = 64 / kPieces * copy + lane / kPieces, in_half = row - (up ? kRows / 2 : 0);
+                const int piece = lane % kPieces ^ first_piece<kPieces>(row);
                 const int64_t left = rows - first - 1;
                 voff[c] = (uint32_t)(min((int64_t)in_half, left) * row_bytes) + 16 * piece;
             } else {
@@ -108,22 +117,23 @@ struct Side {
     // a stage of which only `left` steps are there
     __device__ void copy_some(int c, uint32_t lds, int left, int wave, int lane) const {
         const int copy = wave * kCopies + c;
-        const int step = kAlongK ? 8 * ((lane & 3) ^ first_piece(16 * copy + (lane >> 2))) : copy * (512 / kRows) + lane / (kRows / 8);
+        const int step = kAlongK ? 8 * (lane % kPieces ^ first_piece<kPieces>(64 / kPieces * copy + lane / kPieces)) : copy * (512 / kRows) + lane / (kRows / 8);
         async_copy16_from(step < left ? (const void*)(at + voff[c]) : (const void*)g_zeros, lds + c * 1024);
     }
 };
 
 // Operands of kFrags blocks of 16 rows.  Element e of a lane: row lane % 16 of the block, step 8 (lane / 16) + e.  A read's address is a
 // register and a constant: with an addition in front of every one the products of the large tile waited for their turn to be issued.
-template <int kRows, bool kAlongK, int kFrags, int kStage, int kStages>
+template <int kRows, bool kAlongK, int kFrags, int kStage, int kStages, int kDeep>
 struct Reader {
-    static constexpr int kReach = kStages / 2;   // stages that a read's constant reaches over, 64 KiB
-    uint32_t at[2][kAlongK ? 1 : kFrags];
+    static constexpr int kReach = std::min((kStages + 1) / 2, 65536 / kStage), kBases = (kStages + kReach - 1) / kReach;   // stages that a constant of 16 bits reaches over
+    static constexpr int kRowBytes = kSteps * kDeep * 2;   // along k
+    uint32_t at[kBases][kAlongK ? kDeep : kFrags];
     __device__ void init(uint32_t lds, int first, int lane) {
-        static_assert(kReach * kStage <= 65536 && kStages % 2 == 0, "of 16 bits");
         const int r = lane & 15, g = lane >> 4;
         if constexpr (kAlongK) {
-            at[0][0] = lds + (first + r) * (kSteps * 2) + ((g ^ first_piece(r)) << 4);
+#pragma unroll
+            for (int d = 0; d < kDeep; d++) at[0][d] = lds + (first + r) * kRowBytes + ((4 * d + g) ^ first_piece<4 * kDeep>(r)) * 16;
         } else {
             const int k = 8 * g + (r >> 2);   // and four further
 #pragma unroll
@@ -133,37 +143,42 @@ struct Reader {
             }
         }
 #pragma unroll
-        for (int f = 0; f < (kAlongK ? 1 : kFrags); f++) {
-            at[1][f] = at[0][f] + kReach * kStage;
-            asm("" : "+v"(at[0][f]), "+v"(at[1][f]));   // kept, not worked out again
+        for (int f = 0; f < (kAlongK ? kDeep : kFrags); f++) {
+            asm("" : "+v"(at[0][f]));
+#pragma unroll
+            for (int b = 1; b < kBases; b++) {
+                at[b][f] = at[0][f] + b * kReach * kStage;
+                asm("" : "+v"(at[b][f]));   // kept, not worked out again
+            }
         }
     }
-    // `jump`: bytes that the block lies further than 16 rows a block would put it
-    __device__ uint4 read(int stage, int f, int jump) const {
-        const int to = stage % kReach * kStage;
+    // unit: which 32 steps of the stages.  `jump`: bytes that the block lies further than 16 rows a block would put it
+    __device__ uint4 read(int unit, int f, int jump) const {
+        const int stage = unit / kDeep, d = unit % kDeep, to = stage % kReach * kStage;
         if constexpr (kAlongK) {
-            const product_u32x4 v = *(const __attribute__((address_space(3))) product_u32x4*)(uintptr_t)(at[stage / kReach][0] + (to + f * 16 * (kSteps * 2) + jump));
+            const product_u32x4 v = *(const __attribute__((address_space(3))) product_u32x4*)(uintptr_t)(at[stage / kReach][d] + (to + f * 16 * kRowBytes + jump));
             return make_uint4(v[0], v[1], v[2], v[3]);
         } else {
             uint2 u[2];
 #pragma unroll
             for (int a = 0; a < 2; a++)
                 u[a] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) product_s16x4*)(uintptr_t)(
-                                                     at[stage / kReach][f] + (to + 4 * a * (kRows * 2)))));
+                                                     at[stage / kReach][f] + (to + (d * kSteps + 4 * a) * (kRows * 2)))));
             return make_uint4(u[0].x, u[0].y, u[1].x, u[1].y);
         }
     }
 };
 
-template <int kTileM, int kTileN>
-constexpr int kStageBytes = (kTileM + kTileN) * kSteps * 2;
+template <int kTileM, int kTileN, int kDeep>
+constexpr int kStageBytes = (kTileM + kTileN) * kSteps * kDeep * 2;
 
-template <typename T, int kTileM, int kTileN, int kWavesM, int kWavesN, int kStages, bool kAlongKA, bool kAlongKB, Epilogue kEpilogue>
-__global__ void __launch_bounds__(64 * kWavesM * kWavesN, kTileM == 256 || kStages > 4 ? 1 : 2) tile_kernel(ProductParams p) {
+template <typename T, int kTileM, int kTileN, int kWavesM, int kWavesN, int kStages, int kDeep, bool kAlongKA, bool kAlongKB, Epilogue kEpilogue>
+__global__ void __launch_bounds__(64 * kWavesM * kWavesN, kTileM == 256 || kDeep > 1 ? 1 : 2) tile_kernel(ProductParams p) {
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr bool kGated = kEpilogue == kGate;
     constexpr int kWaves = kWavesM * kWavesN, kFragsM = kTileM / kWavesM / 16, kFragsN = kTileN / kWavesN / 16;
-    constexpr int kStage = kStageBytes<kTileM, kTileN>;
+    constexpr int kStage = kStageBytes<kTileM, kTileN, kDeep>, kStageSteps = kSteps * kDeep, kUnits = kStages * kDeep;
+    static_assert(kUnits % 2 == 0, "of operands in registers, which two take turns for");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / kWavesN, wn = wave % kWavesN;
     int tm, tn, share;
     float* sums = work_of<4>(p, kTileM * kTileN, tm, tn, share);
@@ -172,20 +187,21 @@ __global__ void __launch_bounds__(64 * kWavesM * kWavesN, kTileM == 256 || kStag
     const int64_t k0 = share * p.k_share, steps = sums ? min(p.K - k0, p.k_share) : p.K;
     const uint32_t lds = lds_address(smem);
 
-    using SideA = Side<kTileM, kAlongKA, kWaves>;
-    using SideB = Side<kTileN, kAlongKB, kWaves>;
+    using SideA = Side<kTileM, kAlongKA, kWaves, kDeep>;
+    using SideB = Side<kTileN, kAlongKB, kWaves, kDeep>;
     SideA a;
     SideB b;
     a.template init<false>(p.a, m0, p.M, k0, wave, lane);
     b.template init<kGated>(p.b, n0, cols, k0, wave, lane);
-    Reader<kTileM, kAlongKA, kFragsM, kStage, kStages> ra;
-    Reader<kTileN, kAlongKB, kFragsN, kStage, kStages> rb;
+    Reader<kTileM, kAlongKA, kFragsM, kStage, kStages, kDeep> ra;
+    Reader<kTileN, kAlongKB, kFragsN, kStage, kStages, kDeep> rb;
     ra.init(lds, wm * (kTileM / kWavesM), lane);
     rb.init(lds + SideA::kBytes, kGated ? wn * (kTileN / kWavesN / 2) : wn * (kTileN / kWavesN), lane);
     // with the gate, a wavefront's second half of blocks are the up columns of its first
-    constexpr int kJump = kGated ? (kTileN / 2 - kTileN / kWavesN / 2) * kSteps * 2 : 0;
+    constexpr int kJump = kGated ? (kTileN / 2 - kTileN / kWavesN / 2) * kStageSteps * 2 : 0;
 
-    const int whole = (int)(steps / (kStages * kSteps)) * kStages, left = (int)(steps % (kStages * kSteps));   // stages; steps behind them
+    // Stages that go through the pipeline, and steps behind them: all, where those are no more than are copied in one go.
+    const int whole = steps < kStages * kStageSteps ? 0 : (int)(steps / kStageSteps), left = (int)(steps - (int64_t)whole * kStageSteps);
     constexpr int kCopiesA = SideA::kCopies, kCopies = kCopiesA + SideB::kCopies;
     const uint32_t mine_a = lds + wave * (kCopiesA * 1024), mine_b = lds + SideA::kBytes + wave * (SideB::kCopies * 1024);
     auto copy = [&](int c, uint32_t stage_at) {
@@ -195,7 +211,7 @@ __global__ void __launch_bounds__(64 * kWavesM * kWavesN, kTileM == 256 || kStag
     // The stage that is copied next.  Behind the last whole one comes the first again (to nobody's use, where that is where it began).  Few rows
     // wait for the bytes of B, and workgroups that go through its rows side by side ask for the same few channels of memory at a time: they begin
     // in different places (32 x 28672 x 4096: 62.7 -> 55.2 us.  Where B's steps are its rows, which they share, not: 58 -> 67).
-    int ahead = kStages > 4 && kAlongKB && whole > 0 ? (int)((blockIdx.x * 2654435761u >> 8) % (uint32_t)whole) : 0;
+    int ahead = kDeep > 1 && kAlongKB && whole > 0 ? (int)((blockIdx.x * 2654435761u >> 8) % (uint32_t)whole) : 0;
     const int64_t back_a = (1 - whole) * a.advance, back_b = (1 - whole) * b.advance;
     a.at += ahead * a.advance;
     b.at += ahead * b.advance;
@@ -209,27 +225,29 @@ __global__ void __launch_bounds__(64 * kWavesM * kWavesN, kTileM == 256 || kStag
     asm volatile("s_nop 7" ::: "memory");
     uint4 av[2][kFragsM], bv[2][kFragsN];
     constexpr int kReads = kFragsM + kFragsN, kProducts = kFragsM * kFragsN;
-    auto read = [&](int n, int buf, int stage) {   // in the order in which the products want them
-        if (n == 0) bv[buf][0] = rb.read(stage, 0, 0);
-        else if (n <= kFragsM) av[buf][n - 1] = ra.read(stage, n - 1, 0);
-        else bv[buf][n - kFragsM] = rb.read(stage, n - kFragsM, n - kFragsM >= kFragsN / 2 ? kJump : 0);
+    auto read = [&](int n, int buf, int unit) {   // in the order in which the products want them
+        if (n == 0) bv[buf][0] = rb.read(unit, 0, 0);
+        else if (n <= kFragsM) av[buf][n - 1] = ra.read(unit, n - 1, 0);
+        else bv[buf][n - kFragsM] = rb.read(unit, n - kFragsM, n - kFragsM >= kFragsN / 2 ? kJump : 0);
     };
-    // The products of the stage whose operands are in registers, and between them the next one's operands and copies to its own place.
-    auto step = [&](auto stage_) {
-        constexpr int stage = decltype(stage_)::value, next_stage = (stage + 1) % kStages;
+    // The products of the 32 steps whose operands are in registers, and between them the next ones' operands and, of the last of a stage, copies to
+    // its place.
+    auto step = [&](auto unit_) {
+        constexpr int unit = decltype(unit_)::value, next_unit = (unit + 1) % kUnits;
+        constexpr bool last = unit % kDeep == kDeep - 1;
         each<kProducts>([&](auto n_) {
             constexpr int n = decltype(n_)::value, j = n / kFragsM, i = n % kFragsM;
-            mma<T>(bv[stage % 2][j], av[stage % 2][i], acc[i][j]);
+            mma<T>(bv[unit % 2][j], av[unit % 2][i], acc[i][j]);
             constexpr int kEarly = kProducts * 3 / 4;
             if constexpr (n < kEarly) {
                 constexpr int first = n * kReads / kEarly, end = (n + 1) * kReads / kEarly;
-                each<end - first>([&](auto x) { read(first + decltype(x)::value, next_stage % 2, next_stage); });
+                each<end - first>([&](auto x) { read(first + decltype(x)::value, next_unit % 2, next_unit); });
             }
-            constexpr int from = n * kCopies / kProducts, to = (n + 1) * kCopies / kProducts;
-            each<to - from>([&](auto x) { copy(from + decltype(x)::value, stage * kStage); });
+            constexpr int from = n * kCopies / kProducts, to = last ? (n + 1) * kCopies / kProducts : from;
+            each<to - from>([&](auto x) { copy(from + decltype(x)::value, unit / kDeep * kStage); });
             __builtin_amdgcn_sched_barrier(0);
         });
-        next();
+        if constexpr (last) next();
     };
     if (whole > 0) {
         each<kStages>([&](auto st) {
@@ -240,28 +258,31 @@ __global__ void __launch_bounds__(64 * kWavesM * kWavesN, kTileM == 256 || kStag
         __syncthreads();
         each<kReads>([&](auto n) { read(decltype(n)::value, 0, 0); });
         for (int stage = 0; stage < whole; stage += kStages)
-            each<kStages>([&](auto st) {
-                // Everybody has this stage's operands in registers, so it may be copied over, and the next one is there.
+            each<kUnits>([&](auto unit) {
+                constexpr int u = decltype(unit)::value;
+                if (stage + u / kDeep >= whole) return;
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                wait_copies<(kStages - 2) * kCopies>();
-                __builtin_amdgcn_s_barrier();
-                asm volatile("" ::: "memory");
-                step(st);
+                if constexpr (u % kDeep == kDeep - 1) {   // everybody has the last of this stage in registers, so it may be copied over, and the next one is there
+                    wait_copies<(kStages - 2) * kCopies>();
+                    __builtin_amdgcn_s_barrier();
+                    asm volatile("" ::: "memory");
+                }
+                step(unit);
             });
         sums_done(acc);
         wait_copies<0>();
         __syncthreads();
     }
-    if (left) {   // last stages, one of which may not be whole
+    if (left) {   // stages of which the last may not be whole
         a.at += (whole - ahead) * a.advance;
         b.at += (whole - ahead) * b.advance;
 #pragma unroll
         for (int st = 0; st < kStages; st++) {
-            if (st * kSteps < left) {
+            if (st * kStageSteps < left) {
 #pragma unroll
                 for (int c = 0; c < kCopies; c++)
-                    if (c < kCopiesA) a.copy_some(c, mine_a + st * kStage, left - st * kSteps, wave, lane);
-                    else b.copy_some(c - kCopiesA, mine_b + st * kStage, left - st * kSteps, wave, lane);
+                    if (c < kCopiesA) a.copy_some(c, mine_a + st * kStage, left - st * kStageSteps, wave, lane);
+                    else b.copy_some(c - kCopiesA, mine_b + st * kStage, left - st * kStageSteps, wave, lane);
                 a.at += a.advance;
                 b.at += b.advance;
             }
@@ -269,10 +290,10 @@ __global__ void __launch_bounds__(64 * kWavesM * kWavesN, kTileM == 256 || kStag
         wait_copies<0>();
         __syncthreads();
 #pragma unroll
-        for (int st = 0; st < kStages; st++) {
-            if (st * kSteps < left) {
+        for (int u = 0; u < kUnits; u++) {
+            if (u * kSteps < left) {
 #pragma unroll
-                for (int n = 0; n < kReads; n++) read(n, 0, st);
+                for (int n = 0; n < kReads; n++) read(n, 0, u);
 #pragma unroll
                 for (int n = 0; n < kProducts; n++) mma<T>(bv[0][n / kFragsM], av[0][n % kFragsM], acc[n % kFragsM][n / kFragsM]);
             }
@@ -326,10 +347,10 @@ __global__ void __launch_bounds__(64 * kWavesM * kWavesN, kTileM == 256 || kStag
     }
 }
 
-template <typename T, int kTileM, int kTileN, int kStages, bool kAlongKA, bool kAlongKB, Epilogue kEpilogue>
+template <typename T, int kTileM, int kTileN, int kStages, int kDeep, bool kAlongKA, bool kAlongKB, Epilogue kEpilogue>
 int launch_tiles(const ProductParams& p, const TilePlan& plan, hipStream_t stream) {
-    auto kernel = tile_kernel<T, kTileM, kTileN, 2, 2, kStages, kAlongKA, kAlongKB, kEpilogue>;
-    constexpr int lds = kStages * kStageBytes<kTileM, kTileN>;
+    auto kernel = tile_kernel<T, kTileM, kTileN, 2, 2, kStages, kDeep, kAlongKA, kAlongKB, kEpilogue>;
+    constexpr int lds = kStages * kStageBytes<kTileM, kTileN, kDeep>;
     if (int rc = ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), lds)) return rc;
     hipLaunchKernelGGL(kernel, dim3((unsigned)plan.blocks()), dim3(256), lds, stream, p);
     CKV_HIP_TRY(hipGetLastError());
@@ -338,52 +359,63 @@ int launch_tiles(const ProductParams& p, const TilePlan& plan, hipStream_t strea
 
 template <typename T, bool kAlongKA, bool kAlongKB, Epilogue kEpilogue>
 int launch_tiles(const ProductParams& p, const TilePlan& plan, hipStream_t stream) {
-    if (plan.tile_m == 256) return launch_tiles<T, 256, 256, 4, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
-    if constexpr (kEpilogue == kGate)
-        if (plan.tile_n == 192) return launch_tiles<T, 128, 192, 6, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
-    if (plan.tile_m == 128 && plan.stages == 4) return launch_tiles<T, 128, 128, 4, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
+    if (plan.tile_m == 256) return launch_tiles<T, 256, 256, 4, 1, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
+    if (plan.deep == 1) return launch_tiles<T, 128, 128, 4, 1, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
+    if constexpr (kEpilogue == kGate) {
+        if (plan.tile_n == 192)
+            return plan.tile_m == 128 ? launch_tiles<T, 128, 192, 4, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream)
+                                      : launch_tiles<T, 64, 192, 5, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
+        if (plan.tile_n == 256)
+            return plan.tile_m == 128 ? launch_tiles<T, 128, 256, 3, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream)
+                                      : launch_tiles<T, 64, 256, 4, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
+    }
     if constexpr (kAlongKA)
-        return plan.tile_m == 128 ? launch_tiles<T, 128, 128, 8, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream)
-                                  : launch_tiles<T, 64, 128, 8, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
+        return plan.tile_m == 128 ? launch_tiles<T, 128, 128, 4, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream)
+                                  : launch_tiles<T, 64, 128, 6, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
     return CKV_ERR_UNSUPPORTED;
 }
 
-// A kind of tile, and microseconds that its workgroups take on a compute unit, `resident` of them at a time: a stage, and around the stages.
+// A kind of tile, and microseconds that its workgroups take on a compute unit, `resident` of them at a time: 32 steps, and around the steps.  Deep
+// kinds are for few rows, all of them in a tile, which wait for the bytes of B: 5.9 TB/s over all workgroups, and no less than `step_us`
+// (or 0.33 where B's rows lie across k: 32 x 4096 x 28672 58 us in eight shares, 82 in four).
 struct Kind {
-    int tile_m, tile_n, stages, resident;
-    double stage_us, around_us, first_us;   // first_us: where others hide what is around the stages, once a launch
+    int tile_m, tile_n, deep, resident;
+    double step_us, around_us, first_us;   // first_us: where others hide what is around the steps, once a launch
 };
-constexpr Kind kKinds[] = {{256, 256, 4, 1, 0.73, 8.5, 0}, {128, 128, 4, 2, 0.65, 1.0, 8.0}, {128, 128, 8, 1, 0.33, 4.0, 0}, {64, 128, 8, 1, 0.17, 3.0, 0}, {128, 192, 6, 1, 0.43, 6.0, 0}};
+constexpr Kind kKinds[] = {{256, 256, 1, 1, 0.73, 8.5, 0}, {128, 128, 1, 2, 0.65, 1.0, 8.0}, {128, 128, 2, 1, 0.18, 4.0, 0}, {64, 128, 2, 1, 0.12, 4.0, 0},
+                           {128, 192, 2, 1, 0.36, 5.0, 0}, {64, 192, 2, 1, 0.33, 5.0, 0},    {128, 256, 2, 1, 0.48, 6.0, 0}, {64, 256, 2, 1, 0.42, 6.0, 0}};
 
 }  // namespace
 
 // Tiles fill the compute units round by round; those of the last round may be shared out along k, which costs their sums a trip to memory (4
-// TB/s both ways, 3 us the launch that adds them up).
+// TB/s both ways, 3 us the launch that adds them up).  Of few rows the tiles are as wide as brings the columns nearest to full rounds, at 64 rows
+// (widths 128, 192 and 256): 28672 x 4096 44, 52 and 58 us, 37888 x 3584 60, 55 and 61, 51200 x 5120 more than 111, 107 and 103.
 TilePlan plan_tiles(int64_t M, int64_t N, int64_t K, bool a_along_k, bool gated, int cus) {
     TilePlan best = {};
     double best_us = 0;
-    const double stages = (double)((K + kSteps - 1) / kSteps);
     for (const Kind& kind : kKinds) {
-        const bool few = kind.stages > 4;   // rows, all of them in a tile: bound by the bytes of B, for which there are more stages
-        if (few && (!a_along_k || M > kind.tile_m)) continue;
-        if (kind.tile_n == 192 && !gated) continue;
+        const bool few = kind.deep > 1;
+        if (few && (!a_along_k || M > kind.tile_m || (kind.tile_n > 128 && !gated))) continue;
         const int64_t tiles_m = (M + kind.tile_m - 1) / kind.tile_m, tiles_n = tiles_across(N, kind.tile_n, gated), all = tiles_m * tiles_n;
         const int64_t places = (int64_t)cus * kind.resident, rest = all % places;
+        auto time_of = [&](int64_t workgroups, int64_t steps) {   // of that many at a time
+            const double bytes_us = few ? (double)std::min<int64_t>(workgroups, cus) * kind.tile_n * kSteps * 2 / 5.9e6 : 0;
+            return (double)steps / kSteps * std::max(few && !gated ? 0.33 : kind.step_us, bytes_us) + kind.around_us;
+        };
         for (int shares = 1; shares <= 8; shares++) {
             // Behind full rounds of products compute units may idle: the others' clock rises (2048 x 37888 x 3584, 4.6 rounds: 457 us, 485 with the
-            // rest in three shares), unless it is bytes they wait for (77 x 37888 x 3584, 1.2 rounds: 82 us, 69 in five).
+            // rest in three shares), unless it is bytes they wait for.
             if (shares > 1 && (rest == 0 || K / shares < 256 || (!few && all > places))) break;
-            const int64_t k_share = shares == 1 ? K : ((K + shares - 1) / shares + kSteps * kind.stages - 1) / (kSteps * kind.stages) * (kSteps * kind.stages);
-            const int real = (int)((K + k_share - 1) / k_share);
-            if (real != shares) continue;
+            const int64_t k_share = shares == 1 ? K : ((K + shares - 1) / shares + 63) / 64 * 64;
+            if ((K + k_share - 1) / k_share != shares) continue;
             double rounds = (double)((rest * shares + cus - 1) / cus);
             if (kind.resident > 1)   // they start as others end; one alone on a unit is the faster for it
                 rounds = rest * shares <= cus && all < places ? 0.55 : all > places ? (double)rest / places : std::max(1.0, (double)rest * shares / places);
-            double us = kind.first_us + (double)(all / places) * (stages * kind.stage_us + kind.around_us) + rounds * ((double)k_share / kSteps * kind.stage_us + kind.around_us);
+            double us = kind.first_us + (double)(all / places) * time_of(places, K) + rounds * time_of(rest * shares, k_share);
             if (shares > 1) us += 3.0 + (double)(rest * shares) * kind.tile_m * kind.tile_n * 8 / 4e6;
             if (best_us == 0 || us < best_us) {
                 best_us = us;
-                best = TilePlan{kind.tile_m, kind.tile_n, kind.stages, (int)tiles_m, (int)tiles_n, (int)(all - rest), shares, k_share};
+                best = TilePlan{kind.tile_m, kind.tile_n, kind.deep, (int)tiles_m, (int)tiles_n, (int)(all - rest), shares, k_share};
             }
         }
     }

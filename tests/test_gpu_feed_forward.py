@@ -75,6 +75,21 @@ def test_against_float64(size, dtype):
     close(dw, want["dw"], dtype, "dw")
 
 
+@pytest.mark.parametrize("dtype", TYPES[:2])
+@pytest.mark.parametrize("size", [(50, 328, 18952), (100, 328, 18952), (64, 64, 17000), (33, 1032, 25608), (128, 520, 25608), (64, 456, 31000)], ids=str)
+def test_few_rows_and_wide_layers(size, dtype):
+    """Columns that leave compute units idle, or are more than a round of them, in tiles of one width or another."""
+    x, w, dh = inputs(*size, dtype)
+    xs, ws = x.clone().requires_grad_(), w.clone().requires_grad_()
+    out = gated_feed_forward(xs, ws)
+    dx, dw = torch.autograd.grad(out, (xs, ws), dh)
+    want = exact(x, w, dtype, dh)
+    close(gated_feed_forward(x, w), want["out"], dtype, "output alone")
+    close(out.detach(), want["out"], dtype, "output")
+    close(dx, want["dx"], dtype, "dx")
+    close(dw, want["dw"], dtype, "dw")
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows", [1, 3, 40])
 def test_orders_and_alignment(rows, dtype):
