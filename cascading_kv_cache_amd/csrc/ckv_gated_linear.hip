@@ -176,9 +176,9 @@ __global__ void __launch_bounds__(kThreads<kTile>) product_kernel(ProductParams 
                     const float g = acc[i][j][r], u = acc[i][j + kAcross / 2][r];
                     ((T*)p.out)[m * inter + n] = Elem<T>::from_float(gate_product(g, u));
                     if (p.both) {
-                        T* to = (T*)p.both + m * p.N + n;
-                        to[0] = Elem<T>::from_float(g);
-                        to[inter] = Elem<T>::from_float(u);
+                        float* to = p.both + m * p.N + n;
+                        to[0] = g;
+                        to[inter] = u;
                     }
                 }
             } else {
@@ -224,9 +224,9 @@ __global__ void __launch_bounds__(256) merge_kernel(ProductParams p, int tile_m,
             if constexpr (kGated) {
                 ((T*)p.out)[m * cols + n + e] = Elem<T>::from_float(gate_product(g[e], u[e]));
                 if (p.both) {
-                    T* to = (T*)p.both + m * p.N + n + e;
-                    to[0] = Elem<T>::from_float(g[e]);
-                    to[cols] = Elem<T>::from_float(u[e]);
+                    float* to = p.both + m * p.N + n + e;
+                    to[0] = g[e];
+                    to[cols] = u[e];
                 }
             } else {
                 ((T*)p.out)[m * cols + n + e] = Elem<T>::from_float(g[e]);
@@ -237,22 +237,27 @@ __global__ void __launch_bounds__(256) merge_kernel(ProductParams p, int tile_m,
 
 // ---- gradients of the projections ------------------------------------------------------------------------------------------------------
 
+// dg and du are rounded to the tensor type, that of the operands of the two products behind: off by up to 2^-8 of each (2^-11 of float16), as
+// the products' own results are by their rounding.  The projections they are made from are float32.  Bound by memory: 12 bytes read and 4 written an element.
 template <typename T, int kPer>
-__global__ void __launch_bounds__(256) gate_gradient_kernel(const T* gate_up, const T* dout, T* grad, int64_t rows, int64_t inter) {
+__global__ void __launch_bounds__(256) gate_gradient_kernel(const float* gate_up, const T* dout, T* grad, int64_t rows, int64_t inter) {
     struct alignas(sizeof(T) * kPer) Piece {
         T v[kPer];
+    };
+    struct alignas(kPer > 1 ? 16 : 4) Wide {
+        float v[kPer];
     };
     const int64_t pieces = inter / kPer, all = rows * pieces;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
         int64_t c;
         const int64_t row = div_index(i, pieces, c);
-        const T* from = gate_up + row * 2 * inter + c * kPer;
-        const Piece gate = *reinterpret_cast<const Piece*>(from), up = *reinterpret_cast<const Piece*>(from + inter);
+        const float* from = gate_up + row * 2 * inter + c * kPer;
+        const Wide gate = *reinterpret_cast<const Wide*>(from), up = *reinterpret_cast<const Wide*>(from + inter);
         const Piece dh = *reinterpret_cast<const Piece*>(dout + row * inter + c * kPer);
         Piece dg, du;
 #pragma unroll
         for (int e = 0; e < kPer; e++) {
-            const float g = Elem<T>::to_float(gate.v[e]), u = Elem<T>::to_float(up.v[e]), d = Elem<T>::to_float(dh.v[e]);
+            const float g = gate.v[e], u = up.v[e], d = Elem<T>::to_float(dh.v[e]);
             const float s = 1.f / (1.f + expf(-g));
             dg.v[e] = Elem<T>::from_float(d * u * s * (1.f + g * (1.f - s)));
             du.v[e] = Elem<T>::from_float(d * g * s);
@@ -264,14 +269,14 @@ __global__ void __launch_bounds__(256) gate_gradient_kernel(const T* gate_up, co
 }
 
 template <typename T>
-int gate_gradient(const void* gate_up, const void* dout, void* grad, int64_t rows, int64_t inter, hipStream_t stream) {
+int gate_gradient(const float* gate_up, const void* dout, void* grad, int64_t rows, int64_t inter, hipStream_t stream) {
     constexpr int kPer = 16 / (int)sizeof(T);
     const bool pieces = inter % kPer == 0 &&
                         ((reinterpret_cast<uintptr_t>(gate_up) | reinterpret_cast<uintptr_t>(dout) | reinterpret_cast<uintptr_t>(grad)) & 15) == 0;
     const int64_t all = rows * inter / (pieces ? kPer : 1);
     const unsigned blocks = (unsigned)std::min<int64_t>((all + 255) / 256, 256 * 16);
-    if (pieces) hipLaunchKernelGGL((gate_gradient_kernel<T, kPer>), dim3(blocks), dim3(256), 0, stream, (const T*)gate_up, (const T*)dout, (T*)grad, rows, inter);
-    else hipLaunchKernelGGL((gate_gradient_kernel<T, 1>), dim3(blocks), dim3(256), 0, stream, (const T*)gate_up, (const T*)dout, (T*)grad, rows, inter);
+    if (pieces) hipLaunchKernelGGL((gate_gradient_kernel<T, kPer>), dim3(blocks), dim3(256), 0, stream, gate_up, (const T*)dout, (T*)grad, rows, inter);
+    else hipLaunchKernelGGL((gate_gradient_kernel<T, 1>), dim3(blocks), dim3(256), 0, stream, gate_up, (const T*)dout, (T*)grad, rows, inter);
     CKV_HIP_TRY(hipGetLastError());
     return CKV_OK;
 }
@@ -364,7 +369,7 @@ int check_sizes(int64_t rows, int64_t inter, int64_t k, int64_t x_stride, int32_
 }
 
 template <typename T>
-int run_forward(const void* x, const void* w, void* out, void* gate_up, int64_t rows, int64_t inter, int64_t k, int64_t x_stride, void* workspace,
+int run_forward(const void* x, const void* w, void* out, float* gate_up, int64_t rows, int64_t inter, int64_t k, int64_t x_stride, void* workspace,
                 int64_t bytes, const DeviceInfo& di, hipStream_t stream) {
     // A few rows wait for the weights, and the kernel of a decoding step's products streams them through LDS beside the rows (28672 x 4096, a
     // row: 39.3 us, tiles 52; twelve rows 43 and 53; sixteen, whose rows leave no room for the streams, 59 and 49; sixteen of 3584: 47 and 61).
@@ -385,7 +390,7 @@ int run_forward(const void* x, const void* w, void* out, void* gate_up, int64_t 
 }
 
 template <typename T>
-int run_backward(const void* x, const void* w, const void* gate_up, const void* dout, void* dx, void* dw, int64_t rows, int64_t inter, int64_t k,
+int run_backward(const void* x, const void* w, const float* gate_up, const void* dout, void* dx, void* dw, int64_t rows, int64_t inter, int64_t k,
                  int64_t x_stride, char* workspace, int64_t bytes, const DeviceInfo& di, hipStream_t stream) {
     const int64_t grad_bytes = align_up(rows * 2 * inter * (int64_t)sizeof(T), 256);
     void* grad = workspace;
@@ -430,7 +435,7 @@ extern "C" int64_t ckv_gated_linear_workspace_bytes(int64_t rows, int64_t inter,
     return product_bytes(rows, 2 * inter, k, true, true, di.cus);
 }
 
-extern "C" int ckv_gated_linear(const void* x, const void* w, void* out, void* gate_up, int64_t rows, int64_t inter, int64_t k, int64_t x_stride,
+extern "C" int ckv_gated_linear(const void* x, const void* w, void* out, float* gate_up, int64_t rows, int64_t inter, int64_t k, int64_t x_stride,
                                 int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream_) {
     using namespace ckv;
     if (int rc = check_sizes(rows, inter, k, x_stride, dtype)) return rc;
@@ -454,7 +459,7 @@ extern "C" int64_t ckv_gated_linear_bwd_workspace_bytes(int64_t rows, int64_t in
     return align_up(rows * 2 * inter * elem_bytes(dtype), 256) + std::max(dx, dw);
 }
 
-extern "C" int ckv_gated_linear_bwd(const void* x, const void* w, const void* gate_up, const void* dout, void* dx, void* dw, int64_t rows,
+extern "C" int ckv_gated_linear_bwd(const void* x, const void* w, const float* gate_up, const void* dout, void* dx, void* dw, int64_t rows,
                                     int64_t inter, int64_t k, int64_t x_stride, int32_t dtype, void* workspace, int64_t workspace_bytes,
                                     void* stream_) {
     using namespace ckv;

@@ -15,7 +15,7 @@ struct Operand {
 struct ProductParams {
     Operand a, b;
     void* out;          // (M, N) contiguous, or the gated (M, N / 2)
-    void* both;         // gated, optional: (M, N), gate and up columns
+    float* both;        // gated, optional: (M, N), gate and up columns; of these, not of numbers rounded to the operands' type, gradients are made
     float* partial;     // sums of the shares, tile by tile: (tiles shared out, shares, tile rows, tile columns)
     int64_t M, N, K;
     int64_t k_share;    // steps of a share

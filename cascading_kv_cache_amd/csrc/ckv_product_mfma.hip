@@ -337,8 +337,13 @@ __global__ void __launch_bounds__(64 * kWavesM * kWavesN, kTileM == 256 || kDeep
         if constexpr (kGated) {
             write(i, [&](int j, int r) { return gate_product(acc[i][j][r], acc[i][j + kBlocks][r]); }, p.out, cols, 0);
             if (p.both) {
-                write(i, [&](int j, int r) { return acc[i][j][r]; }, p.both, p.N, 0);
-                write(i, [&](int j, int r) { return acc[i][j + kBlocks][r]; }, p.both, p.N, cols);
+                const int64_t m = mw + 16 * i + r16;
+#pragma unroll
+                for (int j = 0; j < kFragsN; j++) {
+                    const int64_t n = nw + 16 * (j % kBlocks) + c4;
+                    if (m < p.M && n < cols)
+                        *reinterpret_cast<float4*>(p.both + m * p.N + (j < kBlocks ? 0 : cols) + n) = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
+                }
             }
         } else {
             write(i, [&](int j, int r) { return acc[i][j][r]; }, p.out, p.N, 0);

@@ -28,7 +28,7 @@ def _forward(x, w, both):
     inter = w.size(0) // 2
     lib, code = _abi.lib(), _abi.dtype_code(x.dtype)
     out = torch.empty(rows, inter, dtype=x.dtype, device=x.device)
-    gate_up = torch.empty(rows, 2 * inter, dtype=x.dtype, device=x.device) if both else None
+    gate_up = torch.empty(rows, 2 * inter, dtype=torch.float32, device=x.device) if both else None
     with on_device(x.device):
         ws = _scratch(lib.ckv_gated_linear_workspace_bytes(rows, inter, k, code), x.device)
         _abi.check(lib.ckv_gated_linear(_at(x), _at(w), _at(out), _at(gate_up), rows, inter, k, x.stride(0) if rows > 1 else k, code, _at(ws),
@@ -64,8 +64,8 @@ class _GatedFeedForward(torch.autograd.Function):
 
 def gated_feed_forward(x, w_gate_up):
     """``silu(gate) * up`` of ``gate | up = x w_gate_up^T``: x ``(..., K)``, w_gate_up ``(2 I, K)``, one type of float32, float16 and
-    bfloat16; returns ``(..., I)``.  Gradients go back to both (once: not a second time); the projections are kept for that, rounded to the
-    tensor type, ``2 I`` elements a row, and their gradients are rounded to it for the two products.  Works under graph capture; nothing is
+    bfloat16; returns ``(..., I)``.  Gradients go back to both (once: not a second time); the projections are kept for that in
+    float32, ``2 I`` elements a row; their gradients are rounded to the tensor type for the two products.  Works under graph capture; nothing is
     kept between calls."""
     if w_gate_up.ndim != 2 or w_gate_up.size(0) % 2 or w_gate_up.size(0) == 0 or w_gate_up.size(1) == 0:
         raise ValueError(f"weights have shape {tuple(w_gate_up.shape)}; expected (2 * intermediate, hidden)")

@@ -385,16 +385,16 @@ int ckv_norm_rotate_bwd(const ckv_norm_rotate_args* args, void* stream);
  * out (rows, inter) = silu(x Wg^T) * (x Wu^T), the two projections of a gated MLP, the activation and the product in one
  * call: x (rows, k), rows x_stride >= k elements apart, w (2 inter, k) contiguous: gate rows, then up rows.  float32
  * throughout, rounded once (ckv_linear_rows with `gated` and ckv_gated_silu round the projections and the activation too).
- * `gate_up` (rows, 2 inter), optional: the projections, rounded, as the backward pass takes them.  Everything but x
+ * `gate_up` float32 (rows, 2 inter), optional: the projections, as the backward pass takes them.  Everything but x
  * contiguous.  The backward pass writes dx (rows, k) and dw (2 inter, k), either of which may be NULL; it rounds the
  * gradients of the projections to the tensor dtype for its two products, whose sums are float32.  Sums are added up in a
  * fixed order.  The workspace sizes are those of a call on the current device.
  * ---------------------------------------------------------------------------------------- */
 int64_t ckv_gated_linear_workspace_bytes(int64_t rows, int64_t inter, int64_t k, int32_t dtype);
-int ckv_gated_linear(const void* x, const void* w, void* out, void* gate_up, int64_t rows, int64_t inter, int64_t k, int64_t x_stride,
+int ckv_gated_linear(const void* x, const void* w, void* out, float* gate_up, int64_t rows, int64_t inter, int64_t k, int64_t x_stride,
                      int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream);
 int64_t ckv_gated_linear_bwd_workspace_bytes(int64_t rows, int64_t inter, int64_t k, int32_t dtype);
-int ckv_gated_linear_bwd(const void* x, const void* w, const void* gate_up, const void* dout, void* dx, void* dw, int64_t rows,
+int ckv_gated_linear_bwd(const void* x, const void* w, const float* gate_up, const void* dout, void* dx, void* dw, int64_t rows,
                          int64_t inter, int64_t k, int64_t x_stride, int32_t dtype, void* workspace, int64_t workspace_bytes,
                          void* stream);
 
