@@ -288,7 +288,7 @@ template <typename T>
 bool fits_tiles(const ProductParams& p, bool along_a, bool along_b, bool gated) {
     if (sizeof(T) != 2) return false;
     auto whole = [&](const Operand& o, bool along, int64_t rows) {
-        return reinterpret_cast<uintptr_t>(o.p) % 16 == 0 && o.stride % 8 == 0 && (along ? p.K : rows) % 8 == 0 && o.stride < (1 << 22);
+        return reinterpret_cast<uintptr_t>(o.p) % 16 == 0 && o.stride % 8 == 0 && (along ? p.K : rows) % 8 == 0 && o.stride < (1 << 21);   // a tile of rows within 31 bits
     };
     return whole(p.a, along_a, p.M) && whole(p.b, along_b, p.N) && (gated ? p.N / 2 : p.N) % 8 == 0 &&
            ((reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.both)) & 15) == 0;

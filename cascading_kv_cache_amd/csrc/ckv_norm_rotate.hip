@@ -348,7 +348,7 @@ int launch_norm(NormParams& p, const ckv_norm_rotate_args* a, bool backward, int
     // Heads a block walks over: as many as leave sixteen wavefronts to a compute unit (a token's angles are worked out once a block)
     const int all = (int)(a->H + a->KVH);
     const int64_t wanted = std::max<int64_t>(1, 4 * (int64_t)cus / blocks);
-    p.heads_per = (int)std::max<int64_t>(1, all / wanted);
+    p.heads_per = (int)std::max<int64_t>((all + 32767) / 32768, all / wanted);   // chunks are a grid's y
     if (backward) p.heads_per = std::max(p.heads_per, (all + kMostChunks - 1) / kMostChunks);
     int chunks = 0;
     for (NormSide& s : p.side) chunks += s.chunks = (s.heads + p.heads_per - 1) / p.heads_per;

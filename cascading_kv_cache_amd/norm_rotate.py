@@ -150,6 +150,8 @@ def _check(q, k, q_weight, k_weight, positions, inv_freq):
 
 
 def _check_out(out, q, k):
+    if len(out) != 2:
+        raise ValueError(f"out is {len(out)} tensors; expected one for the queries and one for the keys")
     for name, t, like in (("queries", out[0], q), ("keys", out[1], k)):
         if t.dtype != like.dtype or t.device != like.device or t.shape != like.shape:
             raise ValueError(f"out holds {name} {tuple(t.shape)} of {t.dtype} on {t.device}; expected {tuple(like.shape)} of {like.dtype} on {like.device}")
@@ -166,7 +168,8 @@ def norm_rotate(q, k, q_weight=None, k_weight=None, positions=None, inv_freq=Non
     q ``(B, H, n, D)`` and k ``(B, KVH, n, D)``, float32, float16 or bfloat16, any strides.  ``q_weight``, ``k_weight`` ``(D,)``, dtype of q: the
     weights of the norm, or None for no norm.  ``positions`` int64 ``(n,)`` or ``(B, n)`` and ``inv_freq`` float32 ``(R / 2,)``: the first
     R <= D dims are rotated, dim j with dim j + R / 2 by ``position * inv_freq[j]``; or None for no rotation.  Gradients go back to q, k
-    and the weights (once: not a second time).  Works under graph capture; nothing is kept between calls."""
+    and the weights (once: not a second time).  Works under graph capture; nothing of the tensors is kept between calls.  Recorded into a graph, a
+    backward pass wants no eager graph of the same leaves alive: torch would have the recording wait for it."""
     tensors = q, k, q_weight, k_weight, positions, inv_freq
     followed = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors[:4])
     if out is not None:

@@ -48,7 +48,7 @@ def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0
             if value != value:
                 raise ValueError(f"{name} is not a number")
             # limits beyond 64 bits are none
-            setattr(a, number, max(0, min(int(value), MAX_VOCAB + 1)) if name == "top_k" else float(value))
+            setattr(a, number, int(max(0, min(value, MAX_VOCAB + 1))) if name == "top_k" else float(value))
             continue
         if value.dtype != dtype:
             raise TypeError(f"{name} is {value.dtype}, expected {dtype}")

@@ -264,3 +264,40 @@ def test_outputs_that_cannot_be_written_to():
             norm_rotate(q, k, qw, kw, out=out)
     with pytest.raises(ValueError, match="gradients"):
         norm_rotate(q, k, qw.requires_grad_(), kw, out=(q, k))
+
+
+def test_calls_alike_are_not_one_another():
+    """The same sizes and strides again and again, with other tensors, eps and positions, with gradients and without, in place and not."""
+    for dtype in (torch.bfloat16, torch.float32):
+        for seed in range(4):
+            q, k, qw, kw, (gq, gk) = inputs(2, 4, 2, 9, 64, dtype, "projected", seed)
+            pos, inv_freq, eps = torch.randint(0, 1000, (9,), device="cuda"), freqs(64, 1e4 * (seed + 1)), 10.0 ** (-seed - 1)
+            ins = [t.detach().requires_grad_() for t in (q, k, qw, kw)]
+            outs = norm_rotate(*ins, pos, inv_freq, eps)
+            grads = torch.autograd.grad(outs, ins, (gq, gk) if seed % 2 else (gq.transpose(1, 2).contiguous().transpose(1, 2), gk))
+            alone = norm_rotate(q, k, qw, kw, pos, inv_freq, eps)
+            for i, (x, w, g) in enumerate(((q, qw, gq), (k, kw, gk))):
+                want = exact(x, w, pos, inv_freq, eps, g)
+                close(outs[i], want["out"], dtype, "output")
+                close(grads[i], want["dx"], dtype, "gradient")
+                close(grads[2 + i], want["dw"], dtype, "weight gradient")
+            norm_rotate(q, k, qw, kw, pos, inv_freq, eps, out=(q, k))
+            assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(outs, alone, (q, k)))
+            with pytest.raises(ValueError, match="no gradient"):
+                norm_rotate(q, k, qw, kw, pos, inv_freq.clone().requires_grad_(), eps)
+            with pytest.raises(ValueError):
+                norm_rotate(q, k, qw, kw, pos, inv_freq, eps, out=(q,))
+
+
+@pytest.mark.parametrize("n", [1, 3])
+def test_many_heads(n):
+    q, k, qw, kw, (gq, gk) = inputs(1, 70000, 3, n, 4, torch.float16, "dense")
+    pos, inv_freq = torch.arange(n, device="cuda"), freqs(4)
+    ins = [t.detach().requires_grad_() for t in (q, k, qw, kw)]
+    outs = norm_rotate(*ins, pos, inv_freq, 1e-5)
+    grads = torch.autograd.grad(outs, ins, (gq, gk))
+    for i, (x, w, g) in enumerate(((q, qw, gq), (k, kw, gk))):
+        want = exact(x, w, pos, inv_freq, 1e-5, g)
+        close(outs[i], want["out"], torch.float16, "output")
+        close(grads[i], want["dx"], torch.float16, "gradient")
+        close(grads[2 + i], want["dw"], torch.float16, "weight gradient")

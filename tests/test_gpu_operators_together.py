@@ -186,3 +186,49 @@ def test_a_layers_gradients():
         results.append([out.detach(), *torch.autograd.grad(out, ins, dy if own else dy.double())])
     for i, (got, want) in enumerate(zip(*results)):
         assert (got - want).abs().max() <= 1e-3 * want.abs().max(), i
+
+
+def test_rows_further_apart_than_31_bits():
+    """Logits, heads and rows of a buffer of 2^32 elements, of which only theirs are written."""
+    far = 2 ** 31
+    base = torch.empty(2 * far + 4096, dtype=torch.bfloat16, device="cuda")
+    small = torch.randn(3, 4096, device="cuda").bfloat16()
+    wide = base.as_strided((3, 4096), (far, 1))
+    wide.copy_(small)
+    u = torch.rand(3, device="cuda")
+    assert all(torch.equal(a, b) for a, b in zip(sample_tokens(wide, u, top_p=0.9), sample_tokens(small, u, top_p=0.9)))
+    w = (torch.randn(512, 4096, device="cuda") / 64).bfloat16()
+    torch.testing.assert_close(gated_feed_forward(wide, w), gated_feed_forward(small, w), rtol=2.0 ** -7, atol=1e-6)   # half a step each, another order
+    q, far_q = small.view(1, 3, 32, 128).transpose(1, 2), wide.unflatten(1, (32, 128))[None].transpose(1, 2)
+    weight, pos = torch.rand(128, device="cuda").bfloat16(), torch.arange(3, device="cuda")
+    inv_freq = 1.0 / 1e4 ** (torch.arange(0, 128, 2, device="cuda").float() / 128)
+    near = norm_rotate(q, q, weight, weight, pos, inv_freq)
+    assert all(torch.equal(a, b) for a, b in zip(norm_rotate(far_q, far_q, weight, weight, pos, inv_freq), near))
+    norm_rotate(q, q, weight, weight, pos, inv_freq, out=(far_q, torch.empty_like(q)))
+    assert torch.equal(far_q, near[0])
+
+
+def test_a_layer_on_two_streams():
+    """Forward and backward of two layers' worth of operators at a time, each with scratch of its own."""
+    def step(seed):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        q, k = (torch.randn(2, h, 33, 64, generator=g, device="cuda").bfloat16().requires_grad_() for h in (8, 2))
+        qw, kw = (torch.rand(64, generator=g, device="cuda").bfloat16().requires_grad_() for _ in range(2))
+        x = torch.randn(66, 264, generator=g, device="cuda").bfloat16().requires_grad_()
+        w = (torch.randn(528, 264, generator=g, device="cuda") / 16).bfloat16().requires_grad_()
+        qs, ks = norm_rotate(q, k, qw, kw)
+        h = gated_feed_forward(x, w)
+        grads = torch.autograd.grad((qs, ks, h), (q, k, qw, kw, x, w), (torch.ones_like(qs), torch.ones_like(ks), torch.ones_like(h)))
+        return [t.detach() for t in (qs, ks, h)] + list(grads)
+
+    want = [step(s) for s in (1, 2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(i + 1))
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(a, b) for one in g for a, b in zip(one, w))

@@ -200,3 +200,30 @@ def test_another_stream_and_replays_of_a_graph(rows):
         fresh = sample_tokens(logits, u, **settings)       # the program's own work between two replays
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(recorded, fresh)), rep
+
+
+def test_no_limit_in_any_number():
+    logits, u = normal(3, 500, torch.float32, 2.0)
+    want = sample_tokens(logits, u)
+    for k in (0, -1, 500, 10 ** 30, float("inf")):
+        got = sample_tokens(logits, u, top_k=k)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    with pytest.raises(ValueError):
+        sample_tokens(logits, u, top_k=float("nan"))
+
+
+@pytest.mark.parametrize("rows", [1, 3, 140])
+def test_two_streams_at_a_time(rows):
+    a, b = normal(rows, 90001, torch.bfloat16, 3.0, 1), normal(rows, 90001, torch.bfloat16, 3.0, 2)
+    settings = dict(top_k=60, top_p=0.9)
+    want = [sample_tokens(*x, **settings) for x in (a, b)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for s, x, g in zip(streams, (a, b), got):
+            with torch.cuda.stream(s):
+                g.append(sample_tokens(*x, **settings))
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(t, w[0]) and torch.equal(l, w[1]) for t, l in g)
