@@ -124,37 +124,60 @@ __device__ inline uint64_t mass_of(int n, uint64_t some, const double* table) {
     return (uint64_t)rint(bin_weight(n, table) * (double)((count << 31) + rests - count * (int64_t)kBias) * 8192.0);   // 2^44 / 2^31
 }
 
-// fn(index, value) for a slice of a row: vectors of 16 bytes between what lies in front of the first aligned one and behind the last.
-template <typename T, typename Fn>
-__device__ inline void for_each(const T* row, int vocab, int slice, int slices, Fn fn) {
-    constexpr int kPer = 16 / (int)sizeof(T);
+// A slice of a row: vectors of 16 bytes between what lies in front of the first aligned one and behind the last.
+template <typename T>
+struct Slice {
+    static constexpr int kPer = 16 / (int)sizeof(T), kAhead = 4;
     struct alignas(16) Sixteen {
         T v[kPer];
     };
-    const int head = min(vocab, (int)(((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(T)));
-    const int vectors = (vocab - head) / kPer, behind = head + vectors * kPer;
-    if (slice == 0)
-        for (int i = threadIdx.x; i < head; i += blockDim.x) fn(i, Elem<T>::to_float(row[i]));
-    if (slice == slices - 1)
-        for (int i = behind + threadIdx.x; i < vocab; i += blockDim.x) fn(i, Elem<T>::to_float(row[i]));
-    const Sixteen* body = reinterpret_cast<const Sixteen*>(row + head);
-    const int each = (vectors + slices - 1) / slices, end = min(vectors, (slice + 1) * each);
-    constexpr int kAhead = 4;
-    for (int i = slice * each + threadIdx.x; i < end; i += kAhead * blockDim.x) {
-        Sixteen x[kAhead];
-#pragma unroll
-        for (int a = 0; a < kAhead; a++)
-            if (i + a * (int)blockDim.x < end) x[a] = body[i + a * blockDim.x];
-#pragma unroll
-        for (int a = 0; a < kAhead; a++)
-            if (i + a * (int)blockDim.x < end) {
-#pragma unroll
-                for (int e = 0; e < kPer; e++) fn(head + (i + a * (int)blockDim.x) * kPer + e, Elem<T>::to_float(x[a].v[e]));
-            }
+    const T* row;
+    const Sixteen* body;
+    int vocab, head, behind, first, end;
+    bool has_head, has_rest;
+    Sixteen x[kAhead];
+    __device__ Slice(const T* row_, int vocab_, int slice, int slices) : row(row_), vocab(vocab_) {
+        head = min(vocab, (int)(((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(T)));
+        const int vectors = (vocab - head) / kPer, each = (vectors + slices - 1) / slices;
+        behind = head + vectors * kPer;
+        body = reinterpret_cast<const Sixteen*>(row + head);
+        first = slice * each + threadIdx.x;
+        end = min(vectors, (slice + 1) * each);
+        has_head = slice == 0;
+        has_rest = slice == slices - 1;
     }
+    __device__ void load(int from) {
+#pragma unroll
+        for (int a = 0; a < kAhead; a++)
+            if (from + a * (int)blockDim.x < end) x[a] = body[from + a * blockDim.x];
+    }
+    // fn(index, value) for all of it, the first vectors of which are loaded
+    template <typename Fn>
+    __device__ void each_loaded(Fn fn) {
+        if (has_head)
+            for (int i = threadIdx.x; i < head; i += blockDim.x) fn(i, Elem<T>::to_float(row[i]));
+        if (has_rest)
+            for (int i = behind + threadIdx.x; i < vocab; i += blockDim.x) fn(i, Elem<T>::to_float(row[i]));
+        for (int i = first; i < end; i += kAhead * blockDim.x) {
+            if (i != first) load(i);
+#pragma unroll
+            for (int a = 0; a < kAhead; a++)
+                if (i + a * (int)blockDim.x < end) {
+#pragma unroll
+                    for (int e = 0; e < kPer; e++) fn(head + (i + a * (int)blockDim.x) * kPer + e, Elem<T>::to_float(x[a].v[e]));
+                }
+        }
+    }
+};
+
+template <typename T, typename Fn>
+__device__ inline void for_each(const T* row, int vocab, int slice, int slices, Fn fn) {
+    Slice<T> part(row, vocab, slice, slices);
+    part.load(part.first);
+    part.each_loaded(fn);
 }
 
-// Running sums over the workgroup (any whole number of wavefronts): what lies in front of this thread; `all` gets the total.
+// Running sums over the workgroup (up to sixteen wavefronts): what lies in front of this thread; `all` gets the total.
 template <typename V>
 __device__ inline V before_me(V v, V* waves, V* all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, many = blockDim.x >> 6;
@@ -167,18 +190,20 @@ __device__ inline V before_me(V v, V* waves, V* all) {
     __syncthreads();
     if (lane == 63) waves[wave] = s;
     __syncthreads();
-    V front = 0, total = 0;
-    for (int w = 0; w < many; w++) {
-        if (w < wave) front += waves[w];
-        total += waves[w];
+    V w = lane < many ? waves[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) {
+        const V other = __shfl_up(w, o);
+        if (lane >= o) w += other;
     }
-    *all = total;
-    return front + s - v;
+    *all = __shfl(w, 15);
+    const V front = __shfl(w, (wave + 63) & 63);
+    return (wave ? front : 0) + s - v;
 }
 
 // The largest of all in front of this thread; 0 if there is none.
 __device__ inline uint32_t latest_before_me(uint32_t v, uint32_t* waves) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, many = blockDim.x >> 6;
     uint32_t s = v;
 #pragma unroll
     for (int o = 1; o < CKV_WAVE; o <<= 1) {
@@ -189,19 +214,21 @@ __device__ inline uint32_t latest_before_me(uint32_t v, uint32_t* waves) {
     if (lane == 63) waves[wave] = s;
     const uint32_t before = __shfl_up(s, 1);
     __syncthreads();
-    uint32_t front = lane ? before : 0;
-    for (int w = 0; w < wave; w++) front = max(front, waves[w]);
-    return front;
+    uint32_t w = lane < min(wave, many) ? waves[lane] : 0;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) w = max(w, __shfl_xor(w, o));
+    return lane ? max(w, before) : w;
 }
 
-__device__ inline float block_max(float v, float* waves) {
+__device__ inline float block_max(float v, float* waves) {   // of sixteen wavefronts
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
     __syncthreads();
     if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = waves[0];
-    for (int w = 1; w < (int)(blockDim.x >> 6); w++) v = fmaxf(v, waves[w]);
+    v = waves[threadIdx.x & 15];
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
     return v;
 }
 
@@ -213,7 +240,7 @@ struct Shared {
     uint32_t narrow[16];
     float tops[16];
     uint32_t listed, last;
-    int first[2], counted[2];
+    int first[5], counted[2];
     Borders borders;
     unsigned long long answer[3];
 };
@@ -225,12 +252,15 @@ struct Lists {
 
 // ---- the bins --------------------------------------------------------------------------------------------------------------------------
 
-template <typename T>
-__device__ inline void fill_bins(Shared& sh, const T* row, const SampleParams& s, const Settings& set, float m, int slice) {
+__device__ inline void clear_bins(Shared& sh) {
     for (int i = threadIdx.x; i < kBins; i += blockDim.x) sh.mass[i] = 0;
     fill_table(sh.table);
+}
+
+template <typename T>
+__device__ inline void fill_bins(Shared& sh, Slice<T>& part, const Settings& set, float m) {
     __syncthreads();
-    for_each(row, s.vocab, slice, s.slices, [&](int, float l) {
+    part.each_loaded([&](int, float l) {
         double x;
         if (!distance(l, m, set.inv_t, x)) return;
         const float n = bin_of(x);
@@ -239,22 +269,16 @@ __device__ inline void fill_bins(Shared& sh, const T* row, const SampleParams& s
     __syncthreads();
 }
 
-// The first bins at whose ends `low` and `high` hold, which they then do behind every later one; the last bin if nowhere.
-template <typename Low, typename High>
-__device__ inline int2 first_bins(Shared& sh, Low low, High high) {
-    __syncthreads();
-    if (threadIdx.x == 0) sh.first[0] = sh.first[1] = kBins - 1;
-    __syncthreads();
-    for (int b = threadIdx.x; b < kBins; b += blockDim.x) {
-        if (low(b + 1) && (b == 0 || !low(b))) sh.first[0] = b;
-        if (high(b + 1) && (b == 0 || !high(b))) sh.first[1] = b;
-    }
-    __syncthreads();
-    return make_int2(sh.first[0], sh.first[1]);
-}
+// The first bin at whose end `reached` holds, which it then does behind every later one; the last bin if nowhere.
 template <typename Fn>
 __device__ inline int first_bin(Shared& sh, Fn reached) {
-    return first_bins(sh, reached, [](int) { return false; }).x;
+    __syncthreads();
+    if (threadIdx.x == 0) sh.first[0] = kBins - 1;
+    __syncthreads();
+    for (int b = threadIdx.x; b < kBins; b += blockDim.x)
+        if (reached(b + 1) && (b == 0 || !reached(b))) sh.first[0] = b;
+    __syncthreads();
+    return sh.first[0];
 }
 
 // u times a mass, as a whole number below it
@@ -264,11 +288,12 @@ __device__ inline uint64_t draw_below(double u, uint64_t mass) {
     return w < mass ? w : mass - 1;
 }
 
-// Bins become running sums, and the borders are looked up in them.
+// Bins become running sums, and the borders are looked up by the threads that have them: in registers, one exchange for top-k, one for top-p, one
+// for the token.
 __device__ inline void find_borders(Shared& sh, const Settings& set) {
     constexpr int kEach = (kBins + kThreads - 1) / kThreads;
-    uint64_t m[kEach], sm = 0, all_m;
-    uint32_t c[kEach], sc = 0, all_c;
+    uint64_t m[kEach + 1], sm = 0, all_m;
+    uint32_t c[kEach + 1], sc = 0, all_c;
     const int first = threadIdx.x * kEach;
 #pragma unroll
     for (int i = 0; i < kEach; i++) {
@@ -278,22 +303,32 @@ __device__ inline void find_borders(Shared& sh, const Settings& set) {
         sm += m[i];
         sc += c[i];
     }
+    if (threadIdx.x < 5) sh.first[threadIdx.x] = kBins - 1;
     uint64_t fm = before_me(sm, sh.wide, &all_m);   // its barriers let everybody read the bins first
     uint32_t fc = before_me(sc, sh.narrow, &all_c);
 #pragma unroll
-    for (int i = 0; i < kEach; i++) {
-        if (first + i < kBins) {
+    for (int i = 0; i <= kEach; i++) {
+        const uint64_t dm = i < kEach ? m[i] : 0;
+        const uint32_t dc = i < kEach ? c[i] : 0;
+        m[i] = fm;
+        c[i] = fc;
+        if (i < kEach && first + i < kBins) {
             sh.mass[first + i] = fm;
             sh.count[first + i] = fc;
         }
-        fm += m[i];
-        fc += c[i];
+        fm += dm;
+        fc += dc;
     }
     if (threadIdx.x == 0) {
         sh.mass[kBins] = all_m;
         sh.count[kBins] = all_c;
     }
-    __syncthreads();
+    // the first bin at whose end `reached` holds, which it then does behind every later one; the last bin if nowhere
+    auto look = [&](int slot, auto reached) {
+#pragma unroll
+        for (int i = 0; i < kEach; i++)
+            if (first + i < kBins && reached(m[i + 1], c[i + 1]) && (first + i == 0 || !reached(m[i], c[i]))) sh.first[slot] = first + i;
+    };
     Borders r;
     r.partial_k = 0;
 #pragma unroll
@@ -302,8 +337,11 @@ __device__ inline void find_borders(Shared& sh, const Settings& set) {
         r.to[i] = 0;
     }
     uint64_t low = all_m, high = all_m;   // of what is kept
-    if (set.k < (int)all_c) {
-        const int b = first_bin(sh, [&](int e) { return sh.count[e] >= (uint32_t)set.k; });
+    const bool some = set.k < (int)all_c;
+    if (some) look(0, [&](uint64_t, uint32_t e) { return e >= (uint32_t)set.k; });
+    __syncthreads();
+    if (some) {
+        const int b = sh.first[0];
         low = high = sh.mass[b + 1];
         if (sh.count[b + 1] != (uint32_t)set.k) {
             low = max((uint64_t)sh.mass[b], kOne);
@@ -314,9 +352,11 @@ __device__ inline void find_borders(Shared& sh, const Settings& set) {
     r.mass_k = high;
     if (set.p < 1.0) {
         const double t0 = set.p * (double)low, t1 = set.p * (double)high;
-        const int2 b = first_bins(sh, [&](int e) { return (double)sh.mass[e] >= t0; }, [&](int e) { return (double)sh.mass[e] >= t1; });
-        r.from[1] = b.x;
-        r.to[1] = b.y;
+        look(1, [&](uint64_t e, uint32_t) { return (double)e >= t0; });
+        look(2, [&](uint64_t e, uint32_t) { return (double)e >= t1; });
+        __syncthreads();
+        r.from[1] = sh.first[1];
+        r.to[1] = sh.first[2];
         low = min(low, max((uint64_t)sh.mass[r.from[1]], kOne));
         high = min(high, (uint64_t)sh.mass[r.to[1] + 1]);
     }
@@ -327,15 +367,16 @@ __device__ inline void find_borders(Shared& sh, const Settings& set) {
         high = min(high, (uint64_t)sh.mass[b + 1]);
     }
     const uint64_t d0 = draw_below(set.u, low), d1 = draw_below(set.u, high);
-    const int2 drawn = first_bins(sh, [&](int e) { return sh.mass[e] > d0; }, [&](int e) { return sh.mass[e] > d1; });
-    r.from[3] = drawn.x;
-    r.to[3] = drawn.y;
+    look(3, [&](uint64_t e, uint32_t) { return e > d0; });
+    look(4, [&](uint64_t e, uint32_t) { return e > d1; });
+    __syncthreads();
+    r.from[3] = sh.first[3];
+    r.to[3] = sh.first[4];
     uint32_t many = 0;
 #pragma unroll
     for (int i = 0; i < 4; i++)
         if (r.from[i] <= r.to[i]) many += sh.count[r.to[i] + 1] - sh.count[r.from[i]];
     r.many = many > (uint32_t)kListMax;
-    __syncthreads();
     if (threadIdx.x == 0) sh.borders = r;
     __syncthreads();
 }
@@ -349,7 +390,7 @@ __device__ inline float logit_of(uint64_t order) { return value_of(~(uint32_t)(o
 
 // The elements of the borders' bins.  All of them lie in one stretch of values: two comparisons pass most of a row over.
 template <typename T, typename Fn>
-__device__ inline void for_wanted(const T* row, const SampleParams& s, const Settings& set, float m, const Borders& r, int slice, int slices, Fn fn) {
+__device__ inline void for_wanted(Slice<T>& part, const Settings& set, float m, const Borders& r, Fn fn) {
     int low = kBins, high = 0;
 #pragma unroll
     for (int i = 0; i < 4; i++)
@@ -361,7 +402,7 @@ __device__ inline void for_wanted(const T* row, const SampleParams& s, const Set
     const double least = (double)m - (high + 1.5) * kBinWidth / set.inv_t, most = (double)m - (low - 1.5) * kBinWidth / set.inv_t;
     const float floor = least > -3.4e38 ? (float)least - fabsf((float)least) * 2.4e-7f : -__builtin_huge_valf();
     const float ceiling = most < 3.4e38 ? (float)most + fabsf((float)most) * 2.4e-7f : __builtin_huge_valf();
-    for_each(row, s.vocab, slice, slices, [&](int i, float l) {
+    part.each_loaded([&](int i, float l) {
         if (l < floor || l > ceiling) return;
         double x;
         if (distance(l, m, set.inv_t, x) && wanted(r, (int)bin_of(x))) fn(order_of(l, i));
@@ -580,14 +621,19 @@ __global__ void __launch_bounds__(kThreads) sample_row_kernel(SampleParams s) {
     const int64_t row = blockIdx.x;
     const T* logits = (const T*)s.logits + row * s.stride;
     const Settings set = settings_of(s, row);
+    Slice<T> part(logits, s.vocab, 0, 1);
+    part.load(part.first);
+    clear_bins(sh);
     float m = -__builtin_huge_valf();
-    for_each(logits, s.vocab, 0, 1, [&](int, float l) { m = fmaxf(m, l); });   // NaN is passed over
+    part.each_loaded([&](int, float l) { m = fmaxf(m, l); });   // NaN is passed over
+    part.load(part.first);
     m = block_max(m, sh.tops);
     if (!(m > -__builtin_huge_valf())) {
         if (threadIdx.x == 0) no_answer(s, row);
         return;
     }
-    fill_bins(sh, logits, s, set, m, 0);
+    fill_bins(sh, part, set, m);
+    part.load(part.first);
     find_borders(sh, set);
     const Borders r = sh.borders;
     if (r.many) {
@@ -596,7 +642,7 @@ __global__ void __launch_bounds__(kThreads) sample_row_kernel(SampleParams s) {
     }
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
-    for_wanted(logits, s, set, m, r, 0, 1, [&](uint64_t o) { li.list[atomicAdd(&sh.listed, 1u)] = o; });
+    for_wanted(part, set, m, r, [&](uint64_t o) { li.list[atomicAdd(&sh.listed, 1u)] = o; });
     __syncthreads();
     const int n = (int)sh.listed;
     __syncthreads();
@@ -618,8 +664,10 @@ __global__ void __launch_bounds__(kThreads) sample_max_kernel(SampleParams s) {
     if (threadIdx.x == 0) space.maxima[blockIdx.x] = m;
 }
 
-__device__ inline float top_of(const RowSpace& space, int slices) {
-    float m = (int)(threadIdx.x & 63) < slices ? space.maxima[threadIdx.x & 63] : -__builtin_huge_valf();
+__device__ inline float maximum_of(const RowSpace& space, int slices) {   // of a slice, a lane each
+    return (int)(threadIdx.x & 63) < slices ? space.maxima[threadIdx.x & 63] : -__builtin_huge_valf();
+}
+__device__ inline float top_of(float m) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
     return m;
@@ -646,10 +694,15 @@ __global__ void __launch_bounds__(kThreads) sample_bins_kernel(SampleParams s) {
     __shared__ Shared sh;
     const int64_t row = blockIdx.y;
     RowSpace& space = s.space[row];
-    const float m = top_of(space, s.slices);
-    if (!(m > -__builtin_huge_valf())) return;   // all of the row's workgroups
+    // everything there is to wait for on the way before the first of it is needed
+    const float maximum = maximum_of(space, s.slices);
+    Slice<T> part((const T*)s.logits + row * s.stride, s.vocab, blockIdx.x, s.slices);
+    part.load(part.first);
     const Settings set = settings_of(s, row);
-    fill_bins(sh, (const T*)s.logits + row * s.stride, s, set, m, blockIdx.x);
+    clear_bins(sh);
+    const float m = top_of(maximum);
+    if (!(m > -__builtin_huge_valf())) return;   // all of the row's workgroups
+    fill_bins(sh, part, set, m);
     for (int b = threadIdx.x; b < kBins; b += kThreads)
         if (sh.mass[b]) (void)__hip_atomic_fetch_add(&space.bins[b], sh.mass[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (!last_to_arrive(&space.arrived[0], s.slices, &sh.last)) return;
@@ -670,17 +723,20 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(SampleParams s) {
     const int64_t row = blockIdx.y;
     RowSpace& space = s.space[row];
     const T* logits = (const T*)s.logits + row * s.stride;
-    const float m = top_of(space, s.slices);
-    if (!(m > -__builtin_huge_valf())) {
+    const float maximum = maximum_of(space, s.slices);
+    const Borders r = space.borders;
+    Slice<T> part(logits, s.vocab, blockIdx.x, s.slices);
+    part.load(part.first);
+    const Settings set = settings_of(s, row);
+    const float m = top_of(maximum);
+    if (!(m > -__builtin_huge_valf())) {   // then there are no borders either
         if (blockIdx.x == 0 && threadIdx.x == 0) no_answer(s, row);
         return;
     }
-    const Settings set = settings_of(s, row);
-    const Borders r = space.borders;
     if (!r.many) {   // a slice's elements are collected here and take their place in the row's list together
         if (threadIdx.x == 0) sh.listed = 0;
         __syncthreads();
-        for_wanted(logits, s, set, m, r, blockIdx.x, s.slices, [&](uint64_t o) { li.list[atomicAdd(&sh.listed, 1u)] = o; });
+        for_wanted(part, set, m, r, [&](uint64_t o) { li.list[atomicAdd(&sh.listed, 1u)] = o; });
         __syncthreads();
         const uint32_t n = sh.listed;
         if (threadIdx.x == 0) sh.last = n ? __hip_atomic_fetch_add(&space.listed, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
@@ -689,10 +745,12 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(SampleParams s) {
         for (uint32_t i = threadIdx.x; i < n; i += kThreads) __hip_atomic_store(&space.list[at + i], li.list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     if (!last_to_arrive(&space.arrived[1], s.slices, &sh.last)) return;
+    const int n = r.many ? 0 : (int)read_through(&space.listed);
     for (int b = threadIdx.x; b <= kBins; b += kThreads) {
         sh.mass[b] = space.mass[b];
         sh.count[b] = space.count[b];
     }
+    for (int i = threadIdx.x; i < n; i += kThreads) li.list[i] = read_through(&space.list[i]);
     fill_table(sh.table);
     if (threadIdx.x == 0) sh.borders = r;
     __syncthreads();
@@ -700,9 +758,6 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(SampleParams s) {
         draw_from_row(sh, li, logits, s, row, set, m);
         return;
     }
-    const int n = (int)read_through(&space.listed);
-    for (int i = threadIdx.x; i < n; i += kThreads) li.list[i] = read_through(&space.list[i]);
-    __syncthreads();
     draw_from_list(sh, li, s, row, set, m, n);
 }
 
