@@ -227,3 +227,39 @@ def test_two_streams_at_a_time(rows):
     torch.cuda.synchronize()
     for g, w in zip(got, want):
         assert all(torch.equal(t, w[0]) and torch.equal(l, w[1]) for t, l in g)
+
+
+@pytest.mark.parametrize("settings", [dict(), dict(top_k=37), dict(top_p=0.5), dict(top_k=60001, top_p=0.25), dict(min_p=1.0), dict(top_k=50, top_p=0.95)], ids=str)
+def test_ties_in_long_rows(settings):
+    test_ties(2, 150001, settings)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [70001, 128256])
+def test_long_rows_alone_are_those_of_a_batch(vocab, dtype):
+    """In slices or not: the same tokens and the same logarithms."""
+    logits, u = normal(131, vocab, dtype, 2.5, 7)
+    low = torch.finfo(dtype).min
+    for i, spoil in enumerate((float("-inf"), float("nan"), low, float("inf"))):
+        logits[i, ::3] = spoil
+        logits[i, :9000] = spoil
+    logits[4] = float("nan")
+    logits[5] = float("-inf")
+    logits[6] = float("-inf")
+    logits[6, vocab - 1] = 2.0
+    logits[7] = 0.25
+    logits[8] = logits[8].clamp(max=1.0)      # a tie of many at the top
+    u[9:15] = torch.tensor([0.0, -1.0, 1.0, 2.0, 1 - 2.0 ** -24, float("nan")])
+    g = torch.Generator(device="cuda").manual_seed(8)
+    draw = lambda *values: torch.tensor(values, device="cuda")[torch.randint(0, len(values), (131,), generator=g, device="cuda")]   # noqa: E731
+    each = dict(temperature=draw(0.0, 0.5, 1.0, 2.0), top_k=draw(0, 1, 30, 500, 50000), top_p=draw(0.0, 0.5, 0.9, 1.0), min_p=draw(0.0, 0.01, 0.5, 1.0))
+    for settings in (dict(), dict(top_k=40), dict(top_p=0.9, temperature=0.8), dict(min_p=0.02), each):
+        tokens, logs = sample_tokens(logits, u, **settings)
+        for first, many in [(i, 1) for i in range(16)] + [(16, 3), (40, 33), (100, 31)]:
+            own = {n: v[first:first + many] if torch.is_tensor(v) else v for n, v in settings.items()}
+            t, l = sample_tokens(logits[first:first + many], u[first:first + many], **own)
+            assert torch.equal(t, tokens[first:first + many]), (settings, first)
+            assert torch.equal(l.view(torch.int32), logs[first:first + many].view(torch.int32)), (settings, first)
+    few = slice(9, 20)
+    check(logits[16:22], u[16:22], top_k=40, top_p=0.9)
+    check(logits[few], torch.rand(11, generator=g, device="cuda"), top_p=0.95)
