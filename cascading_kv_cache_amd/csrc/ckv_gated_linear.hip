@@ -14,6 +14,9 @@ namespace ckv {
 namespace {
 
 // ---- any type, stride and size: float32 products on v_mfma_f32_16x16x4 -----------------------------------------------------------------
+//
+// Bound by that instruction: 2048 x 16384 x 4096 takes 2210 us, 124 TFLOP/s, the matrix pipe busy 78 % of the cycles (the library's product 1820 us);
+// rows of an odd number of elements, which no load finds aligned, cost another tenth to quarter (509 x 5462 x 1023 85 us, x 1024 71).
 
 // kTile 128: eight wavefronts of 32 x 64, two on a SIMD: one's loads and stores stand beside the other's products.  64: four of 32 x 32, of
 // which several workgroups share a compute unit.
@@ -238,7 +241,8 @@ __global__ void __launch_bounds__(256) merge_kernel(ProductParams p, int tile_m,
 // ---- gradients of the projections ------------------------------------------------------------------------------------------------------
 
 // dg and du are rounded to the tensor type, that of the operands of the two products behind: off by up to 2^-8 of each (2^-11 of float16), as
-// the products' own results are by their rounding.  The projections they are made from are float32.  Bound by memory: 12 bytes read and 4 written an element.
+// the products' own results are by their rounding.  The projections they are made from are float32.  Bound by memory: 10 bytes read and 4 written an element
+// of 16 bits, 2048 x 18944 98 us, 5.5 TB/s.
 template <typename T, int kPer>
 __global__ void __launch_bounds__(256) gate_gradient_kernel(const float* gate_up, const T* dout, T* grad, int64_t rows, int64_t inter) {
     struct alignas(sizeof(T) * kPer) Piece {
