@@ -354,7 +354,8 @@ __global__ void __launch_bounds__(64 * kWavesM * kWavesN, kTileM == 256 || kDeep
 
 template <typename T, int kTileM, int kTileN, int kStages, int kDeep, bool kAlongKA, bool kAlongKB, Epilogue kEpilogue>
 int launch_tiles(const ProductParams& p, const TilePlan& plan, hipStream_t stream) {
-    auto kernel = tile_kernel<T, kTileM, kTileN, 2, 2, kStages, kDeep, kAlongKA, kAlongKB, kEpilogue>;
+    constexpr int kWavesN = kTileN % 64 ? 1 : 2;   // gate and up columns of a wavefront are whole blocks
+    auto kernel = tile_kernel<T, kTileM, kTileN, 4 / kWavesN, kWavesN, kStages, kDeep, kAlongKA, kAlongKB, kEpilogue>;
     constexpr int lds = kStages * kStageBytes<kTileM, kTileN, kDeep>;
     if (int rc = ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), lds)) return rc;
     hipLaunchKernelGGL(kernel, dim3((unsigned)plan.blocks()), dim3(256), lds, stream, p);
@@ -366,14 +367,19 @@ template <typename T, bool kAlongKA, bool kAlongKB, Epilogue kEpilogue>
 int launch_tiles(const ProductParams& p, const TilePlan& plan, hipStream_t stream) {
     if (plan.tile_m == 256) return launch_tiles<T, 256, 256, 4, 1, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
     if (plan.deep == 1) return launch_tiles<T, 128, 128, 4, 1, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
-    if constexpr (kEpilogue == kGate) {
-        if (plan.tile_n == 192)
-            return plan.tile_m == 128 ? launch_tiles<T, 128, 192, 4, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream)
-                                      : launch_tiles<T, 64, 192, 5, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
-        if (plan.tile_n == 256)
-            return plan.tile_m == 128 ? launch_tiles<T, 128, 256, 3, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream)
-                                      : launch_tiles<T, 64, 256, 4, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
-    }
+    if constexpr (kEpilogue == kGate)
+        switch (plan.tile_m * 1000 + plan.tile_n) {
+            case 128096: return launch_tiles<T, 128, 96, 5, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
+            case 128160: return launch_tiles<T, 128, 160, 4, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
+            case 128192: return launch_tiles<T, 128, 192, 4, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
+            case 128224: return launch_tiles<T, 128, 224, 3, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
+            case 128256: return launch_tiles<T, 128, 256, 3, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
+            case 64096: return launch_tiles<T, 64, 96, 7, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
+            case 64160: return launch_tiles<T, 64, 160, 5, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
+            case 64192: return launch_tiles<T, 64, 192, 5, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
+            case 64224: return launch_tiles<T, 64, 224, 4, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
+            case 64256: return launch_tiles<T, 64, 256, 4, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
+        }
     if constexpr (kAlongKA)
         return plan.tile_m == 128 ? launch_tiles<T, 128, 128, 4, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream)
                                   : launch_tiles<T, 64, 128, 6, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
@@ -381,30 +387,33 @@ int launch_tiles(const ProductParams& p, const TilePlan& plan, hipStream_t strea
 }
 
 // A kind of tile, and microseconds that its workgroups take on a compute unit, `resident` of them at a time: 32 steps, and around the steps.  Deep
-// kinds are for few rows, all of them in a tile, which wait for the bytes of B: 5.9 TB/s over all workgroups, and no less than `step_us`
-// (or 0.33 where B's rows lie across k: 32 x 4096 x 28672 58 us in eight shares, 82 in four).
+// kinds are for few rows, all of them in a tile, which wait for the bytes of B: 5.9 TB/s over all workgroups (halves of lines 4.6), and no less than
+// `step_us` (or 0.33 where B's rows lie across k: 32 x 4096 x 28672 58 us in eight shares, 82 in four).
 struct Kind {
     int tile_m, tile_n, deep, resident;
     double step_us, around_us, first_us;   // first_us: where others hide what is around the steps, once a launch
 };
-constexpr Kind kKinds[] = {{256, 256, 1, 1, 0.73, 8.5, 0}, {128, 128, 1, 2, 0.65, 1.0, 8.0}, {128, 128, 2, 1, 0.18, 4.0, 0}, {64, 128, 2, 1, 0.12, 4.0, 0},
-                           {128, 192, 2, 1, 0.36, 5.0, 0}, {64, 192, 2, 1, 0.33, 5.0, 0},    {128, 256, 2, 1, 0.48, 6.0, 0}, {64, 256, 2, 1, 0.42, 6.0, 0}};
+constexpr Kind kKinds[] = {{256, 256, 1, 1, 0.73, 8.5, 0}, {128, 128, 1, 2, 0.65, 1.0, 8.0},   // of two alike the first is taken: the lower, the wider
+                           {64, 256, 2, 1, 0.42, 6.0, 0},  {128, 256, 2, 1, 0.48, 6.0, 0},  {64, 224, 2, 1, 0.40, 6.0, 0}, {128, 224, 2, 1, 0.40, 6.0, 0},
+                           {64, 192, 2, 1, 0.33, 5.0, 0},  {128, 192, 2, 1, 0.36, 5.0, 0},  {64, 160, 2, 1, 0.30, 5.0, 0}, {128, 160, 2, 1, 0.30, 5.0, 0},
+                           {64, 128, 2, 1, 0.12, 4.0, 0},  {128, 128, 2, 1, 0.18, 4.0, 0},  {64, 96, 2, 1, 0.115, 4.0, 0}, {128, 96, 2, 1, 0.155, 4.0, 0}};
 
 }  // namespace
 
 // Tiles fill the compute units round by round; those of the last round may be shared out along k, which costs their sums a trip to memory (4
-// TB/s both ways, 3 us the launch that adds them up).  Of few rows the tiles are as wide as brings the columns nearest to full rounds, at 64 rows
-// (widths 128, 192 and 256): 28672 x 4096 44, 52 and 58 us, 37888 x 3584 60, 55 and 61, 51200 x 5120 more than 111, 107 and 103.
+// TB/s both ways, 3 us the launch that adds them up).  Of few rows the tiles are as wide as brings the columns nearest to full rounds, at 128 rows
+// (widths 96, 128, 160, 192, 224 and 256, each with the best number of shares): 22016 x 4096 41, 46, 51, 47, 49 and 49 us; 28672 x 4096 59, 49, 55, 59, 61
+// and 62; 37888 x 3584 more than 69, 68, 58, 61, 63 and 68; 51200 x 5120 more than 124, more than 124, 124, 116, 109 and 114.
 TilePlan plan_tiles(int64_t M, int64_t N, int64_t K, bool a_along_k, bool gated, int cus) {
     TilePlan best = {};
     double best_us = 0;
     for (const Kind& kind : kKinds) {
         const bool few = kind.deep > 1;
-        if (few && (!a_along_k || M > kind.tile_m || (kind.tile_n > 128 && !gated))) continue;
+        if (few && (!a_along_k || M > kind.tile_m || (kind.tile_n != 128 && !gated))) continue;
         const int64_t tiles_m = (M + kind.tile_m - 1) / kind.tile_m, tiles_n = tiles_across(N, kind.tile_n, gated), all = tiles_m * tiles_n;
         const int64_t places = (int64_t)cus * kind.resident, rest = all % places;
         auto time_of = [&](int64_t workgroups, int64_t steps) {   // of that many at a time
-            const double bytes_us = few ? (double)std::min<int64_t>(workgroups, cus) * kind.tile_n * kSteps * 2 / 5.9e6 : 0;
+            const double bytes_us = (double)std::min(workgroups, places) / tiles_m * kind.tile_n * kSteps * 2 / (few ? 5.9e6 : 4.6e6);
             return (double)steps / kSteps * std::max(few && !gated ? 0.33 : kind.step_us, bytes_us) + kind.around_us;
         };
         for (int shares = 1; shares <= 8; shares++) {

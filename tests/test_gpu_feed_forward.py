@@ -76,7 +76,8 @@ def test_against_float64(size, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES[:2])
-@pytest.mark.parametrize("size", [(50, 328, 18952), (100, 328, 18952), (64, 64, 17000), (33, 1032, 25608), (128, 520, 25608), (64, 456, 31000)], ids=str)
+@pytest.mark.parametrize("size", [(50, 328, 18952), (100, 328, 18952), (64, 64, 17000), (33, 1032, 25608), (128, 520, 25608), (64, 456, 31000),
+                                  (40, 520, 11016), (90, 776, 9736), (50, 2056, 22024), (100, 2056, 22024), (100, 2056, 28680), (20, 1536, 9728)], ids=str)
 def test_few_rows_and_wide_layers(size, dtype):
     """Columns that leave compute units idle, or are more than a round of them, in tiles of one width or another."""
     x, w, dh = inputs(*size, dtype)
