@@ -1,14 +1,14 @@
 // C (M, N) = sum over k of A (m, k) B (n, k) of 16-bit operands on v_mfma_f32_16x16x32, with the gate of a gated MLP or shares of the
 // sum behind it.
 //
-// A workgroup has a tile of C and brings 32 steps of both operands at a time into one of four stages of LDS by asynchronous copies, three
-// stages ahead: one barrier a stage.  An operand whose rows are adjacent along k lies in LDS as rows of 64 bytes, and an operand read is 16 of
-// them; one whose steps are adjacent along its rows lies as it is, and is turned on the way into registers (ds_read_b64_tr_b16).  Pieces of 16
-// bytes are permuted within a row as they are copied, so that an operand read meets every bank once.
+// A workgroup has a tile of C and brings 32 or 64 steps of both operands at a time into one of three to seven stages of LDS by asynchronous copies,
+// all but one of them ahead: one barrier a stage.  An operand whose rows are adjacent along k lies in LDS as rows of 64 or 128 bytes, and an operand
+// read is 16 of them; one whose steps are adjacent along its rows lies as it is, and is turned on the way into registers (ds_read_b64_tr_b16).
+// Pieces of 16 bytes are permuted within a row as they are copied, so that an operand read meets every bank once.
 //
-// Few rows wait for the bytes of B: their stages have 64 steps, whose rows are whole lines of 128 bytes (77 x 28672 x 4096 by halves of lines 53 us,
-// 44 so: 5.3 TB/s).  Many are bound by the products: 4096 x 28672 x 4096 takes 720 us, 1.34 PFLOP/s, which is what the library's product alone,
-// without the gate, takes on the same card.
+// Few rows wait for the bytes of B, and 64 steps of a row along k are a whole line (77 x 28672 x 4096 by halves of lines 53 us, 44 so: 5.3 TB/s).
+// Many are bound by the products and the power they take: 4096 x 28672 x 4096 720 us, 1.34 PFLOP/s (the library's product alone, without the gate, 640),
+// 2048 x 37888 x 3584 440 (510).  There the largest tile has room for stages of 32 steps alone, and is level with lower ones of 64.
 //
 // A wavefront of the large tile has 128 x 128 of it: with 64 x 128 each (eight wavefronts) the reads and copies of LDS alone take as long as the
 // products (a stage of 64 steps: 1536 + 512 of 2048 cycles).  One wavefront on a SIMD hides nothing behind another, so reads of the next
@@ -210,8 +210,9 @@ __global__ void __launch_bounds__(64 * kWavesM * kWavesN, kTileM == 256 || kDeep
     };
     // The stage that is copied next.  Behind the last whole one comes the first again (to nobody's use, where that is where it began).  Few rows
     // wait for the bytes of B, and workgroups that go through its rows side by side ask for the same few channels of memory at a time: they begin
-    // in different places (32 x 28672 x 4096: 62.7 -> 55.2 us.  Where B's steps are its rows, which they share, not: 58 -> 67).
-    int ahead = kDeep > 1 && kAlongKB && whole > 0 ? (int)((blockIdx.x * 2654435761u >> 8) % (uint32_t)whole) : 0;
+    // in different places (32 x 28672 x 4096: 62.7 -> 55.2 us).  Those that share rows do not: they would miss each other's in the L2 (tiles of
+    // 256 x 128, 1024 x 22016 x 4096: 158 us, 290 so; where B's steps are its rows, which all share, 58 -> 67).
+    int ahead = kDeep > 1 && kAlongKB && whole > 0 && p.tiles_m == 1 ? (int)(((uint32_t)tn * 2654435761u >> 8) % (uint32_t)whole) : 0;
     const int64_t back_a = (1 - whole) * a.advance, back_b = (1 - whole) * b.advance;
     a.at += ahead * a.advance;
     b.at += ahead * b.advance;
@@ -365,10 +366,12 @@ int launch_tiles(const ProductParams& p, const TilePlan& plan, hipStream_t strea
 
 template <typename T, bool kAlongKA, bool kAlongKB, Epilogue kEpilogue>
 int launch_tiles(const ProductParams& p, const TilePlan& plan, hipStream_t stream) {
-    if (plan.tile_m == 256) return launch_tiles<T, 256, 256, 4, 1, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
+    if (plan.tile_m == 256 && plan.deep == 1) return launch_tiles<T, 256, 256, 4, 1, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
     if (plan.deep == 1) return launch_tiles<T, 128, 128, 4, 1, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
     if constexpr (kEpilogue == kGate)
         switch (plan.tile_m * 1000 + plan.tile_n) {
+            case 256096: return launch_tiles<T, 256, 96, 3, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
+            case 256160: return launch_tiles<T, 256, 160, 3, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
             case 128096: return launch_tiles<T, 128, 96, 5, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
             case 128160: return launch_tiles<T, 128, 160, 4, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
             case 128192: return launch_tiles<T, 128, 192, 4, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
@@ -380,46 +383,53 @@ int launch_tiles(const ProductParams& p, const TilePlan& plan, hipStream_t strea
             case 64224: return launch_tiles<T, 64, 224, 4, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
             case 64256: return launch_tiles<T, 64, 256, 4, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
         }
-    if constexpr (kAlongKA)
+    if constexpr (kAlongKA) {
+        if (plan.tile_m == 256) return launch_tiles<T, 256, 128, 3, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
         return plan.tile_m == 128 ? launch_tiles<T, 128, 128, 4, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream)
                                   : launch_tiles<T, 64, 128, 6, 2, kAlongKA, kAlongKB, kEpilogue>(p, plan, stream);
+    }
     return CKV_ERR_UNSUPPORTED;
 }
 
-// A kind of tile, and microseconds that its workgroups take on a compute unit, `resident` of them at a time: 32 steps, and around the steps.  Deep
-// kinds are for few rows, all of them in a tile, which wait for the bytes of B: 5.9 TB/s over all workgroups (halves of lines 4.6), and no less than
-// `step_us` (or 0.33 where B's rows lie across k: 32 x 4096 x 28672 58 us in eight shares, 82 in four).
+// A kind of tile, and microseconds that its workgroups take on a compute unit, `resident` of them at a time: 32 steps, and around the steps.  More
+// the more units have one, as the clock falls; no less than the bytes of B take, 5.9 TB/s by whole lines (deep kinds) and 4.6 by halves.  Where B's rows
+// lie across k, deep kinds are for rows that fit in a tile, at 0.33 (32 x 4096 x 28672 58 us in eight shares, 82 in four).
 struct Kind {
     int tile_m, tile_n, deep, resident;
-    double step_us, around_us, first_us;   // first_us: where others hide what is around the steps, once a launch
+    double step_us, full_us, around_us, first_us;   // alone, and on all units; first_us: where others hide what is around the steps, once a launch
 };
-constexpr Kind kKinds[] = {{256, 256, 1, 1, 0.73, 8.5, 0}, {128, 128, 1, 2, 0.65, 1.0, 8.0},   // of two alike the first is taken: the lower, the wider
-                           {64, 256, 2, 1, 0.42, 6.0, 0},  {128, 256, 2, 1, 0.48, 6.0, 0},  {64, 224, 2, 1, 0.40, 6.0, 0}, {128, 224, 2, 1, 0.40, 6.0, 0},
-                           {64, 192, 2, 1, 0.33, 5.0, 0},  {128, 192, 2, 1, 0.36, 5.0, 0},  {64, 160, 2, 1, 0.30, 5.0, 0}, {128, 160, 2, 1, 0.30, 5.0, 0},
-                           {64, 128, 2, 1, 0.12, 4.0, 0},  {128, 128, 2, 1, 0.18, 4.0, 0},  {64, 96, 2, 1, 0.115, 4.0, 0}, {128, 96, 2, 1, 0.155, 4.0, 0}};
+constexpr Kind kKinds[] = {{256, 256, 1, 1, 0.47, 0.74, 8.5, 0}, {128, 128, 1, 2, 0.65, 0.65, 1.0, 8.0},   // of two alike the first is taken
+                           {64, 96, 2, 1, 0.10, 0.15, 4.0, 0},   {128, 96, 2, 1, 0.145, 0.20, 4.0, 0},  {256, 96, 2, 1, 0.22, 0.30, 5.0, 0},
+                           {64, 128, 2, 1, 0.11, 0.16, 4.0, 0},  {128, 128, 2, 1, 0.13, 0.24, 4.0, 0},  {256, 128, 2, 1, 0.28, 0.37, 5.0, 0},
+                           {64, 160, 2, 1, 0.10, 0.36, 5.0, 0},  {128, 160, 2, 1, 0.15, 0.28, 5.0, 0},  {256, 160, 2, 1, 0.36, 0.445, 6.0, 0},
+                           {64, 192, 2, 1, 0.12, 0.45, 5.0, 0},  {128, 192, 2, 1, 0.20, 0.33, 5.0, 0},  {64, 256, 2, 1, 0.20, 0.60, 6.0, 0},
+                           {128, 256, 2, 1, 0.42, 0.43, 6.0, 0}, {64, 224, 2, 1, 0.14, 0.50, 6.0, 0},   {128, 224, 2, 1, 0.30, 0.36, 6.0, 0}};
 
 }  // namespace
 
 // Tiles fill the compute units round by round; those of the last round may be shared out along k, which costs their sums a trip to memory (4
-// TB/s both ways, 3 us the launch that adds them up).  Of few rows the tiles are as wide as brings the columns nearest to full rounds, at 128 rows
-// (widths 96, 128, 160, 192, 224 and 256, each with the best number of shares): 22016 x 4096 41, 46, 51, 47, 49 and 49 us; 28672 x 4096 59, 49, 55, 59, 61
-// and 62; 37888 x 3584 more than 69, 68, 58, 61, 63 and 68; 51200 x 5120 more than 124, more than 124, 124, 116, 109 and 114.
+// TB/s both ways, 3 us the launch that adds them up).  What decides between the kinds is how near the tiles come to full rounds.  128
+// rows, 128 high and 96, 128, 160, 192, 224 and 256 wide, each in the best number of shares: 22016 x 4096 41, 46, 51, 47, 49 and 49 us; 28672 x 4096 59, 49,
+// 55, 59, 61 and 62; 37888 x 3584 more than 69, 68, 58, 61, 63 and 68; 51200 x 5120 more than 124 twice, 124, 116, 109 and 114.  More rows, 256 high
+// and 128, 160 and (32 steps a stage) 256 wide: 256 x 28672 x 4096 61, 66 and 96; 512 x 37888 x 3584 146, 115 and 173; 1024 x 34816 x 5120 336, 303 and
+// 371; 4096 x 28672 x 4096 733, 721 and 713.
 TilePlan plan_tiles(int64_t M, int64_t N, int64_t K, bool a_along_k, bool gated, int cus) {
     TilePlan best = {};
     double best_us = 0;
     for (const Kind& kind : kKinds) {
-        const bool few = kind.deep > 1;
-        if (few && (!a_along_k || M > kind.tile_m || (kind.tile_n != 128 && !gated))) continue;
+        const bool deep = kind.deep > 1;
+        if (deep && (!a_along_k || (!gated && (M > kind.tile_m || kind.tile_n != 128)))) continue;
         const int64_t tiles_m = (M + kind.tile_m - 1) / kind.tile_m, tiles_n = tiles_across(N, kind.tile_n, gated), all = tiles_m * tiles_n;
         const int64_t places = (int64_t)cus * kind.resident, rest = all % places;
         auto time_of = [&](int64_t workgroups, int64_t steps) {   // of that many at a time
-            const double bytes_us = (double)std::min(workgroups, places) / tiles_m * kind.tile_n * kSteps * 2 / (few ? 5.9e6 : 4.6e6);
-            return (double)steps / kSteps * std::max(few && !gated ? 0.33 : kind.step_us, bytes_us) + kind.around_us;
+            const double bytes_us = (double)std::min(workgroups, places) / tiles_m * kind.tile_n * kSteps * 2 / (deep ? 5.9e6 : 4.6e6);
+            const double step_us = deep && !gated ? 0.33 : kind.step_us + (kind.full_us - kind.step_us) * (double)std::min<int64_t>(workgroups, cus) / cus;
+            return (double)steps / kSteps * std::max(step_us, bytes_us) + kind.around_us;
         };
         for (int shares = 1; shares <= 8; shares++) {
             // Behind full rounds of products compute units may idle: the others' clock rises (2048 x 37888 x 3584, 4.6 rounds: 457 us, 485 with the
-            // rest in three shares), unless it is bytes they wait for.
-            if (shares > 1 && (rest == 0 || K / shares < 256 || (!few && all > places))) break;
+            // rest in three shares), unless it is bytes they wait for, as few rows do.
+            if (shares > 1 && (rest == 0 || K / shares < 256 || (!(deep && tiles_m == 1) && all > places))) break;
             const int64_t k_share = shares == 1 ? K : ((K + shares - 1) / shares + 63) / 64 * 64;
             if ((K + k_share - 1) / k_share != shares) continue;
             double rounds = (double)((rest * shares + cus - 1) / cus);

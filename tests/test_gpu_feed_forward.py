@@ -77,7 +77,9 @@ def test_against_float64(size, dtype):
 
 @pytest.mark.parametrize("dtype", TYPES[:2])
 @pytest.mark.parametrize("size", [(50, 328, 18952), (100, 328, 18952), (64, 64, 17000), (33, 1032, 25608), (128, 520, 25608), (64, 456, 31000),
-                                  (40, 520, 11016), (90, 776, 9736), (50, 2056, 22024), (100, 2056, 22024), (100, 2056, 28680), (20, 1536, 9728)], ids=str)
+                                  (40, 520, 11016), (90, 776, 9736), (50, 2056, 22024), (100, 2056, 22024), (100, 2056, 28680), (20, 1536, 9728),
+                                  (200, 1032, 14344), (250, 520, 18952), (140, 264, 11016), (300, 520, 18952), (300, 456, 5640), (700, 328, 5640), (520, 1032, 17416),
+                                  (390, 264, 2824)], ids=str)
 def test_few_rows_and_wide_layers(size, dtype):
     """Columns that leave compute units idle, or are more than a round of them, in tiles of one width or another."""
     x, w, dh = inputs(*size, dtype)
