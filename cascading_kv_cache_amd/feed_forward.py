@@ -8,10 +8,10 @@ rounded once, where ``gated_silu`` behind a product, and the fused products of a
 operations and round three times.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _abi
 from .cascading_cache import _require_device, on_device, raw_stream
+from .norm_rotate import once
 
 
 def _scratch(nbytes, device):
@@ -45,21 +45,28 @@ class _GatedFeedForward(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
-        x, w, gate_up = ctx.saved_tensors
-        rows, k = x.shape
-        inter = w.size(0) // 2
-        lib, code = _abi.lib(), _abi.dtype_code(x.dtype)
-        dout = dout.to(x.dtype).contiguous()
-        dx = torch.empty(rows, k, dtype=x.dtype, device=x.device) if ctx.needs_input_grad[0] else None
-        dw = torch.empty(w.shape, dtype=w.dtype, device=w.device) if ctx.needs_input_grad[1] else None
-        with on_device(x.device):
-            ws = _scratch(lib.ckv_gated_linear_bwd_workspace_bytes(rows, inter, k, code), x.device)
-            _abi.check(lib.ckv_gated_linear_bwd(_at(x), _at(w), _at(gate_up), _at(dout), _at(dx), _at(dw), rows, inter, k,
-                                                x.stride(0) if rows > 1 else k, code, _at(ws), 0 if ws is None else ws.numel(),
-                                                raw_stream(x.device)), "ckv_gated_linear_bwd")
-        return dx, dw
+        if not torch.is_grad_enabled():
+            return _gradients(ctx, dout)
+        with torch.no_grad():
+            results = _gradients(ctx, dout)
+        return once(results, (*ctx.saved_tensors[:2], dout))
+
+
+def _gradients(ctx, dout):
+    x, w, gate_up = ctx.saved_tensors
+    rows, k = x.shape
+    inter = w.size(0) // 2
+    lib, code = _abi.lib(), _abi.dtype_code(x.dtype)
+    dout = dout.to(x.dtype).contiguous()
+    dx = torch.empty(rows, k, dtype=x.dtype, device=x.device) if ctx.needs_input_grad[0] else None
+    dw = torch.empty(w.shape, dtype=w.dtype, device=w.device) if ctx.needs_input_grad[1] else None
+    with on_device(x.device):
+        ws = _scratch(lib.ckv_gated_linear_bwd_workspace_bytes(rows, inter, k, code), x.device)
+        _abi.check(lib.ckv_gated_linear_bwd(_at(x), _at(w), _at(gate_up), _at(dout), _at(dx), _at(dw), rows, inter, k,
+                                            x.stride(0) if rows > 1 else k, code, _at(ws), 0 if ws is None else ws.numel(),
+                                            raw_stream(x.device)), "ckv_gated_linear_bwd")
+    return dx, dw
 
 
 def gated_feed_forward(x, w_gate_up):

@@ -11,7 +11,6 @@ to the tensor dtype on the way, everything here is float32, the angle the exact 
 import ctypes as C
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _abi
 from .cascading_cache import _require_device, on_device, raw_stream
@@ -83,6 +82,25 @@ def _forward(layout, q, k, q_weight, k_weight, positions, inv_freq, eps, out=Non
     return q_out, k_out
 
 
+class _Refused(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, many, *tensors):
+        return tuple(t.view_as(t) for t in tensors[:many])
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("gradients of this operator have none of their own (once_differentiable)")
+
+
+def once(results, tensors):
+    """Gradients in a graph that is made of them: as ``torch.autograd.function.once_differentiable``, which lets a second time pass as if nothing led from
+    the operator's inputs to its gradients where the gradient handed to it has no graph, but refused on every way to ``tensors``."""
+    there = [r for r in results if r is not None]
+    refused = iter(_Refused.apply(len(there), *there, *(t for t in tensors if t is not None and t.requires_grad)))
+    return tuple(None if r is None else next(refused) for r in results)
+
+
 class _NormRotate(torch.autograd.Function):
 
     @staticmethod
@@ -92,26 +110,33 @@ class _NormRotate(torch.autograd.Function):
         return _forward(layout, q, k, q_weight, k_weight, positions, inv_freq, eps)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, *grads):
-        q, k, q_weight, k_weight, positions, inv_freq = ctx.saved_tensors
-        # a gradient may be an expanded scalar, or in an order of its own
-        q_grad, k_grad = (g if g.stride(-1) == 1 or g.size(-1) == 1 else g.contiguous() for g in grads)
-        dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
-        a = ctx.layout.block((q_grad, k_grad), dq, dk)
-        _point(a, q, k, q_weight, k_weight, positions, inv_freq, ctx.eps)
-        a.q_grad, a.k_grad, a.dq, a.dk = q_grad.data_ptr(), k_grad.data_ptr(), dq.data_ptr(), dk.data_ptr()
-        dqw = dkw = None
-        device = q.device
-        with on_device(device):
-            if q_weight is not None:
-                dqw, dkw = q_weight.new_empty(q_weight.shape), k_weight.new_empty(k_weight.shape)
-                a.dq_weight, a.dk_weight = dqw.data_ptr(), dkw.data_ptr()
-                # of this call alone: a graph that records it must share its scratch with nobody
-                ws = torch.empty(ctx.layout.scratch, dtype=torch.uint8, device=device)
-                a.workspace, a.workspace_bytes = ws.data_ptr(), ctx.layout.scratch
-            _abi.check(_abi.lib().ckv_norm_rotate_bwd(C.byref(a), raw_stream(device)), "ckv_norm_rotate_bwd")
-        return None, None, dq, dk, dqw, dkw, None, None
+        if not torch.is_grad_enabled():
+            return _gradients(ctx, *grads)
+        with torch.no_grad():
+            results = _gradients(ctx, *grads)
+        return once(results, (*ctx.saved_tensors, *grads))
+
+
+def _gradients(ctx, *grads):
+    q, k, q_weight, k_weight, positions, inv_freq = ctx.saved_tensors
+    # a gradient may be an expanded scalar, or in an order of its own
+    q_grad, k_grad = (g if g.stride(-1) == 1 or g.size(-1) == 1 else g.contiguous() for g in grads)
+    dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
+    a = ctx.layout.block((q_grad, k_grad), dq, dk)
+    _point(a, q, k, q_weight, k_weight, positions, inv_freq, ctx.eps)
+    a.q_grad, a.k_grad, a.dq, a.dk = q_grad.data_ptr(), k_grad.data_ptr(), dq.data_ptr(), dk.data_ptr()
+    dqw = dkw = None
+    device = q.device
+    with on_device(device):
+        if q_weight is not None:
+            dqw, dkw = q_weight.new_empty(q_weight.shape), k_weight.new_empty(k_weight.shape)
+            a.dq_weight, a.dk_weight = dqw.data_ptr(), dkw.data_ptr()
+            # of this call alone: a graph that records it must share its scratch with nobody
+            ws = torch.empty(ctx.layout.scratch, dtype=torch.uint8, device=device)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), ctx.layout.scratch
+        _abi.check(_abi.lib().ckv_norm_rotate_bwd(C.byref(a), raw_stream(device)), "ckv_norm_rotate_bwd")
+    return None, None, dq, dk, dqw, dkw, None, None
 
 
 def _check(q, k, q_weight, k_weight, positions, inv_freq):

@@ -232,3 +232,16 @@ def test_a_layer_on_two_streams():
     torch.cuda.synchronize()
     for g, w in zip(got, want):
         assert all(torch.equal(a, b) for one in g for a, b in zip(one, w))
+
+
+def test_a_graph_of_the_gradients_can_be_made_and_not_gone_through():
+    q, k = (torch.randn(1, h, 5, 64, device="cuda", requires_grad=True) for h in (4, 2))
+    qw, kw = (torch.rand(64, device="cuda", requires_grad=True) for _ in range(2))
+    x, w = torch.randn(6, 32, device="cuda", requires_grad=True), torch.randn(32, 32, device="cuda", requires_grad=True)
+    for leaves, outs in (((q, k, qw, kw), norm_rotate(q, k, qw, kw)), ((x, w), (gated_feed_forward(x, w),))):
+        once = torch.autograd.grad(outs, leaves, [torch.ones_like(o) for o in outs], retain_graph=True)
+        made = torch.autograd.grad(outs, leaves, [torch.ones_like(o) for o in outs], create_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(once, made))
+        for which in (0, -1):
+            with pytest.raises(RuntimeError, match="once_differentiable"):
+                torch.autograd.grad(made[which].sum() + leaves[0].sum(), leaves[0], retain_graph=True)
