@@ -9,6 +9,7 @@
 #include "ckv_product.h"
 
 #include <algorithm>
+#include <initializer_list>
 
 namespace ckv {
 namespace {
@@ -185,10 +186,11 @@ __global__ void __launch_bounds__(kThreads<kTile>) product_kernel(ProductParams 
                     }
                 }
             } else {
+                const float power = power_of<T, kAlongKA>(p, m);
 #pragma unroll
                 for (int j = 0; j < kAcross; j++) {
                     const int64_t n = n0 + column(j) + l;
-                    if (n < p.N) ((T*)p.out)[m * p.N + n] = Elem<T>::from_float(acc[i][j][r]);
+                    if (n < p.N) ((T*)p.out)[m * p.N + n] = Elem<T>::from_float(times_power<T>(acc[i][j][r], power));
                 }
             }
         }
@@ -196,7 +198,7 @@ __global__ void __launch_bounds__(kThreads<kTile>) product_kernel(ProductParams 
 
 // Sums of the shares of a tile, in their order, and what the product's own epilogue does.  A workgroup has some rows of a tile, a thread four
 // columns.
-template <typename T, Epilogue kEpilogue>
+template <typename T, Epilogue kEpilogue, bool kAlongKA>
 __global__ void __launch_bounds__(256) merge_kernel(ProductParams p, int tile_m, int tile_n, int high, int rows) {
     constexpr bool kGated = kEpilogue == kGate;
     const int tile = p.whole_tiles + blockIdx.x;
@@ -212,6 +214,7 @@ __global__ void __launch_bounds__(256) merge_kernel(ProductParams p, int tile_m,
         const int64_t m = m0 + row, n = n0 + col;
         if (m >= p.M || n >= cols) continue;
         const float* at = from + (int64_t)row * tile_n + col;
+        const float power = kGated ? 1.f : power_of<T, kAlongKA>(p, m);
         float g[4] = {}, u[4] = {};
         for (int s = 0; s < p.shares; s++) {
             const float4 a = *reinterpret_cast<const float4*>(at + s * share);
@@ -232,7 +235,7 @@ __global__ void __launch_bounds__(256) merge_kernel(ProductParams p, int tile_m,
                     to[cols] = u[e];
                 }
             } else {
-                ((T*)p.out)[m * cols + n + e] = Elem<T>::from_float(g[e]);
+                ((T*)p.out)[m * cols + n + e] = Elem<T>::from_float(times_power<T>(g[e], power));
             }
         }
     }
@@ -243,6 +246,12 @@ __global__ void __launch_bounds__(256) merge_kernel(ProductParams p, int tile_m,
 // dg and du are rounded to the tensor type, that of the operands of the two products behind: off by up to 2^-8 of each (2^-11 of float16), as
 // the products' own results are by their rounding.  The projections they are made from are float32.  Bound by memory: 10 bytes read and 4 written an element
 // of 16 bits, 2048 x 18944 98 us, 5.5 TB/s.
+__device__ inline void gate_gradients(float g, float u, float d, float& dg, float& du) {
+    const float s = 1.f / (1.f + expf(-g));
+    dg = d * u * s * (1.f + g * (1.f - s));
+    du = d * g * s;
+}
+
 template <typename T, int kPer>
 __global__ void __launch_bounds__(256) gate_gradient_kernel(const float* gate_up, const T* dout, T* grad, int64_t rows, int64_t inter) {
     struct alignas(sizeof(T) * kPer) Piece {
@@ -261,10 +270,10 @@ __global__ void __launch_bounds__(256) gate_gradient_kernel(const float* gate_up
         Piece dg, du;
 #pragma unroll
         for (int e = 0; e < kPer; e++) {
-            const float g = gate.v[e], u = up.v[e], d = Elem<T>::to_float(dh.v[e]);
-            const float s = 1.f / (1.f + expf(-g));
-            dg.v[e] = Elem<T>::from_float(d * u * s * (1.f + g * (1.f - s)));
-            du.v[e] = Elem<T>::from_float(d * g * s);
+            float a, b;
+            gate_gradients(gate.v[e], up.v[e], Elem<T>::to_float(dh.v[e]), a, b);
+            dg.v[e] = Elem<T>::from_float(a);
+            du.v[e] = Elem<T>::from_float(b);
         }
         T* to = grad + row * 2 * inter + c * kPer;
         *reinterpret_cast<Piece*>(to) = dg;
@@ -281,6 +290,163 @@ int gate_gradient(const float* gate_up, const void* dout, void* grad, int64_t ro
     const unsigned blocks = (unsigned)std::min<int64_t>((all + 255) / 256, 256 * 16);
     if (pieces) hipLaunchKernelGGL((gate_gradient_kernel<T, kPer>), dim3(blocks), dim3(256), 0, stream, gate_up, (const T*)dout, (T*)grad, rows, inter);
     else hipLaunchKernelGGL((gate_gradient_kernel<T, 1>), dim3(blocks), dim3(256), 0, stream, gate_up, (const T*)dout, (T*)grad, rows, inter);
+    CKV_HIP_TRY(hipGetLastError());
+    return CKV_OK;
+}
+
+// float16 ends at 65504 and thins out below 2^-14, where dg and du, products of three numbers, need not stop: a dh of a scaled loss that is well inside the
+// type makes a dg that is not, and so does a small one at the other end.  So a row of [dg du] is kept as numbers below 2^15 times a power of two of its own,
+// 2^e, which dx's row is multiplied by in float32 (exact, until the row is rounded).  For dW, whose sums run over rows, row m of x takes 2^(e_m - T) along,
+// T the largest of e_m and the exponent of x's row, so that no row is above 2^15 and the largest product of two rows is at the top of the range:
+//   dx_m = 2^(e_m) ([dg du]_m 2^(-e_m)) W,   dW = 2^T sum over m of ([dg du]_m 2^(-e_m)) (x_m 2^(e_m - T)).
+// Below 2^-28 of its row's largest an element of [dg du] loses digits, and one of x below 2^-28 of what its row would have at the top; it is then off by up to
+// 2^-39 of those.  bfloat16 has float32's range and needs none of it.
+
+constexpr int kNoExponent = -1000;   // of a row of zeros
+
+// 2^e of a row whose largest number is m: m 2^-e lies in [2^14, 2^15)
+__device__ inline int exponent_above(float m) { return m > 0.f ? __builtin_amdgcn_frexp_expf(m) - 15 : kNoExponent; }
+__device__ inline float larger_finite(float m, float v) {
+    v = fabsf(v);
+    return v < __builtin_huge_valf() ? fmaxf(m, v) : m;   // infinities and NaN stay what they are at any scale
+}
+
+// A workgroup a row: the row's gradients stay in registers (kHeld pieces a thread; what is behind is worked out twice) until its largest is known.
+// exponents: e of every row, then e and the exponent of x's row together.  2048 x 18944 117 us, 4.7 TB/s: a workgroup's loads and stores take turns,
+// which is why it is 16 wavefronts with three pieces a thread (of 8 with five or four: 136 and 125 us).
+constexpr int kRowThreads = 1024;
+template <int kPer, int kHeld>
+__global__ void __launch_bounds__(kRowThreads, 4) gate_gradient_rows_kernel(const float* gate_up, const __half* dout, __half* grad, const __half* x, int64_t x_stride, int* exponents,
+                                                                         int64_t rows, int64_t inter, int64_t k) {
+    struct alignas(sizeof(__half) * kPer) Piece {
+        __half v[kPer];
+    };
+    struct alignas(kPer > 1 ? 16 : 4) Wide {
+        float v[kPer];
+    };
+    __shared__ float tops[2][kRowThreads / 64];
+    const int64_t pieces = inter / kPer;
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const float* from = gate_up + row * 2 * inter;
+        const __half* dh = dout + row * inter;
+        __half* to = grad + row * 2 * inter;
+        auto gradients = [&](int64_t c, float (&dg)[kPer], float (&du)[kPer]) {
+            const Wide gate = *reinterpret_cast<const Wide*>(from + c * kPer), up = *reinterpret_cast<const Wide*>(from + inter + c * kPer);
+            const Piece d = *reinterpret_cast<const Piece*>(dh + c * kPer);
+#pragma unroll
+            for (int e = 0; e < kPer; e++) gate_gradients(gate.v[e], up.v[e], __half2float(d.v[e]), dg[e], du[e]);
+        };
+        float dg[kHeld][kPer], du[kHeld][kPer], most = 0.f, most_x = 0.f;
+        auto look = [&](const float (&a)[kPer], const float (&b)[kPer]) {
+#pragma unroll
+            for (int e = 0; e < kPer; e++) most = larger_finite(larger_finite(most, a[e]), b[e]);
+        };
+#pragma unroll
+        for (int h = 0; h < kHeld; h++) {
+            const int64_t c = threadIdx.x + h * (int64_t)blockDim.x;
+            if (c < pieces) {
+                gradients(c, dg[h], du[h]);
+                look(dg[h], du[h]);
+            }
+        }
+        for (int64_t c = threadIdx.x + kHeld * (int64_t)blockDim.x; c < pieces; c += blockDim.x) {
+            float a[kPer], b[kPer];
+            gradients(c, a, b);
+            look(a, b);
+        }
+        for (int64_t i = threadIdx.x; i < k; i += blockDim.x) most_x = larger_finite(most_x, __half2float(x[row * x_stride + i]));
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            most = fmaxf(most, __shfl_xor(most, o));
+            most_x = fmaxf(most_x, __shfl_xor(most_x, o));
+        }
+        if ((threadIdx.x & 63) == 0) {
+            tops[0][threadIdx.x >> 6] = most;
+            tops[1][threadIdx.x >> 6] = most_x;
+        }
+        __syncthreads();
+        for (int w = 0; w < (int)blockDim.x >> 6; w++) {
+            most = fmaxf(most, tops[0][w]);
+            most_x = fmaxf(most_x, tops[1][w]);
+        }
+        const int e = exponent_above(most);
+        if (threadIdx.x == 0) {
+            exponents[row] = e;
+            exponents[rows + row] = e + exponent_above(most_x);
+        }
+        auto store = [&](int64_t c, const float (&a)[kPer], const float (&b)[kPer]) {
+            Piece g, u;
+#pragma unroll
+            for (int i = 0; i < kPer; i++) {
+                g.v[i] = __float2half(__builtin_amdgcn_ldexpf(a[i], -e));
+                u.v[i] = __float2half(__builtin_amdgcn_ldexpf(b[i], -e));
+            }
+            *reinterpret_cast<Piece*>(to + c * kPer) = g;
+            *reinterpret_cast<Piece*>(to + inter + c * kPer) = u;
+        };
+#pragma unroll
+        for (int h = 0; h < kHeld; h++) {
+            const int64_t c = threadIdx.x + h * (int64_t)blockDim.x;
+            if (c < pieces) store(c, dg[h], du[h]);
+        }
+        for (int64_t c = threadIdx.x + kHeld * (int64_t)blockDim.x; c < pieces; c += blockDim.x) {
+            float a[kPer], b[kPer];
+            gradients(c, a, b);
+            store(c, a, b);
+        }
+        __syncthreads();   // the next row's largest come where this one's are
+    }
+}
+
+// Rows of x times 2^(e_m - T), contiguous, and T behind the exponents.  Every workgroup looks for T by itself.  2048 x 3584 10 us.
+template <int kPer>
+__global__ void __launch_bounds__(256) scale_rows_kernel(const __half* x, int64_t x_stride, __half* out, int* exponents, int64_t rows, int64_t k) {
+    struct alignas(sizeof(__half) * kPer) Piece {
+        __half v[kPer];
+    };
+    __shared__ int tops[4];
+    int top = 2 * kNoExponent;
+    for (int64_t i = threadIdx.x; i < rows; i += 256) top = max(top, exponents[rows + i]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = max(top, __shfl_xor(top, o));
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+    __syncthreads();
+    top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+    if (blockIdx.x == 0 && threadIdx.x == 0) exponents[2 * rows] = top;
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const int by = exponents[row] - top;
+        for (int64_t i = (int64_t)threadIdx.x * kPer; i < k; i += 256 * kPer) {
+            Piece v = *reinterpret_cast<const Piece*>(x + row * x_stride + i);
+#pragma unroll
+            for (int e = 0; e < kPer; e++) v.v[e] = __float2half(__builtin_amdgcn_ldexpf(__half2float(v.v[e]), by));
+            *reinterpret_cast<Piece*>(out + row * k + i) = v;
+        }
+    }
+}
+
+// Both, for a product of every row and one of all rows.
+int gate_gradient_rows(const float* gate_up, const void* dout, void* grad, const void* x, int64_t x_stride, void* scaled_x, int* exponents, int64_t rows,
+                       int64_t inter, int64_t k, hipStream_t stream) {
+    auto aligned = [](std::initializer_list<const void*> all) {
+        uintptr_t bits = 0;
+        for (const void* p : all) bits |= reinterpret_cast<uintptr_t>(p);
+        return (bits & 15) == 0;
+    };
+    const bool pieces = inter % 8 == 0 && aligned({gate_up, dout, grad});
+    const int64_t many = pieces ? inter / 8 : inter;
+    const unsigned threads = (unsigned)std::min<int64_t>(kRowThreads, align_up(many, CKV_WAVE));
+    auto launch = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)std::min<int64_t>(rows, 1 << 22)), dim3(threads), 0, stream, gate_up, (const __half*)dout, (__half*)grad, (const __half*)x, x_stride, exponents, rows,
+                           inter, k);
+    };
+    if (pieces) launch(gate_gradient_rows_kernel<8, 3>);
+    else launch(gate_gradient_rows_kernel<1, 16>);
+    CKV_HIP_TRY(hipGetLastError());
+    if (!scaled_x) return CKV_OK;
+    const dim3 grid((unsigned)std::min<int64_t>(rows, 2048));
+    if (k % 8 == 0 && x_stride % 8 == 0 && aligned({x, scaled_x}))
+        hipLaunchKernelGGL((scale_rows_kernel<8>), grid, dim3(256), 0, stream, (const __half*)x, x_stride, (__half*)scaled_x, exponents, rows, k);
+    else hipLaunchKernelGGL((scale_rows_kernel<1>), grid, dim3(256), 0, stream, (const __half*)x, x_stride, (__half*)scaled_x, exponents, rows, k);
     CKV_HIP_TRY(hipGetLastError());
     return CKV_OK;
 }
@@ -356,7 +522,7 @@ int run_product(ProductParams& p, const DeviceInfo& di, void* workspace, int64_t
     }
     if (plan.shares > 1) {
         constexpr int kRows = 8;
-        hipLaunchKernelGGL((merge_kernel<T, kEpilogue>), dim3(plan.tiles_m * plan.tiles_n - plan.whole_tiles, plan.tile_m / kRows), dim3(256), 0, stream, p, plan.tile_m,
+        hipLaunchKernelGGL((merge_kernel<T, kEpilogue, kAlongKA>), dim3(plan.tiles_m * plan.tiles_n - plan.whole_tiles, plan.tile_m / kRows), dim3(256), 0, stream, p, plan.tile_m,
                            plan.tile_n, tiles ? 4 : 8, kRows);
         CKV_HIP_TRY(hipGetLastError());
     }
@@ -393,19 +559,38 @@ int run_forward(const void* x, const void* w, void* out, float* gate_up, int64_t
     return run_product<T, true, true, kGate>(p, di, workspace, bytes, stream);
 }
 
+// Scratch of a backward pass in front of its products': [dg du], and in float16 the exponents of its rows and x by them.
+struct Scratch {
+    int64_t exponents, x, products;   // where they begin
+    Scratch(int64_t rows, int64_t inter, int64_t k, int32_t dtype) {
+        exponents = align_up(rows * 2 * inter * elem_bytes(dtype), 256);
+        x = exponents + (dtype == CKV_F16 ? align_up((2 * rows + 1) * (int64_t)sizeof(int), 256) : 0);
+        products = x + (dtype == CKV_F16 ? align_up(rows * k * 2, 256) : 0);
+    }
+};
+
 template <typename T>
 int run_backward(const void* x, const void* w, const float* gate_up, const void* dout, void* dx, void* dw, int64_t rows, int64_t inter, int64_t k,
                  int64_t x_stride, char* workspace, int64_t bytes, const DeviceInfo& di, hipStream_t stream) {
-    const int64_t grad_bytes = align_up(rows * 2 * inter * (int64_t)sizeof(T), 256);
+    const Scratch at(rows, inter, k, Elem<T>::code);
     void* grad = workspace;
-    if (int rc = gate_gradient<T>(gate_up, dout, grad, rows, inter, stream)) return rc;
-    workspace += grad_bytes;
-    bytes -= grad_bytes;
+    int* exponents = nullptr;
+    if constexpr (std::is_same<T, __half>::value) {
+        exponents = (int*)(workspace + at.exponents);
+        if (int rc = gate_gradient_rows(gate_up, dout, grad, x, x_stride, dw ? workspace + at.x : nullptr, exponents, rows, inter, k, stream)) return rc;
+        x = workspace + at.x;
+        x_stride = k;
+    } else {
+        if (int rc = gate_gradient<T>(gate_up, dout, grad, rows, inter, stream)) return rc;
+    }
+    workspace += at.products;
+    bytes -= at.products;
     if (dx) {
         ProductParams p = {};
         p.a = Operand{grad, 2 * inter};
         p.b = Operand{w, k};
         p.out = dx;
+        p.exponents = exponents;
         p.M = rows;
         p.N = k;
         p.K = 2 * inter;
@@ -416,6 +601,7 @@ int run_backward(const void* x, const void* w, const float* gate_up, const void*
         p.a = Operand{grad, 2 * inter};
         p.b = Operand{x, x_stride};
         p.out = dw;
+        p.exponents = exponents ? exponents + 2 * rows : nullptr;
         p.M = 2 * inter;
         p.N = k;
         p.K = rows;
@@ -460,7 +646,7 @@ extern "C" int64_t ckv_gated_linear_bwd_workspace_bytes(int64_t rows, int64_t in
     DeviceInfo di;
     if (check_sizes(rows, inter, k, k, dtype) || rows == 0 || current_device_info(&di)) return 0;
     const int64_t dx = product_bytes(rows, k, 2 * inter, true, false, di.cus), dw = product_bytes(2 * inter, k, rows, false, false, di.cus);
-    return align_up(rows * 2 * inter * elem_bytes(dtype), 256) + std::max(dx, dw);
+    return Scratch(rows, inter, k, dtype).products + std::max(dx, dw);
 }
 
 extern "C" int ckv_gated_linear_bwd(const void* x, const void* w, const float* gate_up, const void* dout, void* dx, void* dw, int64_t rows,
@@ -479,7 +665,7 @@ extern "C" int ckv_gated_linear_bwd(const void* x, const void* w, const float* g
     if (!x || !w || !gate_up || !dout) return CKV_ERR_NULL;
     DeviceInfo di;
     if (int rc = current_device_info(&di)) return rc;
-    if (!workspace || workspace_bytes < align_up(rows * 2 * inter * elem_bytes(dtype), 256)) return CKV_ERR_WORKSPACE;
+    if (!workspace || workspace_bytes < Scratch(rows, inter, k, dtype).products) return CKV_ERR_WORKSPACE;
     char* ws = (char*)workspace;
     switch (dtype) {
         case CKV_F32: return run_backward<float>(x, w, gate_up, dout, dx, dw, rows, inter, k, x_stride, ws, workspace_bytes, di, stream);

@@ -3,6 +3,8 @@
 
 #include "ckv_common.h"
 
+#include <type_traits>
+
 namespace ckv {
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
@@ -16,6 +18,7 @@ struct ProductParams {
     Operand a, b;
     void* out;          // (M, N) contiguous, or the gated (M, N / 2)
     float* both;        // gated, optional: (M, N), gate and up columns; of these, not of numbers rounded to the operands' type, gradients are made
+    const int* exponents;    // optional, float16 and not gated: C is times 2 to that power; one for each of its rows where A lies along k, else one for all
     float* partial;     // sums of the shares, tile by tile: (tiles shared out, shares, tile rows, tile columns)
     int64_t M, N, K;
     int64_t k_share;    // steps of a share
@@ -25,6 +28,20 @@ struct ProductParams {
 };
 
 enum Epilogue { kStore, kGate };
+
+// What row m of C is times: a power of two, exact until the result is rounded to float16.  One beyond float32's normal numbers is the nearest of them:
+// whatever it meets is nothing in float16 or above its end either way.  One for other types.
+template <typename T, bool kAlongKA>
+__device__ inline float power_of(const ProductParams& p, int64_t m) {
+    if constexpr (std::is_same<T, __half>::value)
+        return p.exponents && m < p.M ? __int_as_float((min(max(p.exponents[kAlongKA ? m : 0], -126), 127) + 127) << 23) : 1.f;
+    else return 1.f;
+}
+template <typename T>
+__device__ inline float times_power(float v, float power) {
+    if constexpr (std::is_same<T, __half>::value) return v * power;
+    else return v;
+}
 
 // Workgroups go round the eight XCDs: each gets a stretch of the tiles, and behind those one of the shares.  Tiles are numbered in bands
 // kHigh tiles of M high, so that the tiles of a stretch that run at a time share operands in its L2.

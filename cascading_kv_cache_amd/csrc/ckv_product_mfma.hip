@@ -186,6 +186,9 @@ __global__ void __launch_bounds__(64 * kWavesM * kWavesN, kTileM == 256 || kDeep
     const int64_t m0 = (int64_t)tm * kTileM, n0 = (int64_t)tn * (kGated ? kTileN / 2 : kTileN);
     const int64_t k0 = share * p.k_share, steps = sums ? min(p.K - k0, p.k_share) : p.K;
     const uint32_t lds = lds_address(smem);
+    // One for all rows is asked for now and kept in a scalar register: a load in front of every 16 rows' results, of which a compute unit has eight
+    // tiles (2048 x 37888 x 3584), was 25 us of 490.
+    [[maybe_unused]] const float power = !kGated && !kAlongKA ? __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(power_of<T, kAlongKA>(p, 0)))) : 1.f;
 
     using SideA = Side<kTileM, kAlongKA, kWaves, kDeep>;
     using SideB = Side<kTileN, kAlongKB, kWaves, kDeep>;
@@ -347,7 +350,8 @@ __global__ void __launch_bounds__(64 * kWavesM * kWavesN, kTileM == 256 || kDeep
                 }
             }
         } else {
-            write(i, [&](int j, int r) { return acc[i][j][r]; }, p.out, p.N, 0);
+            const float by = kAlongKA ? power_of<T, kAlongKA>(p, mw + 16 * i + r16) : power;
+            write(i, [&](int j, int r) { return times_power<T>(acc[i][j][r], by); }, p.out, p.N, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
     }

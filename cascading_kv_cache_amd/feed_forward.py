@@ -72,8 +72,8 @@ def _gradients(ctx, dout):
 def gated_feed_forward(x, w_gate_up):
     """``silu(gate) * up`` of ``gate | up = x w_gate_up^T``: x ``(..., K)``, w_gate_up ``(2 I, K)``, one type of float32, float16 and
     bfloat16; returns ``(..., I)``.  Gradients go back to both (once: not a second time); the projections are kept for that in
-    float32, ``2 I`` elements a row; their gradients are rounded to the tensor type for the two products.  Works under graph capture; nothing is
-    kept between calls.  Recorded into a graph, a backward pass wants no eager graph of the same leaves alive: torch would have the recording
+    float32, ``2 I`` elements a row; their gradients are rounded to the tensor type for the two products (float16: times a power of two a row,
+    so that none of them is above its end, or below its beginning beside the row's others).  Works under graph capture; nothing is kept between calls.  Recorded into a graph, a backward pass wants no eager graph of the same leaves alive: torch would have the recording
     wait for it."""
     if w_gate_up.ndim != 2 or w_gate_up.size(0) % 2 or w_gate_up.size(0) == 0 or w_gate_up.size(1) == 0:
         raise ValueError(f"weights have shape {tuple(w_gate_up.shape)}; expected (2 * intermediate, hidden)")

@@ -387,7 +387,8 @@ int ckv_norm_rotate_bwd(const ckv_norm_rotate_args* args, void* stream);
  * throughout, rounded once (ckv_linear_rows with `gated` and ckv_gated_silu round the projections and the activation too).
  * `gate_up` float32 (rows, 2 inter), optional: the projections, as the backward pass takes them.  Everything but x
  * contiguous.  The backward pass writes dx (rows, k) and dw (2 inter, k), either of which may be NULL; it rounds the
- * gradients of the projections to the tensor dtype for its two products, whose sums are float32.  Sums are added up in a
+ * gradients of the projections to the tensor dtype for its two products, whose sums are float32; in float16 they are kept
+ * times a power of two a row, so that only dx and dw have to be inside its range.  Sums are added up in a
  * fixed order.  The workspace sizes are those of a call on the current device.
  * ---------------------------------------------------------------------------------------- */
 int64_t ckv_gated_linear_workspace_bytes(int64_t rows, int64_t inter, int64_t k, int32_t dtype);
