@@ -133,3 +133,29 @@ def test_float16_gradients_that_are_no_numbers():
         rows = torch.zeros(2 * i, dtype=torch.bool, device="cuda")
         rows[5] = rows[i + 5] = True
         assert not dw[rows].isfinite().any() and not beyond(dw[~rows], tuple(t[~rows] for t in exact(x, w, torch.float16, dh)["dw"]))
+
+
+# One row: an element of dW is one product, so what its two factors were rounded by stands in it undiluted.
+ONE = (1, 64, 4096)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_projections_are_kept_in_float32(dtype):
+    x, w, dh = inputs(*ONE, dtype, "cuda", seed=4)
+    check(x, w, dh.to(dtype), "one row")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_the_limit_tells_projections_of_16_bits(dtype):
+    """The operator restated on the CPU: as it is, and with projections rounded to the tensor type."""
+    x, w, dh = inputs(*ONE, dtype, "cpu", seed=4)
+    dh = dh.to(dtype)
+    value = exact(x, w, dtype, dh)["dw"]
+    for rounded in (False, True):
+        proj = x.float() @ w.float().T
+        g, u = (proj.to(dtype).float() if rounded else proj).chunk(2, -1)
+        s = torch.sigmoid(g)
+        d = torch.cat((dh.float() * u * s * (1 + g * (1 - s)), dh.float() * g * s), -1).to(dtype).float()
+        many = beyond((d.T @ x.float()).to(dtype), value)
+        assert (many > 100) if rounded else many == 0
