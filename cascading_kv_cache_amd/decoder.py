@@ -21,7 +21,7 @@ from torch import nn
 from .cascading_cache import CascadingKVCache
 from .feed_forward import gated_feed_forward
 from .latency import ProjectedCascadeAttention
-from .row_products import followed as _followed, gated_silu, library_orders, own_methods, plain, product_settings, row_linear
+from .row_products import followed as _followed, followed_beyond_gradients, gated_silu, library_orders, own_methods, plain, product_settings, row_linear
 from .sampling import sample_tokens
 
 
@@ -88,7 +88,7 @@ class GatedMLP(nn.Module):
     def forward(self, x):
         if self._w_gate_up is None:
             return self.down_proj(nn.functional.silu(self.gate_proj(x)) * self.up_proj(x))
-        if self.one_launch and not torch.is_autocast_enabled():
+        if self.one_launch and not torch.is_autocast_enabled() and not followed_beyond_gradients(x):
             return self.down_proj(gated_feed_forward(x, self._w_gate_up))
         return self.down_proj(gated_silu(nn.functional.linear(x, self._w_gate_up)))
 

@@ -12,6 +12,7 @@ import torch
 from . import _abi
 from .cascading_cache import _require_device, on_device, raw_stream
 from .norm_rotate import once
+from .row_products import refuse_followers
 
 
 def _scratch(nbytes, device):
@@ -55,6 +56,7 @@ class _GatedFeedForward(torch.autograd.Function):
 
 def _gradients(ctx, dout):
     x, w, gate_up = ctx.saved_tensors
+    refuse_followers("gated_feed_forward's backward pass", dout)
     rows, k = x.shape
     inter = w.size(0) // 2
     lib, code = _abi.lib(), _abi.dtype_code(x.dtype)
@@ -71,10 +73,12 @@ def _gradients(ctx, dout):
 
 def gated_feed_forward(x, w_gate_up):
     """``silu(gate) * up`` of ``gate | up = x w_gate_up^T``: x ``(..., K)``, w_gate_up ``(2 I, K)``, one type of float32, float16 and
-    bfloat16; returns ``(..., I)``.  Gradients go back to both (once: not a second time); the projections are kept for that in
+    bfloat16; returns ``(..., I)``.  Gradients go back to both (once: not a second time, and not by forward mode, torch.func's transforms or a
+    trace, which are refused); the projections are kept for that in
     float32, ``2 I`` elements a row; their gradients are rounded to the tensor type for the two products (float16: times a power of two a row,
     so that none of them is above its end, or below its beginning beside the row's others).  Works under graph capture; nothing is kept between calls.  Recorded into a graph, a backward pass wants no eager graph of the same leaves alive: torch would have the recording
     wait for it."""
+    refuse_followers("gated_feed_forward", x, w_gate_up)
     if w_gate_up.ndim != 2 or w_gate_up.size(0) % 2 or w_gate_up.size(0) == 0 or w_gate_up.size(1) == 0:
         raise ValueError(f"weights have shape {tuple(w_gate_up.shape)}; expected (2 * intermediate, hidden)")
     if x.ndim == 0 or x.size(-1) != w_gate_up.size(1):

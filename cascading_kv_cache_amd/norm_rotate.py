@@ -14,6 +14,7 @@ import torch
 
 from . import _abi
 from .cascading_cache import _require_device, on_device, raw_stream
+from .row_products import refuse_followers
 
 MAX_HEAD_DIM = 256
 
@@ -120,6 +121,7 @@ class _NormRotate(torch.autograd.Function):
 
 def _gradients(ctx, *grads):
     q, k, q_weight, k_weight, positions, inv_freq = ctx.saved_tensors
+    refuse_followers("norm_rotate's backward pass", *grads)
     # a gradient may be an expanded scalar, or in an order of its own
     q_grad, k_grad = (g if g.stride(-1) == 1 or g.size(-1) == 1 else g.contiguous() for g in grads)
     dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
@@ -193,9 +195,10 @@ def norm_rotate(q, k, q_weight=None, k_weight=None, positions=None, inv_freq=Non
     q ``(B, H, n, D)`` and k ``(B, KVH, n, D)``, float32, float16 or bfloat16, any strides.  ``q_weight``, ``k_weight`` ``(D,)``, dtype of q: the
     weights of the norm, or None for no norm.  ``positions`` int64 ``(n,)`` or ``(B, n)`` and ``inv_freq`` float32 ``(R / 2,)``: the first
     R <= D dims are rotated, dim j with dim j + R / 2 by ``position * inv_freq[j]``; or None for no rotation.  Gradients go back to q, k
-    and the weights (once: not a second time).  Works under graph capture; nothing of the tensors is kept between calls.  Recorded into a graph, a
+    and the weights (once: not a second time, and not by forward mode, torch.func's transforms or a trace, which are refused).  Works under graph capture; nothing of the tensors is kept between calls.  Recorded into a graph, a
     backward pass wants no eager graph of the same leaves alive: torch would have the recording wait for it."""
     tensors = q, k, q_weight, k_weight, positions, inv_freq
+    refuse_followers("norm_rotate", *tensors)
     followed = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors[:4])
     if out is not None:
         if followed:

@@ -7,9 +7,11 @@ torch's product of the same sizes (:func:`library_orders` tries them, once, when
 stays everywhere else.
 """
 import math
+import sys
 
 import torch
 from torch import nn
+from torch.utils._python_dispatch import _get_current_dispatch_mode_stack
 
 from . import _abi
 from .cascading_cache import on_device, raw_stream
@@ -25,11 +27,45 @@ _dispatch_modes = getattr(torch._C, "_len_torch_dispatch_stack", lambda: 1)
 _functorch_levels = getattr(getattr(torch._C, "_functorch", None), "peek_interpreter_stack", lambda: 1)
 
 
-def followed(x) -> bool:
-    """May anybody follow torch's operations on ``x``: gradients of either mode, vmap, tracing, a tensor subclass, a mode?"""
-    return (type(x) is not torch.Tensor or torch.is_grad_enabled() or x.requires_grad or _function_modes() != 0 or _dispatch_modes() != 0
+def followed_beyond_gradients(x) -> bool:
+    """May anybody follow torch's operations on ``x`` other than for its gradients: forward mode, vmap, tracing, a tensor subclass, a mode?"""
+    return (type(x) is not torch.Tensor or _function_modes() != 0 or _dispatch_modes() != 0
             or getattr(torch.autograd.forward_ad, "_current_level", 0) >= 0 or _functorch_levels() is not None
             or torch.jit.is_tracing() or torch.compiler.is_compiling())
+
+
+def followed(x) -> bool:
+    """May anybody follow torch's operations on ``x``: gradients of either mode, vmap, tracing, a tensor subclass, a mode?"""
+    return torch.is_grad_enabled() or x.requires_grad or followed_beyond_gradients(x)
+
+
+_wrapped = getattr(getattr(torch._C, "_functorch", None), "is_functorch_wrapped_tensor", lambda t: True)
+_no_dispatch = getattr(torch._C, "_disabled_torch_dispatch_impl", None)
+_tracing = getattr(torch._C, "_is_tracing", torch.jit.is_tracing)
+_forward_ad = torch.autograd.forward_ad
+_OWN_TYPES = frozenset((torch.Tensor, nn.Parameter, type(None)))
+
+
+def _is_dual(t) -> bool:
+    return t.is_floating_point() and _forward_ad.unpack_dual(t).tangent is not None
+
+
+def refuse_followers(what, *tensors):
+    """Raises where somebody who follows torch's operations on ``tensors`` (or None) would lose their way, since ``what`` reads and writes them by address
+    and has no rule for them: a tangent, a batch, a trace, a subclass whose data are elsewhere.  Gradients are ``what``'s own affair."""
+    for t in tensors:
+        if type(t) not in _OWN_TYPES and type(t).__torch_dispatch__ is not _no_dispatch:
+            raise TypeError(f"{what} takes torch's own tensors, not {type(t).__name__}")
+    if _dispatch_modes() == 0 and _functorch_levels() is None and getattr(_forward_ad, "_current_level", 0) < 0 and not _tracing():
+        return
+    proxies = sys.modules.get("torch.fx.experimental.proxy_tensor")   # not loaded: nobody traces with it
+    if _tracing() or (proxies is not None and any(isinstance(m, proxies.ProxyTorchDispatchMode) for m in _get_current_dispatch_mode_stack())):
+        raise RuntimeError(f"{what} cannot be traced: of a launch by address a trace would hold nothing")
+    there = [t for t in tensors if t is not None]
+    if _functorch_levels() is not None and any(map(_wrapped, there)):
+        raise RuntimeError(f"{what} has no rule for torch.func's transforms")
+    if getattr(_forward_ad, "_current_level", 0) >= 0 and any(map(_is_dual, there)):
+        raise RuntimeError(f"{what} has no derivative of forward mode")
 
 
 #: kind of module: (name, method) of what calling one runs

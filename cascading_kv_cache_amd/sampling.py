@@ -11,6 +11,7 @@ import torch
 
 from . import _abi
 from .cascading_cache import _require_device, on_device, raw_stream
+from .row_products import refuse_followers
 
 MAX_VOCAB = (1 << 19) - 1
 
@@ -29,8 +30,9 @@ def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0
     least ``min_p`` of the first one; the first one always.  The token is the first whose running kept weight exceeds the row's number times
     all of it, ``logprobs`` the logarithm of its share.  Every setting is a number or a tensor with one a row (float32, top_k int64) on the
     logits' device; those are not checked, what lies outside their ranges means the nearest in it.  ``temperature`` 0: the largest logit,
-    whatever the number.  Logits of NaN and minus infinity are no tokens; a row without any gives -1 and NaN.  No gradients.  Works under graph
-    capture; nothing is kept between calls."""
+    whatever the number.  Logits of NaN and minus infinity are no tokens; a row without any gives -1 and NaN.  No gradients; traces and torch.func's
+    transforms are refused.  Works under graph capture; nothing is kept between calls."""
+    refuse_followers("sample_tokens", logits, uniforms, *(t for t in (temperature, top_k, top_p, min_p) if isinstance(t, torch.Tensor)))
     if logits.ndim != 2 or uniforms.shape != logits.shape[:1]:
         raise ValueError(f"logits {tuple(logits.shape)} and random numbers {tuple(uniforms.shape)}; expected (rows, vocab) and (rows,)")
     rows, vocab = logits.shape
