@@ -65,6 +65,20 @@ class RMSNorm(nn.Module):
         return self.weight * xf.to(x.dtype)
 
 
+class _Joined(torch.autograd.Function):
+    """A buffer whose parts two parameters are views of, as what is made of those: its gradient goes back to them by its halves."""
+
+    @staticmethod
+    def forward(ctx, buffer, first, second):
+        ctx.save_for_backward(first, second)
+        return buffer.detach()
+
+    @staticmethod
+    def backward(ctx, grad):
+        first, second = ctx.saved_tensors   # torch's own check that nobody has written to them since
+        return None, *grad.split((first.size(0), second.size(0)))
+
+
 class GatedMLP(nn.Module):
     def __init__(self, cfg, dtype, device):
         super().__init__()
@@ -85,12 +99,31 @@ class GatedMLP(nn.Module):
             self.gate_proj.weight.data, self.up_proj.weight.data = w[:n], w[n:]
             self._w_gate_up = w
 
+    def _shared(self) -> bool:
+        """Are both weights where the buffer has them, and not in storage of their own since: copied, moved, replaced?"""
+        gate, up, both = self.gate_proj.weight, self.up_proj.weight, self._w_gate_up
+        try:
+            return gate.dtype == both.dtype and gate.data_ptr() == both.data_ptr() and up.data_ptr() == both.data_ptr() + gate.nbytes
+        except RuntimeError:   # of a transform's tensor there is no address
+            return False
+
+    def _weights(self):
+        """Both projections' weights in one: the buffer, or where somebody follows the parameters, what they can be followed through."""
+        gate, up, both = self.gate_proj.weight, self.up_proj.weight, self._w_gate_up
+        if followed_beyond_gradients(both):
+            return torch.cat((gate, up))
+        return _Joined.apply(both, gate, up) if torch.is_grad_enabled() and (gate.requires_grad or up.requires_grad) else both
+
     def forward(self, x):
+        if self._w_gate_up is not None and (torch.is_grad_enabled() or followed_beyond_gradients(x)) and not self._shared():
+            if type(self.gate_proj.weight) is type(self.up_proj.weight) is nn.Parameter:
+                self._w_gate_up = None   # for good: what they learn from here on, the buffer would not
+            return self.down_proj(nn.functional.silu(self.gate_proj(x)) * self.up_proj(x))
         if self._w_gate_up is None:
             return self.down_proj(nn.functional.silu(self.gate_proj(x)) * self.up_proj(x))
         if self.one_launch and not torch.is_autocast_enabled() and not followed_beyond_gradients(x):
-            return self.down_proj(gated_feed_forward(x, self._w_gate_up))
-        return self.down_proj(gated_silu(nn.functional.linear(x, self._w_gate_up)))
+            return self.down_proj(gated_feed_forward(x, self._weights()))
+        return self.down_proj(gated_silu(nn.functional.linear(x, self._weights())))
 
 
 own_methods(RMSNorm)
