@@ -188,9 +188,25 @@ def _check_out(out, q, k):
             raise ValueError("out is expanded: its rows are not its own")
 
 
+def _written(out, tensors):
+    """What a call that writes ``out`` asks of where its tensors lie, and its announcement to whoever has saved one of them."""
+    if out[0].numel():
+        at = [None if t is None else t.data_ptr() for t in tensors]
+        for i, t in enumerate(out):
+            own, here = tensors[i], t.data_ptr()
+            if here in at[:i] + at[i + 1:] or here == out[1 - i].data_ptr():
+                raise ValueError("out lies where something else is: the queries' may be the queries, the keys' the keys")
+            if here == at[i] and any(n > 1 and a != b for n, a, b in zip(t.shape, t.stride(), own.stride())):
+                raise ValueError("out begins where its input does, in another order")
+    for t in out:
+        if not t.is_inference():   # those have no versions
+            torch.autograd.graph.increment_version(t)
+
+
 def norm_rotate(q, k, q_weight=None, k_weight=None, positions=None, inv_freq=None, eps=1e-6, out=None):
     """``(q, k)`` with every head's row normed and rotated, contiguous, or written to ``out``: two tensors of their shapes, apart from the inputs
-    or the inputs themselves (a decoding step has no other use for them); such a call has no gradients.
+    and each other, or the inputs themselves (a decoding step has no other use for them); such a call has no gradients, and counts as one of torch's
+    operations in place: who has saved one of the two for a backward pass is told.
 
     q ``(B, H, n, D)`` and k ``(B, KVH, n, D)``, float32, float16 or bfloat16, any strides.  ``q_weight``, ``k_weight`` ``(D,)``, dtype of q: the
     weights of the norm, or None for no norm.  ``positions`` int64 ``(n,)`` or ``(B, n)`` and ``inv_freq`` float32 ``(R / 2,)``: the first
@@ -201,9 +217,10 @@ def norm_rotate(q, k, q_weight=None, k_weight=None, positions=None, inv_freq=Non
     refuse_followers("norm_rotate", *tensors)
     followed = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors[:4])
     if out is not None:
-        if followed:
-            raise ValueError("no gradients go through out")
         out = tuple(out)
+        if followed or (torch.is_grad_enabled() and any(t.requires_grad for t in out)):
+            raise ValueError("no gradients go through out")
+        refuse_followers("norm_rotate", *out)
     key = [(t.shape, t.stride(), t.dtype, t.device) if t is not None else None for t in (tensors if out is None else tensors + out)]
     key = tuple(key)
     layout = _LAYOUTS.get(key)
@@ -222,4 +239,6 @@ def norm_rotate(q, k, q_weight=None, k_weight=None, positions=None, inv_freq=Non
             _LAYOUTS[key] = layout
     if followed:
         return _NormRotate.apply(layout, float(eps), q, k, q_weight, k_weight, positions, inv_freq)
+    if out is not None:
+        _written(out, tensors)
     return _forward(layout, q, k, q_weight, k_weight, positions, inv_freq, float(eps), out)
