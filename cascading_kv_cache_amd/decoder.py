@@ -128,7 +128,6 @@ class GatedMLP(nn.Module):
 
 own_methods(RMSNorm)
 own_methods(GatedMLP)
-own_methods(ProjectedCascadeAttention, "forward_cascade", "qkv", "_attend", "_split_qkv")
 
 
 class DecoderLayer(nn.Module):

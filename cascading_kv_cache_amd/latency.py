@@ -22,6 +22,7 @@ from torch import nn
 from .cascade_attention import CascadeAttention
 from .cascading_cache import CascadingKVCache
 from .norm_rotate import norm_rotate
+from .row_products import followed, own_methods, plain
 
 
 class ProjectedCascadeAttention(CascadeAttention):
@@ -73,8 +74,8 @@ class ProjectedCascadeAttention(CascadeAttention):
 
     def _attend(self, query_states, key_states, value_states, past_key_value, homogeneous_heads, do_og_pos):
         if self.qk_norm:
-            # the rows of a fused product are this call's alone: normed where they are, beside the values
-            alone = self._w_qkv is not None and type(self).qkv is ProjectedCascadeAttention.qkv and not torch.is_grad_enabled()
+            # the rows of a fused product, which nobody else's method has made or seen, are this call's alone: normed where they are, beside the values
+            alone = self._w_qkv is not None and not followed(query_states) and plain(self, ProjectedCascadeAttention)
             query_states, key_states = norm_rotate(query_states, key_states, self.q_norm_weight, self.k_norm_weight, eps=self.norm_eps,
                                                    out=(query_states, key_states) if alone else None)
             if not alone:
@@ -88,6 +89,9 @@ class ProjectedCascadeAttention(CascadeAttention):
         n_q, n_kv = self.q_proj.weight.size(0), self.k_proj.weight.size(0)
         q, k, v = rows.split((n_q, n_kv, n_kv), dim=-1)
         return q.view(*size).transpose(1, 2), k.view(*kv_size).transpose(1, 2), v.view(*kv_size).transpose(1, 2)
+
+
+own_methods(ProjectedCascadeAttention, "forward_cascade", "qkv", "_attend", "_split_qkv")
 
 
 def stream_through(layer, cache, hidden, stride):

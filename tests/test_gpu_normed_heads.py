@@ -1,0 +1,67 @@
+"""Normed heads of the attention layer: whose tensors they are written over."""
+import pytest
+import torch
+
+from cascading_kv_cache_amd.cascading_cache import CascadingKVCache
+from cascading_kv_cache_amd.latency import ProjectedCascadeAttention
+
+pytestmark = pytest.mark.gpu
+
+SIZES = dict(hidden_size=256, num_heads=4, num_key_value_heads=2, head_dim=128)
+
+
+def layer(kind=ProjectedCascadeAttention, dtype=torch.bfloat16, fused=True):
+    torch.manual_seed(0)
+    made = kind(**SIZES, dtype=dtype, device="cuda", qk_norm=True)
+    with torch.no_grad():
+        for w in (made.q_norm_weight, made.k_norm_weight):
+            w.copy_(1 + 0.3 * torch.randn(128, device="cuda"))
+    if fused:
+        made.fuse_projections()
+    return made
+
+
+def cache(dtype=torch.bfloat16):
+    return CascadingKVCache(32, num_sink_tokens=4, max_batch_size=2, heads=2, dim=128, max_seq_len=64, dtype=dtype, device="cuda", layers=1, verbose=False)
+
+
+def run(made, x, dtype=torch.bfloat16):
+    held = cache(dtype)
+    with torch.no_grad():
+        return made(x, use_cache=True, past_key_value=held)[0], held
+
+
+class Kept(ProjectedCascadeAttention):
+    """Keeps what its projections made."""
+
+    def qkv(self, x, size, kv_size):
+        self.kept = super().qkv(x, size, kv_size)
+        return self.kept
+
+
+class KeptRows(ProjectedCascadeAttention):
+
+    def _split_qkv(self, rows, *sizes):
+        self.kept = super()._split_qkv(rows, *sizes)
+        return self.kept
+
+
+@pytest.mark.parametrize("who", ["class", "class of rows", "object", "object's rows", "hook"])
+def test_tensors_of_somebody_elses_method_stay_as_they_are(who):
+    x = torch.randn(2, 9, 256, device="cuda").bfloat16()
+    want, want_cache = run(layer(), x)
+    made = layer({"class": Kept, "class of rows": KeptRows}.get(who, ProjectedCascadeAttention))
+    kept = []
+    if who == "object":
+        made.qkv = lambda *args: kept.append(ProjectedCascadeAttention.qkv(made, *args)) or kept[0]
+    elif who == "object's rows":
+        made._split_qkv = lambda *args: kept.append(ProjectedCascadeAttention._split_qkv(made, *args)) or kept[0]
+    elif who == "hook":
+        made.register_forward_hook(lambda module, args, result: None)
+    got, got_cache = run(made, x)
+    assert torch.equal(got, want) and torch.equal(got_cache.key_cache[0], want_cache.key_cache[0])
+    if who != "hook":
+        with torch.no_grad():
+            rows = torch.nn.functional.linear(x, made._w_qkv)
+        kept = made.kept if "class" in who else kept[0]
+        assert torch.equal(torch.cat([t.transpose(1, 2).flatten(2) for t in kept], -1), rows)
