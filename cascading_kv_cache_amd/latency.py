@@ -76,7 +76,9 @@ class ProjectedCascadeAttention(CascadeAttention):
         if self.qk_norm:
             # the rows of a fused product, which nobody else's method has made or seen, are this call's alone: normed where they are, beside the values
             alone = self._w_qkv is not None and not followed(query_states) and plain(self, ProjectedCascadeAttention)
-            query_states, key_states = norm_rotate(query_states, key_states, self.q_norm_weight, self.k_norm_weight, eps=self.norm_eps,
+            # autocast's projections come in another type than the layer's; the norm is float32 inside either way
+            weights = (w.to(query_states.dtype) for w in (self.q_norm_weight, self.k_norm_weight))
+            query_states, key_states = norm_rotate(query_states, key_states, *weights, eps=self.norm_eps,
                                                    out=(query_states, key_states) if alone else None)
             if not alone:
                 value_states = value_states.contiguous()   # as the keys lie

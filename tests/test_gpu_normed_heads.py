@@ -65,3 +65,24 @@ def test_tensors_of_somebody_elses_method_stay_as_they_are(who):
             rows = torch.nn.functional.linear(x, made._w_qkv)
         kept = made.kept if "class" in who else kept[0]
         assert torch.equal(torch.cat([t.transpose(1, 2).flatten(2) for t in kept], -1), rows)
+
+
+@pytest.mark.parametrize("fused", [False, True])
+@pytest.mark.parametrize("own", [torch.float32, torch.bfloat16])
+def test_under_autocast(own, fused):
+    """The cache holds the projections' keys, normed: the weight is rounded to autocast's type, and the product, by half a step each."""
+    made = layer(dtype=own, fused=fused)
+    x = torch.randn(2, 9, 256, device="cuda").to(own)
+    with torch.autocast("cuda", torch.float16):
+        out, held = run(made, x, torch.float16)
+    assert out.dtype == torch.float16 and out.isfinite().all()
+    with torch.no_grad():
+        weight = torch.cat([m.weight for m in (made.q_proj, made.k_proj, made.v_proj)]) if fused else made.k_proj.weight
+        k = torch.nn.functional.linear(x.half(), weight.half())[..., 512:768] if fused else torch.nn.functional.linear(x.half(), weight.half())
+    k = k.unflatten(-1, (2, 128)).transpose(1, 2).double()
+    want = k * torch.rsqrt(k.pow(2).mean(-1, keepdim=True) + made.norm_eps) * made.k_norm_weight.double()
+    kept = torch.cat((held.sink_keys[0], held.key_cache[0][:, :, :5]), 2).double()
+    assert ((kept - want).abs() <= 2.01 * 2.0 ** -11 * want.abs() + 2.0 ** -24).all()
+    with torch.no_grad():     # and a single token
+        with torch.autocast("cuda", torch.float16):
+            assert made(x[:, :1], use_cache=True, past_key_value=held)[0].isfinite().all()
