@@ -678,7 +678,9 @@ __device__ inline float top_of(float m) {
 
 // Is this the last of the row's workgroups to arrive?  Then what the others wrote before is there to be read.  Everything that goes from one to
 // another is written by atomics of the device's scope and read by such loads, past the caches of an XCD, so their end is all there is to wait
-// for: a fence would have every wavefront write back and invalidate the L2.
+// for: a fence would have every wavefront write back and invalidate the L2.  That end is what vmcnt counts, of the stores and atomics of every
+// wavefront in front of the barrier, and what a release would wait for too; its write-back of the L2 is for plain stores, of which there are none here
+// (with release and acquire on the one addition 33 x 152064 takes 50 us instead of 46).
 __device__ inline bool last_to_arrive(uint32_t* arrived, int slices, uint32_t* shared) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
