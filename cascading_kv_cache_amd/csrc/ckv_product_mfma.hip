@@ -413,10 +413,10 @@ constexpr Kind kKinds[] = {{256, 256, 1, 1, 0.47, 0.74, 8.5, 0}, {128, 128, 1, 2
 
 // Tiles fill the compute units round by round; those of the last round may be shared out along k, which costs their sums a trip to memory (4
 // TB/s both ways, 3 us the launch that adds them up).  What decides between the kinds is how near the tiles come to full rounds.  128
-// rows, 128 high and 96, 128, 160, 192, 224 and 256 wide, each in the best number of shares: 22016 x 4096 41, 46, 51, 47, 49 and 49 us; 28672 x 4096 59, 49,
-// 55, 59, 61 and 62; 37888 x 3584 more than 69, 68, 58, 61, 63 and 68; 51200 x 5120 more than 124 twice, 124, 116, 109 and 114.  More rows, 256 high
-// and 128, 160 and (32 steps a stage) 256 wide: 256 x 28672 x 4096 61, 66 and 96; 512 x 37888 x 3584 146, 115 and 173; 1024 x 34816 x 5120 336, 303 and
-// 371; 4096 x 28672 x 4096 733, 721 and 713.
+// rows, 128 high and 96, 128, 160, 192, 224 and 256 wide, each in the best number of shares: 22016 x 4096 43, 46, 51, 47, 48 and 49 us; 28672 x 4096 59, 49,
+// 54, 59, 61 and 61; 37888 x 3584 75, 68, 59, 62, 64 and 68; 51200 x 5120 137, 133, 123, 113, 109 and 113.  More rows, 256 high
+// and 128, 160 and (32 steps a stage) 256 wide: 256 x 28672 x 4096 62, 66 and 91; 512 x 37888 x 3584 146, 114 and 171; 1024 x 34816 x 5120 340, 307 and
+// 376; 4096 x 28672 x 4096 744, 722 and 719.  Over 24 to 4096 rows of ten layers the rule is 0.7 % behind the best kind.
 TilePlan plan_tiles(int64_t M, int64_t N, int64_t K, bool a_along_k, bool gated, int cus) {
     TilePlan best = {};
     double best_us = 0;

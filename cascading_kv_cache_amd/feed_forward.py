@@ -76,7 +76,9 @@ def gated_feed_forward(x, w_gate_up):
     bfloat16; returns ``(..., I)``.  Gradients go back to both (once: not a second time, and not by forward mode, torch.func's transforms or a
     trace, which are refused); the projections are kept for that in
     float32, ``2 I`` elements a row; their gradients are rounded to the tensor type for the two products (float16: times a power of two a row,
-    so that none of them is above its end, or below its beginning beside the row's others).  Works under graph capture; nothing is kept between calls.  Recorded into a graph, a backward pass wants no eager graph of the same leaves alive: torch would have the recording
+    so that none of them is above its end, or below its beginning beside the row's others).  In 16 bits, sizes, strides
+    and addresses of whole eight elements are what it is fast for; others are multiplied on float32's instructions, some ten times slower.  Works under graph
+    capture; nothing is kept between calls.  Recorded into a graph, a backward pass wants no eager graph of the same leaves alive: torch would have the recording
     wait for it."""
     refuse_followers("gated_feed_forward", x, w_gate_up)
     if w_gate_up.ndim != 2 or w_gate_up.size(0) % 2 or w_gate_up.size(0) == 0 or w_gate_up.size(1) == 0:
