@@ -311,13 +311,14 @@ __device__ inline float larger_finite(float m, float v) {
     return v < __builtin_huge_valf() ? fmaxf(m, v) : m;   // infinities and NaN stay what they are at any scale
 }
 
-// A workgroup a row: the row's gradients stay in registers (kHeld pieces a thread; what is behind is worked out twice) until its largest is known.
+// A workgroup a row, or for short rows 2^lanes_log of a wavefront's lanes: the row's gradients stay in registers (kHeld pieces a thread; what is behind is worked out twice) until its largest is known.
 // exponents: e of every row, then e and the exponent of x's row together.  2048 x 18944 117 us, 4.7 TB/s: a workgroup's loads and stores take turns,
-// which is why it is 16 wavefronts with three pieces a thread (of 8 with five or four: 136 and 125 us).
+// which is why it is 16 wavefronts with three pieces a thread (of 8 with five or four: 136 and 125 us).  10^6 rows of 128: 340 us (the kernel
+// of the other types, which does not look at rows, 325); 870 by a wavefront a row.
 constexpr int kRowThreads = 1024;
-template <int kPer, int kHeld>
+template <int kPer, int kHeld, bool kShort>
 __global__ void __launch_bounds__(kRowThreads, 4) gate_gradient_rows_kernel(const float* gate_up, const __half* dout, __half* grad, const __half* x, int64_t x_stride, int* exponents,
-                                                                         int64_t rows, int64_t inter, int64_t k) {
+                                                                         int64_t rows, int64_t inter, int64_t k, int lanes_log) {
     struct alignas(sizeof(__half) * kPer) Piece {
         __half v[kPer];
     };
@@ -326,7 +327,10 @@ __global__ void __launch_bounds__(kRowThreads, 4) gate_gradient_rows_kernel(cons
     };
     __shared__ float tops[2][kRowThreads / 64];
     const int64_t pieces = inter / kPer;
-    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    const int many = kShort ? 1 << lanes_log : (int)blockDim.x, me = threadIdx.x & (kShort ? many - 1 : ~0);   // threads of a row
+    const int here = kShort ? (int)blockDim.x >> lanes_log : 1;   // rows of a workgroup
+    const int64_t first = (int64_t)blockIdx.x * here + (kShort ? threadIdx.x >> lanes_log : 0);
+    for (int64_t row = first; row < rows; row += (int64_t)gridDim.x * here) {   // the lanes of a row go together
         const float* from = gate_up + row * 2 * inter;
         const __half* dh = dout + row * inter;
         __half* to = grad + row * 2 * inter;
@@ -343,34 +347,35 @@ __global__ void __launch_bounds__(kRowThreads, 4) gate_gradient_rows_kernel(cons
         };
 #pragma unroll
         for (int h = 0; h < kHeld; h++) {
-            const int64_t c = threadIdx.x + h * (int64_t)blockDim.x;
+            const int64_t c = me + h * (int64_t)many;
             if (c < pieces) {
                 gradients(c, dg[h], du[h]);
                 look(dg[h], du[h]);
             }
         }
-        for (int64_t c = threadIdx.x + kHeld * (int64_t)blockDim.x; c < pieces; c += blockDim.x) {
+        for (int64_t c = me + kHeld * (int64_t)many; c < pieces; c += many) {
             float a[kPer], b[kPer];
             gradients(c, a, b);
             look(a, b);
         }
-        for (int64_t i = threadIdx.x; i < k; i += blockDim.x) most_x = larger_finite(most_x, __half2float(x[row * x_stride + i]));
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
+        for (int64_t i = me; i < k; i += many) most_x = larger_finite(most_x, __half2float(x[row * x_stride + i]));
+        for (int o = (kShort ? many : CKV_WAVE) >> 1; o > 0; o >>= 1) {
             most = fmaxf(most, __shfl_xor(most, o));
             most_x = fmaxf(most_x, __shfl_xor(most_x, o));
         }
-        if ((threadIdx.x & 63) == 0) {
-            tops[0][threadIdx.x >> 6] = most;
-            tops[1][threadIdx.x >> 6] = most_x;
-        }
-        __syncthreads();
-        for (int w = 0; w < (int)blockDim.x >> 6; w++) {
-            most = fmaxf(most, tops[0][w]);
-            most_x = fmaxf(most_x, tops[1][w]);
+        if constexpr (!kShort) {
+            if ((threadIdx.x & 63) == 0) {
+                tops[0][threadIdx.x >> 6] = most;
+                tops[1][threadIdx.x >> 6] = most_x;
+            }
+            __syncthreads();
+            for (int w = 0; w < (int)blockDim.x >> 6; w++) {
+                most = fmaxf(most, tops[0][w]);
+                most_x = fmaxf(most_x, tops[1][w]);
+            }
         }
         const int e = exponent_above(most);
-        if (threadIdx.x == 0) {
+        if (me == 0) {
             exponents[row] = e;
             exponents[rows + row] = e + exponent_above(most_x);
         }
@@ -386,41 +391,45 @@ __global__ void __launch_bounds__(kRowThreads, 4) gate_gradient_rows_kernel(cons
         };
 #pragma unroll
         for (int h = 0; h < kHeld; h++) {
-            const int64_t c = threadIdx.x + h * (int64_t)blockDim.x;
+            const int64_t c = me + h * (int64_t)many;
             if (c < pieces) store(c, dg[h], du[h]);
         }
-        for (int64_t c = threadIdx.x + kHeld * (int64_t)blockDim.x; c < pieces; c += blockDim.x) {
+        for (int64_t c = me + kHeld * (int64_t)many; c < pieces; c += many) {
             float a[kPer], b[kPer];
             gradients(c, a, b);
             store(c, a, b);
         }
-        __syncthreads();   // the next row's largest come where this one's are
+        if constexpr (!kShort) __syncthreads();   // the next row's largest come where this one's are
     }
 }
 
-// Rows of x times 2^(e_m - T), contiguous, and T behind the exponents.  Every workgroup looks for T by itself.  2048 x 3584 10 us.
+// Rows of x times 2^(e_m - T), contiguous, and T behind the exponents.  Every workgroup looks for T by itself, so there are few of them.
+// 2048 x 3584 8 us, 10^6 x 64 113.
 template <int kPer>
-__global__ void __launch_bounds__(256) scale_rows_kernel(const __half* x, int64_t x_stride, __half* out, int* exponents, int64_t rows, int64_t k) {
+__global__ void __launch_bounds__(1024) scale_rows_kernel(const __half* x, int64_t x_stride, __half* out, int* exponents, int64_t rows, int64_t k) {
     struct alignas(sizeof(__half) * kPer) Piece {
         __half v[kPer];
     };
-    __shared__ int tops[4];
+    __shared__ int tops[16];
     int top = 2 * kNoExponent;
-    for (int64_t i = threadIdx.x; i < rows; i += 256) top = max(top, exponents[rows + i]);
+    for (int64_t i = threadIdx.x; i < rows; i += 8 * 1024)
+#pragma unroll
+        for (int j = 0; j < 8; j++) top = max(top, exponents[rows + min(i + j * 1024, rows - 1)]);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) top = max(top, __shfl_xor(top, o));
     if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
     __syncthreads();
-    top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+    for (int w = 0; w < 16; w++) top = max(top, tops[w]);
     if (blockIdx.x == 0 && threadIdx.x == 0) exponents[2 * rows] = top;
-    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    const int64_t pieces = k / kPer, all = rows * pieces;
+    for (int64_t i = (int64_t)blockIdx.x * 1024 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 1024) {
+        int64_t c;
+        const int64_t row = div_index(i, pieces, c);
         const int by = exponents[row] - top;
-        for (int64_t i = (int64_t)threadIdx.x * kPer; i < k; i += 256 * kPer) {
-            Piece v = *reinterpret_cast<const Piece*>(x + row * x_stride + i);
+        Piece v = *reinterpret_cast<const Piece*>(x + row * x_stride + c * kPer);
 #pragma unroll
-            for (int e = 0; e < kPer; e++) v.v[e] = __float2half(__builtin_amdgcn_ldexpf(__half2float(v.v[e]), by));
-            *reinterpret_cast<Piece*>(out + row * k + i) = v;
-        }
+        for (int e = 0; e < kPer; e++) v.v[e] = __float2half(__builtin_amdgcn_ldexpf(__half2float(v.v[e]), by));
+        *reinterpret_cast<Piece*>(out + i * kPer) = v;
     }
 }
 
@@ -434,19 +443,26 @@ int gate_gradient_rows(const float* gate_up, const void* dout, void* grad, const
     };
     const bool pieces = inter % 8 == 0 && aligned({gate_up, dout, grad});
     const int64_t many = pieces ? inter / 8 : inter;
-    const unsigned threads = (unsigned)std::min<int64_t>(kRowThreads, align_up(many, CKV_WAVE));
+    const bool short_rows = many <= 3 * CKV_WAVE;   // what a wavefront holds of a row
+    int lanes_log = 0;
+    while (lanes_log < 6 && (1 << lanes_log) < many) lanes_log++;
+    const unsigned threads = short_rows ? 256 : (unsigned)std::min<int64_t>(kRowThreads, align_up(many, CKV_WAVE));
+    const int64_t here = short_rows ? 256 >> lanes_log : 1, groups = std::min<int64_t>((rows + here - 1) / here, 1 << 22);
     auto launch = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)std::min<int64_t>(rows, 1 << 22)), dim3(threads), 0, stream, gate_up, (const __half*)dout, (__half*)grad, (const __half*)x, x_stride, exponents, rows,
-                           inter, k);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(threads), 0, stream, gate_up, (const __half*)dout, (__half*)grad, (const __half*)x, x_stride, exponents, rows, inter,
+                           k, lanes_log);
     };
-    if (pieces) launch(gate_gradient_rows_kernel<8, 3>);
-    else launch(gate_gradient_rows_kernel<1, 16>);
+    if (pieces && many <= CKV_WAVE) launch(gate_gradient_rows_kernel<8, 1, true>);
+    else if (pieces && short_rows) launch(gate_gradient_rows_kernel<8, 3, true>);
+    else if (pieces) launch(gate_gradient_rows_kernel<8, 3, false>);
+    else if (short_rows) launch(gate_gradient_rows_kernel<1, 3, true>);
+    else launch(gate_gradient_rows_kernel<1, 16, false>);
     CKV_HIP_TRY(hipGetLastError());
     if (!scaled_x) return CKV_OK;
-    const dim3 grid((unsigned)std::min<int64_t>(rows, 2048));
+    const dim3 grid((unsigned)std::min<int64_t>((rows * k + 8191) / 8192, 256));
     if (k % 8 == 0 && x_stride % 8 == 0 && aligned({x, scaled_x}))
-        hipLaunchKernelGGL((scale_rows_kernel<8>), grid, dim3(256), 0, stream, (const __half*)x, x_stride, (__half*)scaled_x, exponents, rows, k);
-    else hipLaunchKernelGGL((scale_rows_kernel<1>), grid, dim3(256), 0, stream, (const __half*)x, x_stride, (__half*)scaled_x, exponents, rows, k);
+        hipLaunchKernelGGL((scale_rows_kernel<8>), grid, dim3(1024), 0, stream, (const __half*)x, x_stride, (__half*)scaled_x, exponents, rows, k);
+    else hipLaunchKernelGGL((scale_rows_kernel<1>), grid, dim3(1024), 0, stream, (const __half*)x, x_stride, (__half*)scaled_x, exponents, rows, k);
     CKV_HIP_TRY(hipGetLastError());
     return CKV_OK;
 }

@@ -159,3 +159,17 @@ def test_the_limit_tells_projections_of_16_bits(dtype):
         d = torch.cat((dh.float() * u * s * (1 + g * (1 - s)), dh.float() * g * s), -1).to(dtype).float()
         many = beyond((d.T @ x.float()).to(dtype), value)
         assert (many > 100) if rounded else many == 0
+
+
+# Rows that a wavefront's lanes share out between several of them, and more rows than one look at the exponents takes
+SHORT = [(65, 40, 24), (1001, 24, 5), (130, 64, 1000), (9, 48, 8), (70001, 16, 16)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", SHORT, ids=str)
+def test_short_rows_in_float16(size):
+    m, k, i = size
+    x, w, dh = inputs(*size, torch.float16, "cuda", seed=5)
+    by = torch.tensor([1.0, 2.0 ** -12, 0.0, 2.0 ** 13, 2.0 ** -20], device="cuda").repeat(m // 5 + 1)[:m, None]
+    for d in (dh * 2e4, dh * 1e-6, dh * by):
+        check(x, w, d.clamp(-65504, 65504).half(), "gradients")
