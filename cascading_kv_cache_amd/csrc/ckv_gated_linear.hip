@@ -679,6 +679,7 @@ extern "C" int ckv_gated_linear_bwd(const void* x, const void* w, const float* g
         return CKV_OK;
     }
     if (!x || !w || !gate_up || !dout) return CKV_ERR_NULL;
+    if (dtype == CKV_F16 && (reinterpret_cast<uintptr_t>(workspace) & 3)) return CKV_ERR_WORKSPACE;   // which exponents lie in
     DeviceInfo di;
     if (int rc = current_device_info(&di)) return rc;
     if (!workspace || workspace_bytes < Scratch(rows, inter, k, dtype).products) return CKV_ERR_WORKSPACE;

@@ -389,7 +389,7 @@ int ckv_norm_rotate_bwd(const ckv_norm_rotate_args* args, void* stream);
  * contiguous.  The backward pass writes dx (rows, k) and dw (2 inter, k), either of which may be NULL; it rounds the
  * gradients of the projections to the tensor dtype for its two products, whose sums are float32; in float16 they are kept
  * times a power of two a row, so that only dx and dw have to be inside its range.  Sums are added up in a
- * fixed order.  The workspace sizes are those of a call on the current device.
+ * fixed order.  The workspace sizes are those of a call on the current device; workspaces are 16-byte aligned.
  * ---------------------------------------------------------------------------------------- */
 int64_t ckv_gated_linear_workspace_bytes(int64_t rows, int64_t inter, int64_t k, int32_t dtype);
 int ckv_gated_linear(const void* x, const void* w, void* out, float* gate_up, int64_t rows, int64_t inter, int64_t k, int64_t x_stride,

@@ -7,6 +7,7 @@ the smallest step, 2^-25, where it is below 2^-14 there: 2^(e - 25) <= 2^-39 of 
 import pytest
 import torch
 
+from cascading_kv_cache_amd import _abi
 from cascading_kv_cache_amd.feed_forward import gated_feed_forward
 
 U = 2.0 ** -24                                   # half a step of float32, relative
@@ -173,3 +174,8 @@ def test_short_rows_in_float16(size):
     by = torch.tensor([1.0, 2.0 ** -12, 0.0, 2.0 ** 13, 2.0 ** -20], device="cuda").repeat(m // 5 + 1)[:m, None]
     for d in (dh * 2e4, dh * 1e-6, dh * by):
         check(x, w, d.clamp(-65504, 65504).half(), "gradients")
+
+
+def test_a_workspace_that_exponents_cannot_lie_in():
+    lib = _abi.lib()
+    assert lib.ckv_gated_linear_bwd(16, 16, 16, 16, 16, 16, 2, 8, 8, 8, _abi.CKV_F16, 18, 1 << 30, None) == -5
