@@ -1,11 +1,13 @@
 """Who follows torch's operations on an operator's inputs, other than for gradients: the operators, which go by address, refuse them, and a decoder's MLP
 takes torch's operations."""
+from dataclasses import replace
+
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 
-from cascading_kv_cache_amd.decoder import PRESETS, GatedMLP
+from cascading_kv_cache_amd.decoder import PRESETS, CascadeDecoder, GatedMLP
 from cascading_kv_cache_amd.feed_forward import gated_feed_forward
 from cascading_kv_cache_amd.norm_rotate import norm_rotate
 from cascading_kv_cache_amd.row_products import followed, followed_beyond_gradients
@@ -157,3 +159,10 @@ def test_a_decoders_mlp_on_the_device():
         for a, b in zip(got, want):
             assert b is not None and torch.allclose(a, b, rtol=1e-4, atol=1e-5)
         assert torch.allclose(torch.jit.trace(fused, x, check_trace=False)(y), fused(y), rtol=1e-4, atol=1e-5)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("hidden,inter,whole", [(256, 512, True), (256, 510, False), (252, 512, False)])
+def test_layers_that_the_operator_is_slow_for_keep_torchs_products(hidden, inter, whole, dtype):
+    model = CascadeDecoder(replace(PRESETS["tiny"], hidden_size=hidden, intermediate_size=inter), dtype, "cpu")
+    assert all(layer.mlp.one_launch == (whole or dtype == torch.float32) for layer in model.fuse_projections(feed_forward=True).layers)
